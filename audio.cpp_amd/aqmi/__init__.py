@@ -34,6 +34,7 @@ EXPORTED = [
     "aq_euclid_encode_strided", "aq_euclid_upload_projected", "aq_euclid_encode_noalloc",
     "aq_dac_encode_ex", "aq_dac_decode_ex", "aq_euclid_upload_device", "aq_weight_norm_fold",
     "aq_linear_upload", "aq_linear_forward", "aq_linear_release",
+    "aq_add_rmsnorm",
 ]
 
 # aq_euclid_recipe / aq_codebook_type
@@ -41,6 +42,8 @@ OMNIVOICE, HIGGS, DIRECT = 0, 1, 2
 # aq_dac_recipe
 DAC_FISH, DAC_INDEXTTS2, DAC_VEVO2, DAC_OUTETTS = 0, 1, 2, 3
 CB_F32, CB_Q8_0, CB_F32_AS_Q8_0 = 0, 1, 2
+# aq_dtype
+T_F32, T_F16, T_BF16, T_I8, T_E4M3 = 0, 1, 2, 3, 4
 
 
 class AqError(RuntimeError):
@@ -84,6 +87,8 @@ def load_library(path: str | pathlib.Path | None = None) -> C.CDLL:
     lib.aq_linear_upload.argtypes = [vp, i64, i64, C.c_int, vp, vp, C.POINTER(vp)]
     lib.aq_linear_forward.argtypes = [vp, vp, vp, i64, i64, i64, i64, i64, vp]
     lib.aq_linear_release.argtypes = [vp]
+    lib.aq_add_rmsnorm.argtypes = [vp, C.c_int, vp, i64, vp, i64, vp, i64, i64, C.c_float, vp, i64, vp, i64, C.c_int,
+                                   i64, vp, vp]
     lib.aq_euclid_decode.argtypes = [vp, vp, vp, i64, vp]
     lib.aq_euclid_encode_noalloc.argtypes = [vp, vp, vp, i64, vp, vp, vp, C.c_int, vp, vp, vp]
     lib.aq_euclid_encode_strided.argtypes = [vp, vp, vp, i64, i64, i64, i64, i64, vp, vp, vp, C.c_int, vp, vp, vp]
@@ -112,6 +117,31 @@ def _dptr(t) -> int | None:
         return None
     assert t.is_cuda and t.is_contiguous(), "device tensors must be contiguous CUDA/HIP tensors"
     return t.data_ptr()
+
+
+def _dtype(t) -> int:
+    """aq_dtype of a torch tensor."""
+    name = str(t.dtype)
+    try:
+        return _DTYPES[name]
+    except KeyError:
+        raise TypeError(f"{name} is no element type of the library") from None
+
+
+_DTYPES = {"torch.float32": T_F32, "torch.float16": T_F16, "torch.bfloat16": T_BF16, "torch.int8": T_I8,
+           "torch.float8_e4m3fn": T_E4M3}
+
+
+def _rows(t, rows: int, cols: int, dtype: int | None = None):
+    """(pointer, row stride) of a device matrix whose row elements are adjacent; (None, 0) of None."""
+    if t is None:
+        return None, 0
+    if not t.is_cuda or t.dim() != 2 or t.shape[0] != rows or t.shape[1] != cols or (cols > 1 and t.stride(1) != 1):
+        raise ValueError(f"expected a device matrix [{rows}, {cols}] with adjacent row elements, got "
+                         f"{tuple(t.shape)} strides {tuple(t.stride())}")
+    if dtype is not None and _dtype(t) != dtype:
+        raise TypeError(f"expected element type {dtype}, got {t.dtype}")
+    return t.data_ptr(), t.stride(0) if rows > 1 else cols
 
 
 class Context:
@@ -481,3 +511,23 @@ def ema_codebook(ctx: Context, embedding_sum, cluster_usage, eps: float, out):
     Q, N, K = embedding_sum.shape
     ctx.use_current_stream()
     ctx.check(ctx.lib.aq_ema_codebook(ctx.h, _dptr(embedding_sum), _dptr(cluster_usage), Q, N, K, eps, _dptr(out)))
+
+
+def add_rmsnorm(ctx: Context, x, weight, eps: float, residual=None, sum=None, y=None, q=None, scale=None,
+                group: int = 0):
+    """aq_add_rmsnorm on device tensors: x, residual, sum, y [M, D] of one
+    floating type (rows may be strided), weight [D] or None; q [M, D] int8 or
+    float8_e4m3fn with scale [M, ceil(D / group)] float32 (group 0: one scale
+    a row)."""
+    M, D = x.shape
+    t = _dtype(x)
+    if weight is not None and (weight.numel() != D or _dtype(weight) != t):
+        raise ValueError(f"weight must hold {D} elements of {x.dtype}")
+    if q is not None:
+        groups = -(-D // group) if group > 0 else 1
+        if scale is None or scale.numel() != M * groups or _dtype(scale) != T_F32 or tuple(q.shape) != (M, D):
+            raise ValueError(f"q needs shape ({M}, {D}) and a float32 scale of ({M}, {groups})")
+    ctx.use_current_stream()
+    ctx.check(ctx.lib.aq_add_rmsnorm(ctx.h, t, *_rows(x, M, D), *_rows(residual, M, D, t), _dptr(weight), M, D, eps,
+                                     *_rows(sum, M, D, t), *_rows(y, M, D, t), T_I8 if q is None else _dtype(q),
+                                     group, _dptr(q), _dptr(scale if q is not None else None)))

@@ -481,6 +481,44 @@ aq_status aq_linear_forward(aq_ctx *ctx, const aq_linear *lin, const float *x, i
                             int64_t clip_stride, int64_t frame_stride, int64_t chan_stride, float *out);
 aq_status aq_linear_release(aq_linear *lin);
 
+/* ---- Answering with codes --------------------------------------------------
+ *
+ * The end of a step of a language model over codes, up to the codes that the
+ * decoders above take.  These operators have no counterpart in the reference
+ * whose bits they would have to give: each says what it computes.
+ *
+ * Rows: row m of a matrix starts at base + m * ld elements; its elements are
+ * adjacent and may start at any element (no alignment beyond the type's). */
+
+/* Element types.  AQ_T_E4M3 is the 8-bit float with 4 exponent and 3 mantissa
+ * bits without infinities (largest value 448). */
+typedef enum aq_dtype { AQ_T_F32 = 0, AQ_T_F16 = 1, AQ_T_BF16 = 2, AQ_T_I8 = 3, AQ_T_E4M3 = 4 } aq_dtype;
+
+/* Root-mean-square norm with the residual's addition and an output in 8 bits:
+ *   h = x + residual              (added in fp32, rounded to the type)
+ *   y = h * weight / sqrt(mean(h*h) + eps)
+ *   scale[m, g] = max |y| of the group's columns / L, L = 127 (I8), 448 (E4M3)
+ *   q = y / scale, to the nearest value of q_type, ties to even
+ * q comes from y before y is rounded to the type.  A group of zeros (or below
+ * 2^-118 times the row's root) has scale 0 and q 0.  A row with a value that
+ * is not finite has the y that the formula gives; the scale of a group whose
+ * y is not finite is NaN.
+ *   type      F32, F16 or BF16: x, residual, weight, sum and y
+ *   x         device [M, D], row stride x_ld (elements, >= D)
+ *   residual  device [M, D], residual_ld, or NULL: h = x
+ *   weight    device [D] or NULL (ones)
+ *   group     columns per scale: 32, 64 or 128, or 0 for one scale a row; the
+ *             last group of a row may be short
+ *   sum       device [M, D], sum_ld, or NULL: h.  May be x or residual.
+ *   y         device [M, D], y_ld, or NULL.  May be x or residual, unless
+ *             sum is the same buffer.
+ *   q_type    I8 or E4M3; q device [M, D] contiguous, or NULL: no 8-bit output
+ *   scale     device [M, ceil(D / group)] (group 0: [M]); with q
+ * Any D from 1 to 2^30.  Sums are held in fp32. */
+aq_status aq_add_rmsnorm(aq_ctx *ctx, int type, const void *x, int64_t x_ld, const void *residual,
+                         int64_t residual_ld, const void *weight, int64_t M, int64_t D, float eps, void *sum,
+                         int64_t sum_ld, void *y, int64_t y_ld, int q_type, int64_t group, void *q, float *scale);
+
 #ifdef __cplusplus
 }
 #endif
