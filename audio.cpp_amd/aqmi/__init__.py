@@ -34,7 +34,7 @@ EXPORTED = [
     "aq_euclid_encode_strided", "aq_euclid_upload_projected", "aq_euclid_encode_noalloc",
     "aq_dac_encode_ex", "aq_dac_decode_ex", "aq_euclid_upload_device", "aq_weight_norm_fold",
     "aq_linear_upload", "aq_linear_forward", "aq_linear_release",
-    "aq_add_rmsnorm",
+    "aq_add_rmsnorm", "aq_q4_upload", "aq_q4_forward", "aq_q4_release",
 ]
 
 # aq_euclid_recipe / aq_codebook_type
@@ -89,6 +89,9 @@ def load_library(path: str | pathlib.Path | None = None) -> C.CDLL:
     lib.aq_linear_release.argtypes = [vp]
     lib.aq_add_rmsnorm.argtypes = [vp, C.c_int, vp, i64, vp, i64, vp, i64, i64, C.c_float, vp, i64, vp, i64, C.c_int,
                                    i64, vp, vp]
+    lib.aq_q4_upload.argtypes = [vp, i64, i64, i64, vp, vp, vp, vp, C.POINTER(vp)]
+    lib.aq_q4_forward.argtypes = [vp, vp, C.c_int, vp, i64, vp, i64, i64, C.c_int, vp, i64]
+    lib.aq_q4_release.argtypes = [vp]
     lib.aq_euclid_decode.argtypes = [vp, vp, vp, i64, vp]
     lib.aq_euclid_encode_noalloc.argtypes = [vp, vp, vp, i64, vp, vp, vp, C.c_int, vp, vp, vp]
     lib.aq_euclid_encode_strided.argtypes = [vp, vp, vp, i64, i64, i64, i64, i64, vp, vp, vp, C.c_int, vp, vp, vp]
@@ -531,3 +534,81 @@ def add_rmsnorm(ctx: Context, x, weight, eps: float, residual=None, sum=None, y=
     ctx.check(ctx.lib.aq_add_rmsnorm(ctx.h, t, *_rows(x, M, D), *_rows(residual, M, D, t), _dptr(weight), M, D, eps,
                                      *_rows(sum, M, D, t), *_rows(y, M, D, t), T_I8 if q is None else _dtype(q),
                                      group, _dptr(q), _dptr(scale if q is not None else None)))
+
+
+def q4_quantize(w: np.ndarray, group: int, zeros: bool = False):
+    """A float32 matrix [out, in] as (codes, scale, zero) of aq_q4_upload, on
+    the host: per row and group of columns a float16 scale (the largest
+    magnitude over 7, or the range over 15 with `zeros`) and each weight's
+    nearest code."""
+    N, K = w.shape
+    groups = -(-K // group)
+    g = np.zeros((N, groups * group), np.float32)
+    g[:, :K] = w
+    g = g.reshape(N, groups, group)
+    if zeros:
+        lo, hi = np.minimum(g.min(2), 0), np.maximum(g.max(2), 0)
+        scale = ((hi - lo) / 15).astype(np.float16)
+    else:
+        scale = (np.abs(g).max(2) / 7).astype(np.float16)
+    inv = np.divide(1, scale, out=np.zeros(scale.shape, np.float32), where=scale > 0, dtype=np.float32)
+    zero = np.clip(np.rint(-lo * inv), 0, 15).astype(np.uint8) if zeros else None
+    codes = np.clip(np.rint(g * inv[:, :, None]) + (zero[:, :, None] if zeros else 8), 0, 15).astype(np.uint8)
+    codes = codes.reshape(N, -1)[:, :K + K % 2]
+    return np.ascontiguousarray(codes[:, 0::2] | codes[:, 1::2] << 4), scale, zero
+
+
+class Q4Linear:
+    """aq_q4: a matrix [out, in_features] with 4-bit weights.
+
+    Host arrays: codes uint8 [out, ceil(in / 2)] (the even column in the low
+    bits), scale float16 [out, ceil(in / group)], zero uint8 like scale or
+    None (8), bias float32 [out] or None."""
+
+    def __init__(self, ctx: Context, codes, scale, in_features: int, group: int, zero=None, bias=None):
+        self.ctx, self.in_features, self.out_features = ctx, in_features, codes.shape[0]
+        if group not in (32, 64, 128):
+            raise ValueError(f"group {group} is not 32, 64 or 128")
+        shape = (self.out_features, -(-in_features // group))
+        if codes.dtype != np.uint8 or codes.shape[1] != (in_features + 1) // 2:
+            raise ValueError(f"codes must be uint8 [out, {(in_features + 1) // 2}]")
+        if scale.dtype != np.float16 or scale.shape != shape or (
+                zero is not None and (zero.dtype != np.uint8 or zero.shape != shape)):
+            raise ValueError(f"scale must be float16 {shape}, zero uint8 {shape}")
+        if bias is not None and bias.shape != (self.out_features,):
+            raise ValueError(f"bias must be float32 ({self.out_features},)")
+        codes, scale = np.ascontiguousarray(codes), np.ascontiguousarray(scale)
+        zero = None if zero is None else np.ascontiguousarray(zero)
+        bias = None if bias is None else np.ascontiguousarray(bias, np.float32)
+        ptr = [None if a is None else a.ctypes.data_as(C.c_void_p) for a in (codes, scale, zero, bias)]
+        h = C.c_void_p()
+        ctx.use_current_stream()
+        ctx.check(ctx.lib.aq_q4_upload(ctx.h, self.out_features, in_features, group, *ptr, C.byref(h)))
+        self.h = h
+
+    def forward(self, x, out, scale=None, group: int = 0):
+        """out [M, out_features] = x [M, in_features] W^T (+ bias); both device
+        matrices of any floating type, rows may be strided.  An int8 or
+        float8_e4m3fn x has a float32 scale [M, ceil(in / group)] (group 0:
+        one a row)."""
+        M, t = x.shape[0], _dtype(x)
+        if t in (T_I8, T_E4M3):
+            groups = -(-self.in_features // group) if group > 0 else 1
+            if scale is None or scale.numel() != M * groups or _dtype(scale) != T_F32:
+                raise ValueError(f"an 8-bit x needs a float32 scale of ({M}, {groups})")
+        elif scale is not None:
+            raise ValueError("scale belongs to an 8-bit x")
+        self.ctx.use_current_stream()
+        self.ctx.check(self.ctx.lib.aq_q4_forward(self.ctx.h, self.h, t, *_rows(x, M, self.in_features), _dptr(scale),
+                                                  group, M, _dtype(out), *_rows(out, M, self.out_features)))
+
+    def close(self):
+        if getattr(self, "h", None):
+            self.ctx.lib.aq_q4_release(self.h)
+            self.h = None
+
+    def __del__(self):
+        try:
+            self.close()
+        except Exception:
+            pass

@@ -519,6 +519,38 @@ aq_status aq_add_rmsnorm(aq_ctx *ctx, int type, const void *x, int64_t x_ld, con
                          int64_t residual_ld, const void *weight, int64_t M, int64_t D, float eps, void *sum,
                          int64_t sum_ld, void *y, int64_t y_ld, int q_type, int64_t group, void *q, float *scale);
 
+/* Products with 4-bit weights and group scales:
+ *   y[m, n] = sum_k x[m, k] * (code[n, k] - zero[n, k / group]) * scale[n, k / group]  (+ bias[n])
+ * x is of a floating type, or an 8-bit row (what aq_add_rmsnorm writes) that
+ * stands for x[m, k] * x_scale[m, k / x_group]. */
+typedef struct aq_q4 aq_q4;
+
+/* Upload a matrix from host memory (once; it is laid out for the kernels on
+ * the device).  The call waits for the layout to be done.
+ *   codes  [out_features, ceil(in_features / 2)]: two codes 0..15 a byte, the
+ *          even column in the low 4 bits
+ *   scale  [out_features, ceil(in_features / group)] F16
+ *   zero   the same shape, one byte each (0..15), or NULL: 8
+ *   bias   [out_features] F32 or NULL
+ *   group  32, 64 or 128 columns per scale; the last group may be short
+ * Any out_features and in_features up to 2^24, 2^34 weights. */
+aq_status aq_q4_upload(aq_ctx *ctx, int64_t out_features, int64_t in_features, int64_t group, const uint8_t *codes,
+                       const void *scale, const uint8_t *zero, const float *bias, aq_q4 **out);
+
+/*   x        device [M, in_features], row stride x_ld (elements), x_type F32,
+ *            F16, BF16, I8 or E4M3
+ *   x_scale  device [M, ceil(in_features / x_group)] for I8 and E4M3 (x_group
+ *            0: [M]); NULL for the others
+ *   x_group  columns per x_scale: 32, 64 or 128, or 0 for one scale a row
+ *   y        device [M, out_features], row stride y_ld, y_type F32, F16 or BF16
+ * Products and sums are fp32, exact whole numbers for I8; an F32 x enters
+ * with all its 24 bits.  A row of x with a value that is not finite (or above
+ * 2^112, where a group's sum may not be) gives a row of NaN.  The order of a
+ * sum depends on M and the matrix alone. */
+aq_status aq_q4_forward(aq_ctx *ctx, const aq_q4 *w, int x_type, const void *x, int64_t x_ld, const float *x_scale,
+                        int64_t x_group, int64_t M, int y_type, void *y, int64_t y_ld);
+aq_status aq_q4_release(aq_q4 *w);
+
 #ifdef __cplusplus
 }
 #endif
