@@ -34,7 +34,7 @@ EXPORTED = [
     "aq_euclid_encode_strided", "aq_euclid_upload_projected", "aq_euclid_encode_noalloc",
     "aq_dac_encode_ex", "aq_dac_decode_ex", "aq_euclid_upload_device", "aq_weight_norm_fold",
     "aq_linear_upload", "aq_linear_forward", "aq_linear_release",
-    "aq_add_rmsnorm", "aq_q4_upload", "aq_q4_forward", "aq_q4_release",
+    "aq_add_rmsnorm", "aq_q4_upload", "aq_q4_forward", "aq_q4_release", "aq_sample",
 ]
 
 # aq_euclid_recipe / aq_codebook_type
@@ -92,6 +92,7 @@ def load_library(path: str | pathlib.Path | None = None) -> C.CDLL:
     lib.aq_q4_upload.argtypes = [vp, i64, i64, i64, vp, vp, vp, vp, C.POINTER(vp)]
     lib.aq_q4_forward.argtypes = [vp, vp, C.c_int, vp, i64, vp, i64, i64, C.c_int, vp, i64]
     lib.aq_q4_release.argtypes = [vp]
+    lib.aq_sample.argtypes = [vp, C.c_int, vp, i64, i64, i64, vp, vp, vp, vp, vp, vp, vp]
     lib.aq_euclid_decode.argtypes = [vp, vp, vp, i64, vp]
     lib.aq_euclid_encode_noalloc.argtypes = [vp, vp, vp, i64, vp, vp, vp, C.c_int, vp, vp, vp]
     lib.aq_euclid_encode_strided.argtypes = [vp, vp, vp, i64, i64, i64, i64, i64, vp, vp, vp, C.c_int, vp, vp, vp]
@@ -612,3 +613,20 @@ class Q4Linear:
             self.close()
         except Exception:
             pass
+
+
+def sample(ctx: Context, logits, u, token, temperature=None, top_k=None, top_p=None, min_p=None, logp=None):
+    """aq_sample on device tensors: logits [rows, V] (rows may be strided); u,
+    temperature, top_p, min_p, logp float32 and top_k, token int32, all of
+    `rows` elements (token may be [B, Q] with B * Q rows)."""
+    rows, V = logits.shape
+    for name, t, want in (("u", u, T_F32), ("temperature", temperature, T_F32), ("top_p", top_p, T_F32),
+                          ("min_p", min_p, T_F32), ("logp", logp, T_F32), ("top_k", top_k, None),
+                          ("token", token, None)):
+        if t is None:
+            continue
+        if t.numel() != rows or str(t.dtype) != ("torch.float32" if want == T_F32 else "torch.int32"):
+            raise ValueError(f"{name} must hold {rows} elements of {'float32' if want == T_F32 else 'int32'}")
+    ctx.use_current_stream()
+    ctx.check(ctx.lib.aq_sample(ctx.h, _dtype(logits), *_rows(logits, rows, V), rows, V, _dptr(u), _dptr(temperature),
+                                _dptr(top_k), _dptr(top_p), _dptr(min_p), _dptr(token), _dptr(logp)))

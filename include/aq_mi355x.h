@@ -551,6 +551,34 @@ aq_status aq_q4_forward(aq_ctx *ctx, const aq_q4 *w, int x_type, const void *x, 
                         int64_t x_group, int64_t M, int y_type, void *y, int64_t y_ld);
 aq_status aq_q4_release(aq_q4 *w);
 
+/* One index per row of logits, drawn with a given random number:
+ *   z[i] = (l[i] - max l) * log2(e) / temperature,  e[i] = 2^z[i]   (fp32)
+ *   w[i] = floor(e[i] * 2^31): whole numbers, so no sum depends on an order
+ *   top-k keeps the k largest logits; top-p of those, in falling order, each
+ *   whose predecessors' weights sum to less than floor(p * sum of what top-k
+ *   kept), and the first; min-p each with e[i] >= min_p.  Of equal logits the
+ *   lower index comes first.
+ *   token = the first index whose running weight (over the kept, in index
+ *   order) exceeds floor(u * kept weight); logp = ln(e[token]) - ln(kept
+ *   weight / 2^31)
+ * u, p and min_p enter as multiples of 2^-24 (u, p; below) and as they are.
+ * A logit of -infinity (or NaN) is never drawn; if a row has no other, its
+ * token is -1 and its logp -infinity.  Where the largest is +infinity, those
+ * that are share the row.
+ *   logits       device [rows, V] of F32, F16 or BF16, row stride ld
+ *   u            device [rows], in [0, 1) (outside: the nearest inside)
+ *   temperature  device [rows] or NULL (1); 0, negative or NaN: the most
+ *                likely index, whatever the filters
+ *   top_k        device [rows] int32 or NULL; 0, negative or >= V: off
+ *   top_p        device [rows] or NULL; >= 1 or NaN: off
+ *   min_p        device [rows] or NULL; <= 0 or NaN: off; above 1 counts as 1
+ *   token        device [rows] int32; [B, Q] codes are rows = B * Q
+ *   logp         device [rows] or NULL
+ * V from 1 to 2^20, rows up to 2^21. */
+aq_status aq_sample(aq_ctx *ctx, int type, const void *logits, int64_t ld, int64_t rows, int64_t V, const float *u,
+                    const float *temperature, const int32_t *top_k, const float *top_p, const float *min_p,
+                    int32_t *token, float *logp);
+
 #ifdef __cplusplus
 }
 #endif
