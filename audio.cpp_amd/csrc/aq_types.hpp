@@ -48,15 +48,16 @@ struct f32 {
     }
 };
 
-// v[0..7] = p[at..at+7], with zeros from column `end` on.
+// v[0..7] = p[at..at+7], with `fill` from column `end` on.
 template <typename T>
-__device__ inline void load8(const typename T::raw *p, int64_t at, int64_t end, float (&v)[8]) {
+__device__ inline void load8(const typename T::raw *p, int64_t at, int64_t end, float (&v)[8],
+                             typename T::raw fill = typename T::raw(0)) {
     typename T::raw r[8];
     if (at + 8 <= end) {
         std::memcpy(r, p + at, sizeof(r));
     } else {
 #pragma unroll
-        for (int i = 0; i < 8; ++i) r[i] = at + i < end ? p[at + i] : typename T::raw(0);
+        for (int i = 0; i < 8; ++i) r[i] = at + i < end ? p[at + i] : fill;
     }
 #pragma unroll
     for (int i = 0; i < 8; ++i) v[i] = T::load(r[i]);
