@@ -140,12 +140,13 @@ def _rows(t, rows: int, cols: int, dtype: int | None = None):
     """(pointer, row stride) of a device matrix whose row elements are adjacent; (None, 0) of None."""
     if t is None:
         return None, 0
-    if not t.is_cuda or t.dim() != 2 or t.shape[0] != rows or t.shape[1] != cols or (cols > 1 and t.stride(1) != 1):
+    strides = t.stride()
+    if not t.is_cuda or t.shape != (rows, cols) or (strides[1] != 1 and cols > 1):
         raise ValueError(f"expected a device matrix [{rows}, {cols}] with adjacent row elements, got "
-                         f"{tuple(t.shape)} strides {tuple(t.stride())}")
-    if dtype is not None and _dtype(t) != dtype:
+                         f"{tuple(t.shape)} strides {strides}")
+    if dtype is not None and _DTYPES.get(str(t.dtype)) != dtype:
         raise TypeError(f"expected element type {dtype}, got {t.dtype}")
-    return t.data_ptr(), t.stride(0) if rows > 1 else cols
+    return t.data_ptr(), strides[0] if rows > 1 else cols
 
 
 class Context:
@@ -159,6 +160,9 @@ class Context:
         self.torch = torch
         self.lib = lib or load_library()
         self.device = device
+        # the current stream's handle, without a Stream object around it where this torch has that call
+        self._raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (
+            lambda d: torch.cuda.current_stream(d).cuda_stream)
         h = C.c_void_p()
         stream = torch.cuda.current_stream(device).cuda_stream
         st = self.lib.aq_ctx_create(device, C.c_void_p(stream), C.byref(h))
@@ -171,8 +175,7 @@ class Context:
             raise AqError(st, self.lib.aq_last_error(self.h).decode())
 
     def use_current_stream(self):
-        s = self.torch.cuda.current_stream(self.device).cuda_stream
-        self.check(self.lib.aq_ctx_set_stream(self.h, C.c_void_p(s)))
+        self.check(self.lib.aq_ctx_set_stream(self.h, self._raw_stream(self.device)))
 
     def synchronize(self):
         self.check(self.lib.aq_ctx_synchronize(self.h))
@@ -620,13 +623,11 @@ def sample(ctx: Context, logits, u, token, temperature=None, top_k=None, top_p=N
     temperature, top_p, min_p, logp float32 and top_k, token int32, all of
     `rows` elements (token may be [B, Q] with B * Q rows)."""
     rows, V = logits.shape
-    for name, t, want in (("u", u, T_F32), ("temperature", temperature, T_F32), ("top_p", top_p, T_F32),
-                          ("min_p", min_p, T_F32), ("logp", logp, T_F32), ("top_k", top_k, None),
-                          ("token", token, None)):
-        if t is None:
-            continue
-        if t.numel() != rows or str(t.dtype) != ("torch.float32" if want == T_F32 else "torch.int32"):
-            raise ValueError(f"{name} must hold {rows} elements of {'float32' if want == T_F32 else 'int32'}")
+    for t, want in ((u, "torch.float32"), (token, "torch.int32"), (temperature, "torch.float32"),
+                    (top_k, "torch.int32"), (top_p, "torch.float32"), (min_p, "torch.float32"),
+                    (logp, "torch.float32")):
+        if t is not None and (t.numel() != rows or str(t.dtype) != want):
+            raise ValueError(f"expected {rows} elements of {want}, got {tuple(t.shape)} of {t.dtype}")
     ctx.use_current_stream()
     ctx.check(ctx.lib.aq_sample(ctx.h, _dtype(logits), *_rows(logits, rows, V), rows, V, _dptr(u), _dptr(temperature),
                                 _dptr(top_k), _dptr(top_p), _dptr(min_p), _dptr(token), _dptr(logp)))

@@ -22,8 +22,9 @@ struct aq_ctx {
     // cascade, 1: per-stage failure counters and lists, 2: projected queries,
     // 3: refine-pass keys, 4: sweep keys and frame norms, 5: gathered
     // strided input rows of a DAC encode, 6: exact values of the frames an
-    // exact scan takes, 7: largest logits and candidates of sampled rows).
-    static constexpr int kScratchSlots = 8;
+    // exact scan takes, 7: largest logits and candidates of sampled rows,
+    // 8: rows of x in operand order).
+    static constexpr int kScratchSlots = 9;
     // Per-stage counters of the last Euclidean encode on this context (in
     // slot 1, or in the no-allocation scratch).
     int32_t *euclid_counts = nullptr;

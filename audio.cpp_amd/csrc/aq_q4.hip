@@ -146,7 +146,7 @@ aq_status aq_q4_forward(aq_ctx *ctx, const aq_q4 *w, int x_type, const void *x, 
                        (long long)x_ld, (long long)w->K, (long long)y_ld, (long long)w->N);
     aq_device_guard g(ctx->device);
     const int xg = eight ? static_cast<int>(x_group) : 0;
-    const aq_q4_impl::args a{w->codes, w->scale, w->zero, w->bias, x, x_scale, y, x_ld, y_ld, static_cast<int>(M),
+    const aq_q4_impl::args a{w->codes, w->scale, w->zero, w->bias, x, x_scale, nullptr, y, x_ld, y_ld, static_cast<int>(M),
                              static_cast<int>(w->N), static_cast<int>(w->K), w->tiles, w->kblocks,
                              static_cast<int>(w->group), xg, xg ? static_cast<int>((w->K + xg - 1) / xg) : 1, y_type};
     switch (x_type) {

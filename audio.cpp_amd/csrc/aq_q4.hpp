@@ -11,6 +11,7 @@ struct args {
     const float *bias;       // [N] or null
     const void *x;
     const float *x_scale;    // [M, x_groups], 8-bit x
+    const float *x_sum;      // of a packed x
     void *y;
     int64_t x_ld, y_ld;
     int M, N, K, tiles, kblocks, group, x_group, x_groups, y_type;

@@ -300,7 +300,7 @@ struct row_list {
                 uint64_t ahead = 0;
                 for (uint32_t i = 0; i < n; ++i) {
                     const uint32_t ki = lane_value(k, i), ai = lane_value(at, i);
-                    ahead += (ki > k) | ((ki == k) & (ai < at)) ? lane_value(amount, i) : 0u;
+                    ahead += ((ki > k) | ((ki == k) & (ai < at))) ? lane_value(amount, i) : 0u;
                 }
                 const int last = __builtin_ctzll(__ballot((ahead < need) & (ahead + amount >= need)));
                 K = lane_value(k, last);
@@ -314,7 +314,7 @@ struct row_list {
         }
         // More than 64 equal logits cross: the first of them in index order.
         const uint32_t equal = lo;
-        const auto one = [&](int e) { return (key[e] == equal) & kept(e) ? 1u : 0u; };
+        const auto one = [&](int e) { return ((key[e] == equal) & kept(e)) ? 1u : 0u; };
         uint64_t each = 1;
         if (by_weight) each = uniform(s.weight[0]);
         const uint64_t count = (need + each - 1) / each;
@@ -688,7 +688,7 @@ struct row_stream {
                 uint64_t ahead = 0;
                 for (uint32_t i = 0; i < n; ++i) {
                     const uint32_t ki = lane_value(k, i), ai = lane_value(at, i);
-                    ahead += (ki > k) | ((ki == k) & (ai < at)) ? lane_value(amount, i) : 0u;
+                    ahead += ((ki > k) | ((ki == k) & (ai < at))) ? lane_value(amount, i) : 0u;
                 }
                 const int last = __builtin_ctzll(__ballot((ahead < need) & (ahead + amount >= need)));
                 K = lane_value(k, last);
@@ -703,7 +703,7 @@ struct row_stream {
         const uint32_t equal = lo;
         const uint64_t each_one = by_weight ? uniform(s.weight[0]) : 1u;
         const uint64_t count = (need + each_one - 1) / each_one;
-        const auto one = [&](uint32_t key, int i) -> uint64_t { return (key == equal) & kept(key, i) ? 1u : 0u; };
+        const auto one = [&](uint32_t key, int i) -> uint64_t { return ((key == equal) & kept(key, i)) ? 1u : 0u; };
         total(one);
         first_over(one, count - 1, [&](uint32_t, int i) { s.chosen = static_cast<uint32_t>(i); });
         __syncthreads();
@@ -830,7 +830,7 @@ __global__ __launch_bounds__(1024) void sample_row_kernel(sample_args a, chunk_s
     }
     const auto amount = [&](uint32_t key, int i) -> uint64_t {
         const float e = e_of(logit_of(key), top, p.per);
-        return (key != 0) & stream.kept(key, i) & (e >= p.min_e) ? w_of(e) : 0u;
+        return ((key != 0) & stream.kept(key, i) & (e >= p.min_e)) ? w_of(e) : 0u;
     };
     const uint64_t total = stream.total(amount);
     stream.first_over(amount, share(p.u, total), [&](uint32_t key, int i) {

@@ -48,6 +48,10 @@ struct f32 {
     }
 };
 
+__device__ inline uint32_t bits_of(float v) { return __float_as_uint(v); }
+__device__ inline uint32_t bits_of(uint16_t v) { return v; }
+__device__ inline uint32_t bits_of(uint8_t v) { return v; }
+
 // v[0..7] = p[at..at+7], with `fill` from column `end` on.
 template <typename T>
 __device__ inline void load8(const typename T::raw *p, int64_t at, int64_t end, float (&v)[8],
