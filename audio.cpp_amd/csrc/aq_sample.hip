@@ -57,14 +57,25 @@ __device__ inline uint64_t share(uint32_t part, uint64_t total) {
     return __umul64hi(static_cast<uint64_t>(part) << 39, total << 1);
 }
 
-__device__ inline float z_of(float l, float top, float per) { return (l == top ? 0.0f : l - top) * per; }
+// log2 of a logit's weight relative to the largest.  (A row whose largest is
+// +infinity is mapped to 0 and -infinity first: finite_of.)
+__device__ inline float z_of(float l, float top, float per) { return (l - top) * per; }
 
-// e of a logit; 0 for -infinity and NaN.
-__device__ inline float e_of(float l, float top, float per) {
-    return l > -INFINITY ? __builtin_amdgcn_exp2f(z_of(l, top, per)) : 0.0f;
+__device__ inline float e_of(float z) { return __builtin_amdgcn_exp2f(z); }
+
+// To a whole number, downwards; a NaN or a negative number to 0.
+__device__ inline uint32_t whole_of(float v) {
+    uint32_t r;
+    asm("v_cvt_u32_f32 %0, %1" : "=v"(r) : "v"(v));
+    return r;
 }
 
-__device__ inline uint32_t w_of(float e) { return static_cast<uint32_t>(e * 0x1p31f); }
+__device__ inline uint32_t w_of(float z) { return whole_of(e_of(z) * 0x1p31f); }
+
+__device__ inline bool is_infinite(float top) { return !(top < INFINITY); }
+
+// A logit of a row whose largest is +infinity, the largest being 0 then.
+__device__ inline float finite_of(float l) { return l == INFINITY ? 0.0f : -INFINITY; }
 
 // ln(2^z / (total / 2^31)), rounded once: the two terms may nearly cancel, or
 // the second be many times the first.
@@ -80,12 +91,6 @@ __device__ inline uint32_t key_of(float l) {
 
 __device__ inline float logit_of(uint32_t key) {
     return __uint_as_float(key & 0x80000000u ? key ^ 0x80000000u : ~key);
-}
-
-// The weight of a key; 0 for key 0 (no element).
-__device__ inline uint32_t weight_of(uint32_t key, float top, float per) {
-    const uint32_t w = w_of(e_of(logit_of(key), top, per));   // key 0 is a NaN: 0
-    return key ? w : 0;
 }
 
 // Lane i gets lane i - n's value (rows of 16: n = 1, 2, 4, 8), or the last of
@@ -124,6 +129,15 @@ __device__ inline uint64_t lane_value(uint64_t v, int lane) {
 // A value that all lanes hold, as a scalar.
 __device__ inline uint32_t uniform(uint32_t v) { return static_cast<uint32_t>(__builtin_amdgcn_readfirstlane(static_cast<int>(v))); }
 
+__device__ inline uint32_t wave_scan(uint32_t v) {
+    v += dpp<0x111, 0xF>(v);
+    v += dpp<0x112, 0xF>(v);
+    v += dpp<0x114, 0xF>(v);
+    v += dpp<0x118, 0xF>(v);
+    v += dpp<0x142, 0xA>(v);
+    return v + dpp<0x143, 0xC>(v);
+}
+
 __device__ inline uint64_t wave_total(uint64_t v) { return lane_value(wave_scan(v), 63); }
 
 // The largest key of the wave (0 is below every key).
@@ -143,33 +157,67 @@ __device__ inline uint32_t wave_max(uint32_t v) {
 // is no element, or one that is never drawn; `w` is the weight.  Every wave
 // takes every decision for itself from what lies in LDS, so a step needs no
 // barrier for its result.
+//
+// The filters.  256 bins by weight (of count and weight at once: 15 bits and
+// 46 of a word); the bin where the running count or weight crosses what is
+// needed holds the end of the kept prefix.  If it has at most 64 elements, a
+// wave orders them by comparing all pairs; else it is divided again, in bins
+// linear in the key, which tells any two different logits apart after at most
+// four times; more than 64 equal ones are counted off in index order.
+constexpr int kCountShift = 48;
+constexpr uint64_t kWeightMask = (uint64_t{1} << kCountShift) - 1;
+
 template <int WAVES>
 struct list_lds {
     uint64_t bins[256];
     uint64_t part[WAVES];
-    uint32_t key[64], index[64], weight[64];
-    uint32_t count, hi, lo, at;
+    uint32_t key[2][64], index[2][64], weight[2][64];
+    uint32_t count[2], hi[2], lo[2], at, each;
 };
 
 template <int WAVES, int E, bool GIVEN = false>   // GIVEN: the elements bring their indices
 struct row_list {
     static constexpr int kThreads = 64 * WAVES;
+    static constexpr int kNoBin = 256;
     list_lds<WAVES> &s;
     const int lane = threadIdx.x & 63, wave = static_cast<int>(uniform(threadIdx.x >> 6));
-    uint32_t key[E], w[E];
+    uint32_t key[E], w[E], bin[E];
     uint32_t given[GIVEN ? E : 1];
     uint32_t K = 1, I = 0xFFFFFFFFu;   // kept: key > K, or key == K and index <= I
 
-    __device__ explicit row_list(list_lds<WAVES> &lds) : s(lds) {}
+    // Clears the bins: a barrier has to follow before filter().
+    __device__ explicit row_list(list_lds<WAVES> &lds) : s(lds) {
+        clear();
+        if (threadIdx.x < 2) {
+            s.count[threadIdx.x] = 0;
+            s.hi[threadIdx.x] = 0;
+            s.lo[threadIdx.x] = 0xFFFFFFFFu;
+        }
+    }
+
+    __device__ void clear() {
+#pragma unroll
+        for (int b = 0; b < 256; b += kThreads)
+            if (b + threadIdx.x < 256) s.bins[b + threadIdx.x] = 0;
+    }
 
     __device__ uint32_t place(int e) const {   // in the list
         return static_cast<uint32_t>(((wave * (E / 8) + e / 8) * 64 + lane) * 8 + e % 8);
     }
     __device__ uint32_t index(int e) const { return GIVEN ? given[e] : place(e); }
+
     // No branches in the tests of elements: they are a few comparisons, and
     // ROCm 7.2's compiler has dropped the copy of a 64-bit value that a
     // short-circuit left to one of its paths.
     __device__ bool kept(int e) const { return (key[e] > K) | ((key[e] == K) & (index(e) <= I)); }
+
+    // Element e: its bin is (-z - z0) * scale.
+    __device__ void set(int e, float l, float top, float per, float z0, float scale) {
+        const float z = z_of(l, top, per);
+        w[e] = w_of(z);
+        key[e] = w[e] ? key_of(l) : 0;
+        bin[e] = min(whole_of((-z - z0) * scale), 255u);
+    }
 
     // Each wave's sum of `mine` in s.part; the sum over the block.
     __device__ uint64_t total(uint64_t mine) {
@@ -184,11 +232,11 @@ struct row_list {
         return sum;
     }
 
-    // After total() of amount(e) summed over each thread's elements: `hit`
-    // runs in the thread of the first element where the running sum in index
-    // order exceeds t.
-    template <typename A, typename H>
-    __device__ void first_over(A &&amount, uint64_t t, uint64_t mine, H &&hit) {
+    // After total() of amount(e) summed over each thread's elements: true in
+    // the thread of the first element where the running sum in index order
+    // exceeds t, with its index and key.
+    template <typename A>
+    __device__ bool first_over(A &&amount, uint64_t t, uint64_t mine, uint32_t &its_index, uint32_t &its_key) {
         uint64_t before = 0;
         if (WAVES > 1) {
             for (int i = 0; i < wave; ++i) before += s.part[i];
@@ -196,136 +244,210 @@ struct row_list {
         } else {
             mine = wave_total(mine);
         }
-        if (t < before || t >= before + mine) return;   // not in this wave
+        if (t < before || t >= before + mine) return false;   // not in this wave
+        bool found = false;
 #pragma unroll
         for (int v = 0; v < E / 8; ++v) {
             uint64_t eight = 0;
 #pragma unroll
             for (int i = 0; i < 8; ++i) eight += amount(8 * v + i);
             const uint64_t upto = before + wave_scan(eight);
-            const uint64_t over = __ballot(upto > t);
-            if (over && t >= before) {
-                if (lane == __builtin_ctzll(over)) {
-                    uint64_t sum = upto - eight;
-                    bool found = false;
+            uint64_t sum = upto - eight;
 #pragma unroll
-                    for (int i = 0; i < 8; ++i) {
-                        sum += amount(8 * v + i);
-                        if (!found && sum > t) {
-                            found = true;
-                            hit(8 * v + i);
-                        }
-                    }
-                }
+            for (int i = 0; i < 8; ++i) {
+                const uint64_t next = sum + amount(8 * v + i);
+                const bool at = (sum <= t) & (next > t);   // one element of one lane
+                its_index = at ? index(8 * v + i) : its_index;
+                its_key = at ? key[8 * v + i] : its_key;
+                found |= at;
+                sum = next;
             }
             before = lane_value(upto, 63);
         }
+        return found;
     }
 
-    // Narrows the kept set to its shortest prefix (logit falling, index
-    // rising) whose amounts (1, or the weights) reach `need` >= 1; leaves it
-    // if they do not.
-    //
-    // 256 bins of the elements in question; the bin where the running amount
-    // crosses `need` is what remains in question, until it holds at most 64
-    // elements, which a wave orders by comparing all pairs.  The first bins
-    // are an eighth of a bit of weight wide (`per`: bits per unit of logit), so
-    // that a usual row needs no others; the next ones are linear in the key,
-    // which tells any two different logits apart after three more.
-    __device__ void select(bool by_weight, uint64_t need, float top, float per) {
-        uint32_t hi = 0xFFFFFFFFu, lo = 1;
-        int shift = -1;   // of the key, from the second level on
-        const float scale = fminf(8.0f * per, 3.4e38f);
-        for (;;) {
-            __syncthreads();
-            for (int b = threadIdx.x; b < 256; b += kThreads) s.bins[b] = 0;
-            if (threadIdx.x == 0) {
-                s.count = 0;
-                s.hi = 0;
-                s.lo = 0xFFFFFFFFu;
-            }
-            __syncthreads();
-            uint32_t bin[E];
+    // Puts the end of the kept prefix into bin `chosen`, where `need` of the
+    // amounts (1, or the weights) are still to come; returns the weight kept
+    // of that bin.  `phase`: 0 and 1, each once after a clear.
+    __device__ uint64_t resolve(uint32_t chosen, int phase, bool by_weight, uint64_t need) {
 #pragma unroll
-            for (int e = 0; e < E; ++e) {
-                bin[e] = 256;
-                uint32_t b;
-                if (shift < 0) {
-                    const float l = logit_of(key[e]);
-                    b = static_cast<uint32_t>(fminf((l == top ? 0.0f : top - l) * scale, 255.0f));
-                } else {
-                    b = (hi - key[e]) >> shift;
-                }
-                if ((key[e] >= lo) & (key[e] <= hi) & kept(e)) bin[e] = b;
-                if (bin[e] < 256) atomicAdd(reinterpret_cast<unsigned long long *>(&s.bins[bin[e]]), by_weight ? w[e] : 1u);
+        for (int e = 0; e < E; ++e) {
+            if ((bin[e] != chosen) | !kept(e)) continue;
+            const uint32_t at = atomicAdd(&s.count[phase], 1u);
+            if (at < 64) {
+                s.key[phase][at] = key[e];
+                s.index[phase][at] = index(e);
+                s.weight[phase][at] = w[e];
+            } else {
+                atomicMax(&s.hi[phase], key[e]);
+                atomicMin(&s.lo[phase], key[e]);
+            }
+        }
+        __syncthreads();
+        const uint32_t n = uniform(s.count[phase]);
+        if (n <= 64) return order(phase, n, by_weight, need);
+        const uint32_t k = s.key[phase][lane];
+        refine(by_weight, need, max(uniform(s.hi[phase]), wave_max(k)), min(uniform(s.lo[phase]), ~wave_max(~k)));
+        uint64_t mine = 0;
+#pragma unroll
+        for (int e = 0; e < E; ++e) mine += ((bin[e] == chosen) & kept(e)) ? w[e] : 0u;
+        return by_weight ? 0 : total(mine);
+    }
+
+    // The end of the kept prefix among the n <= 64 elements of the short list.
+    __device__ uint64_t order(int phase, uint32_t n, bool by_weight, uint64_t need) {
+        const bool there = static_cast<uint32_t>(lane) < n;
+        const uint32_t k = there ? s.key[phase][lane] : 0, at = there ? s.index[phase][lane] : 0;
+        const uint32_t weight = there ? s.weight[phase][lane] : 0;
+        uint64_t ahead_w = weight;
+        uint32_t ahead = 1;
+        for (uint32_t i = 0; i < n; ++i) {
+            const uint32_t ki = lane_value(k, i), ai = lane_value(at, i), wi = lane_value(weight, i);
+            const bool first = (ki > k) | ((ki == k) & (ai < at));
+            ahead_w += first ? wi : 0u;
+            ahead += first ? 1u : 0u;
+        }
+        // Through this element; the last one kept is the first that reaches `need`.
+        const uint64_t through = by_weight ? ahead_w : ahead, before = through - (by_weight ? weight : 1u);
+        const int last = __builtin_ctzll(__ballot(there & (before < need) & (through >= need)));
+        K = lane_value(k, last);
+        I = lane_value(at, last);
+        return lane_value(ahead_w, last);
+    }
+
+    // The same for more than 64 elements, the kept ones with keys from lo to hi.
+    __device__ void refine(bool by_weight, uint64_t need, uint32_t hi, uint32_t lo) {
+        while (hi != lo) {
+            const int shift = max(0, 24 - __builtin_clz(hi - lo));
+            __syncthreads();
+            clear();
+            if (threadIdx.x == 0) {
+                s.count[0] = 0;
+                s.hi[0] = 0;
+                s.lo[0] = 0xFFFFFFFFu;
             }
             __syncthreads();
-            uint64_t four[4], sum = 0;   // bins 4 lane ..+3, the largest logits first
+#pragma unroll
+            for (int e = 0; e < E; ++e)
+                if ((key[e] >= lo) & (key[e] <= hi) & kept(e))
+                    atomicAdd(reinterpret_cast<unsigned long long *>(&s.bins[(hi - key[e]) >> shift]),
+                              by_weight ? w[e] : 1u);
+            __syncthreads();
+            uint64_t four[4], sum = 0;
 #pragma unroll
             for (int b = 0; b < 4; ++b) sum += four[b] = s.bins[4 * lane + b];
             const uint64_t upto = wave_scan(sum);
-            const uint64_t over = __ballot(upto >= need);
-            if (!over) return;   // on the first level only
-            const int owner = __builtin_ctzll(over);
+            const int owner = __builtin_ctzll(__ballot(upto >= need));
             uint64_t before = upto - sum;
-            uint32_t b = 0;
+            uint32_t b = 4 * lane;
 #pragma unroll
-            for (int i = 0; i < 3; ++i)
-                if (b == static_cast<uint32_t>(i) && before + four[i] < need) {
-                    before += four[i];
-                    ++b;
-                }
-            const uint32_t chosen = 4 * owner + lane_value(b, owner);
+            for (int i = 0; i < 3; ++i) {
+                const bool on = (b == static_cast<uint32_t>(4 * lane + i)) & (before + four[i] < need);
+                before += on ? four[i] : 0u;
+                b += on ? 1u : 0u;
+            }
+            const uint32_t chosen = lane_value(b, owner);
             need -= lane_value(before, owner);
-            // The bin's elements: the first 64 into the short list, and their range.
 #pragma unroll
             for (int e = 0; e < E; ++e) {
-                if (bin[e] != chosen) continue;
-                const uint32_t at = atomicAdd(&s.count, 1u);
+                if (!((key[e] >= lo) & (key[e] <= hi) & kept(e)) || (hi - key[e]) >> shift != chosen) continue;
+                const uint32_t at = atomicAdd(&s.count[0], 1u);
                 if (at < 64) {
-                    s.key[at] = key[e];
-                    s.index[at] = index(e);
-                    s.weight[at] = by_weight ? w[e] : 1u;
+                    s.key[0][at] = key[e];
+                    s.index[0][at] = index(e);
+                    s.weight[0][at] = w[e];
                 } else {
-                    atomicMax(&s.hi, key[e]);
-                    atomicMin(&s.lo, key[e]);
+                    atomicMax(&s.hi[0], key[e]);
+                    atomicMin(&s.lo[0], key[e]);
                 }
             }
             __syncthreads();
-            const uint32_t n = uniform(s.count);
-            const uint32_t k = static_cast<uint32_t>(lane) < n ? s.key[lane] : 0;
+            const uint32_t n = uniform(s.count[0]);
             if (n <= 64) {
-                const uint32_t at = static_cast<uint32_t>(lane) < n ? s.index[lane] : 0;
-                const uint32_t amount = static_cast<uint32_t>(lane) < n ? s.weight[lane] : 0;
-                uint64_t ahead = 0;
-                for (uint32_t i = 0; i < n; ++i) {
-                    const uint32_t ki = lane_value(k, i), ai = lane_value(at, i);
-                    ahead += ((ki > k) | ((ki == k) & (ai < at))) ? lane_value(amount, i) : 0u;
-                }
-                const int last = __builtin_ctzll(__ballot((ahead < need) & (ahead + amount >= need)));
-                K = lane_value(k, last);
-                I = lane_value(at, last);
+                order(0, n, by_weight, need);
                 return;
             }
-            hi = max(uniform(s.hi), wave_max(k));
-            lo = min(uniform(s.lo), ~wave_max(~k));
-            if (hi == lo) break;
-            shift = max(0, 24 - __builtin_clz(hi - lo));
+            const uint32_t k = s.key[0][lane];
+            hi = max(uniform(s.hi[0]), wave_max(k));
+            lo = min(uniform(s.lo[0]), ~wave_max(~k));
         }
-        // More than 64 equal logits cross: the first of them in index order.
+        // Equal logits: the first of them in index order.
+        uint64_t mine = 0;
+        uint32_t some = 0;
         const uint32_t equal = lo;
         const auto one = [&](int e) { return ((key[e] == equal) & kept(e)) ? 1u : 0u; };
-        uint64_t each = 1;
-        if (by_weight) each = uniform(s.weight[0]);
-        const uint64_t count = (need + each - 1) / each;
-        uint64_t mine = 0;
 #pragma unroll
-        for (int e = 0; e < E; ++e) mine += one(e);
+        for (int e = 0; e < E; ++e) {
+            mine += one(e);
+            some = max(some, one(e) ? w[e] : 0u);
+        }
+        uint64_t each = 1;
+        if (by_weight) {   // their weight, from whoever has one
+            if (some) s.each = some;
+        }
         total(mine);
-        first_over(one, count - 1, mine, [&](int e) { s.at = index(e); });
+        if (by_weight) {
+            if (WAVES == 1) __syncthreads();
+            each = uniform(s.each);
+        }
+        uint32_t at = 0, unused = 0;
+        if (first_over(one, (need + each - 1) / each - 1, mine, at, unused)) s.at = at;
         __syncthreads();
         K = equal;
         I = uniform(s.at);
+    }
+
+    // Top-k (k > 0), then top-p of the weight that leaves (p < 2^24), or
+    // until `need` > 0 of the weight is reached.
+    __device__ void filter(uint32_t k, uint32_t p, uint64_t need) {
+#pragma unroll
+        for (int e = 0; e < E; ++e)
+            if (key[e])
+                atomicAdd(reinterpret_cast<unsigned long long *>(&s.bins[bin[e]]),
+                          (uint64_t{1} << kCountShift) + w[e]);
+        __syncthreads();
+        uint64_t w4[4], w_sum = 0;
+        uint32_t n4[4], n_sum = 0;
+#pragma unroll
+        for (int b = 0; b < 4; ++b) {   // bins 4 lane ..+3, the largest logits first
+            const uint64_t v = s.bins[4 * lane + b];
+            w_sum += w4[b] = v & kWeightMask;
+            n_sum += n4[b] = static_cast<uint32_t>(v >> kCountShift);
+        }
+        const uint32_t n_upto = wave_scan(n_sum);
+        const uint64_t w_upto = wave_scan(w_sum);
+        uint64_t weight = lane_value(w_upto, 63);   // kept
+        const uint64_t over_n = k ? __ballot(n_upto >= k) : 0;
+        if (over_n) {
+            const int owner = __builtin_ctzll(over_n);
+            uint32_t n = n_upto - n_sum, b = 4 * lane;
+            uint64_t before = w_upto - w_sum;
+#pragma unroll
+            for (int i = 0; i < 3; ++i) {
+                const bool on = (b == static_cast<uint32_t>(4 * lane + i)) & (n + n4[i] < k);
+                n += on ? n4[i] : 0u;
+                before += on ? w4[i] : 0u;
+                b += on ? 1u : 0u;
+            }
+            weight = lane_value(before, owner) + resolve(lane_value(b, owner), 0, false, k - lane_value(n, owner));
+        }
+        if (p < 1u << 24) need = max(share(p, weight), uint64_t{1});
+        if (need) {
+            // (The sums of bins behind top-k's end are too large, but it is crossed before.)
+            const uint64_t over = __ballot(w_upto >= need);
+            if (!over) return;
+            const int owner = __builtin_ctzll(over);
+            uint64_t before = w_upto - w_sum;
+            uint32_t b = 4 * lane;
+#pragma unroll
+            for (int i = 0; i < 3; ++i) {
+                const bool on = (b == static_cast<uint32_t>(4 * lane + i)) & (before + w4[i] < need);
+                before += on ? w4[i] : 0u;
+                b += on ? 1u : 0u;
+            }
+            resolve(lane_value(b, owner), 1, true, need - lane_value(before, owner));
+        }
     }
 
     __device__ uint64_t kept_weight() const {   // this thread's
@@ -335,30 +457,45 @@ struct row_list {
         return mine;
     }
 
-    // Draws from what is kept and is not below min-p, and writes the outputs.
-    __device__ void draw(const sample_args &a, int64_t row, const row_params &r, float top) {
+    // The weights of what is not kept, or is below min-p, to 0; this thread's sum.
+    __device__ uint64_t drop(float min_e, float top, float per) {
         uint64_t mine = 0;
 #pragma unroll
         for (int e = 0; e < E; ++e) {
             w[e] = kept(e) ? w[e] : 0u;
-            if (r.min_e > 0.0f) w[e] = e_of(logit_of(key[e]), top, r.per) >= r.min_e ? w[e] : 0u;
+            if (min_e > 0.0f) w[e] = e_of(z_of(logit_of(key[e]), top, per)) >= min_e ? w[e] : 0u;
             mine += w[e];
         }
-        const uint64_t sum = total(mine);
-        first_over([&](int e) { return w[e]; }, share(r.u, sum), mine, [&](int e) {
-            a.token[row] = static_cast<int32_t>(index(e));
-            if (a.logp) a.logp[row] = logp_of(z_of(logit_of(key[e]), top, r.per), sum);
-        });
+        return mine;
+    }
+
+    // Draws among the weights and writes the outputs: from all of them, or
+    // (sum > 0) as a part of a row whose kept weight is `sum`, t into this part.
+    __device__ void draw(const sample_args &a, int64_t row, const row_params &r, float top, uint64_t mine, uint64_t sum,
+                         uint64_t t) {
+        const uint64_t all = total(mine);
+        if (!sum) {
+            sum = all;
+            t = share(r.u, sum);
+        }
+        uint32_t at = 0, its_key = 0;
+        if (!first_over([&](int e) { return w[e]; }, t, mine, at, its_key)) return;
+        a.token[row] = static_cast<int32_t>(at);
+        if (a.logp) a.logp[row] = logp_of(z_of(logit_of(its_key), top, r.per), sum);
     }
 };
 
-// 8 logits of a row as keys, 0 for those that are never drawn (or past the end).
+// 8 logits of a row, -infinity past the end.
 template <typename T>
-__device__ inline void load_keys(const typename T::raw *logits, int at, int V, uint32_t *key) {
-    float l[8];
+__device__ inline void load_logits(const typename T::raw *logits, int at, int V, float (&l)[8]) {
     load8<T>(logits, at, V, l, T::store(-INFINITY));
+}
+
+__device__ inline uint32_t largest_key(const float (&l)[8]) {
+    float top = l[0];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) key[i] = l[i] > -INFINITY ? key_of(l[i]) : 0;
+    for (int i = 1; i < 8; ++i) top = fmaxf(top, l[i]);   // not a NaN, unless there is no other
+    return top > -INFINITY ? key_of(top) : 0;
 }
 
 __device__ inline void write_empty(const sample_args &a, int64_t row) {
@@ -374,67 +511,69 @@ __global__ __launch_bounds__(64 * WAVES) void sample_short_kernel(sample_args a)
     const int64_t row = blockIdx.x;
     const raw *logits = static_cast<const raw *>(a.logits) + row * a.ld;
     row_list<WAVES, E> list(lds);
+    float l[E / 8][8];
     uint32_t top_key = 0;
 #pragma unroll
-    for (int v = 0; v < E / 8; ++v) load_keys<T>(logits, static_cast<int>(list.index(8 * v)), a.V, list.key + 8 * v);
-#pragma unroll
-    for (int e = 0; e < E; ++e) top_key = max(top_key, list.key[e]);
+    for (int v = 0; v < E / 8; ++v) load_logits<T>(logits, static_cast<int>(list.place(8 * v)), a.V, l[v]);
     const row_params r = params_of(a, row);
+#pragma unroll
+    for (int v = 0; v < E / 8; ++v) top_key = max(top_key, largest_key(l[v]));
     top_key = wave_max(top_key);
+    if (list.lane == 0) lds.part[list.wave] = top_key;
+    __syncthreads();
     if (WAVES > 1) {
-        if (list.lane == 0) lds.part[list.wave] = top_key;
-        __syncthreads();
 #pragma unroll
         for (int i = 0; i < WAVES; ++i) top_key = max(top_key, static_cast<uint32_t>(lds.part[i]));
+        top_key = uniform(top_key);
     }
     if (!top_key) {
         if (threadIdx.x == 0) write_empty(a, row);
         return;
     }
-    const float top = logit_of(top_key);
+    float top = logit_of(top_key);
+    if (is_infinite(top)) {
+        top = 0.0f;
 #pragma unroll
-    for (int e = 0; e < E; ++e) {
-        list.w[e] = weight_of(list.key[e], top, r.per);
-        if (!list.w[e]) list.key[e] = 0;
+        for (int e = 0; e < E; ++e) l[e / 8][e % 8] = finite_of(l[e / 8][e % 8]);
     }
-    if (r.k) list.select(false, r.k, top, r.per);
-    if (r.p < 1u << 24) {
-        const uint64_t need = share(r.p, list.total(list.kept_weight()));
-        list.select(true, need ? need : 1, top, r.per);
-    }
-    list.draw(a, row, r, top);
+#pragma unroll
+    for (int e = 0; e < E; ++e) list.set(e, l[e / 8][e % 8], top, r.per, 0.0f, 8.0f);
+    if (r.k || r.p < 1u << 24) list.filter(r.k, r.p, 0);
+    list.draw(a, row, r, top, list.drop(r.min_e, top, r.per), 0, 0);
 }
 
 // Longer rows: chunks of 4096 elements, a block each, in three launches.
 //
 //  1. the largest logit of each chunk;
-//  2. the weights, relative to the row's largest; their sum over the chunk;
-//     and, for rows with filters, the chunk's candidates: the elements of its
-//     largest logits, in index order, as many whole half-bits of weight as fit
-//     its slots;
+//  2. the weights, relative to the row's largest, and their sum over the
+//     chunk; for rows with filters also the chunk's count and weight per
+//     half-bit of weight, and its candidates: the elements of its largest
+//     half-bits, in index order, as many whole ones as fit its slots;
 //  3. a block per row.  Without filters it finds the chunk that the draw falls
 //     into from the sums, and draws in it.  With filters it works on the
 //     candidates down to the least half-bit that every chunk has given whole,
-//     which holds the kept set unless that is very wide; else it streams the
-//     row.
+//     which hold the kept set unless that is wide.  A wide one ends, without
+//     top-k, in a half-bit that the sums tell: its elements are collected from
+//     the chunks and decide where, and the sums over what lies above it decide
+//     the chunk to draw in.  What is left (a top-k of thousands, min-p's end
+//     in a wide set, more than 8192 elements in half a bit) streams the row.
 constexpr int kChunk = 4096;          // 256 threads, 16 elements each
 constexpr int kSlots = 8192;          // candidates of a row: 1024 threads, 8 each
-constexpr int kRowsAtOnce = 1024;
+constexpr int kMostChunks = kMaxV / kChunk;
+constexpr int kRowsAtOnce = 256;
 
 struct chunk_store {
-    uint32_t *top;      // [rows][chunks] largest key
+    uint64_t *bins;     // [rows][chunks][64] count and weight of each half-bit, as kCountShift has them
     uint64_t *weight;   // [rows][chunks] sum of weights (of those that min-p leaves, for rows without other filters)
-    int32_t *whole;     // [rows][chunks] the last half-bit given whole, -1: none
+    uint2 *slot;        // [rows][chunks][cap] logit's bits, index
+    uint32_t *top;      // [rows][chunks] largest key
     uint32_t *count;    // [rows][chunks] candidates
-    uint2 *slot;        // [rows][chunks][cap] key, index
+    int32_t *whole;     // [rows][chunks] the last half-bit given whole, -1: none
     int chunks, cap;
 };
 
-// The half-bit of weight below the largest that a key falls into, 0 to 63.
-__device__ inline uint32_t half_bit(uint32_t key, float top, float scale) {
-    const float l = logit_of(key);
-    return static_cast<uint32_t>(fminf((l == top ? 0.0f : top - l) * scale, 63.0f));
-}
+// The half-bit of weight below the largest, 0 to 63.
+__device__ inline uint32_t half_bit(float z) { return min(whole_of(z * -2.0f), 63u); }
 
 template <typename T>
 __global__ __launch_bounds__(256) void sample_top_kernel(sample_args a, chunk_store c, int64_t row0) {
@@ -442,12 +581,10 @@ __global__ __launch_bounds__(256) void sample_top_kernel(sample_args a, chunk_st
     const int64_t r = blockIdx.y;
     const typename T::raw *logits = static_cast<const typename T::raw *>(a.logits) + (row0 + r) * a.ld;
     const int at = static_cast<int>(blockIdx.x) * kChunk + static_cast<int>(threadIdx.x) * 8;
-    uint32_t key[16], top = 0;
-    load_keys<T>(logits, at, a.V, key);
-    load_keys<T>(logits, at + 2048, a.V, key + 8);
-#pragma unroll
-    for (int e = 0; e < 16; ++e) top = max(top, key[e]);
-    top = wave_max(top);
+    float l[2][8];
+    load_logits<T>(logits, at, a.V, l[0]);
+    load_logits<T>(logits, at + 2048, a.V, l[1]);
+    const uint32_t top = wave_max(max(largest_key(l[0]), largest_key(l[1])));
     if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = top;
     __syncthreads();
     if (threadIdx.x == 0) c.top[r * c.chunks + blockIdx.x] = max(max(part[0], part[1]), max(part[2], part[3]));
@@ -462,62 +599,86 @@ __device__ inline uint32_t row_top(const chunk_store &c, int64_t r) {
 
 template <typename T>
 __global__ __launch_bounds__(256) void sample_chunk_kernel(sample_args a, chunk_store c, int64_t row0) {
-    __shared__ uint32_t bins[64];
+    // Copies of the bins for every wave and every fourth lane: lanes of one
+    // wave often meet in a bin.
+    constexpr int kCopies = 16;
+    __shared__ uint64_t bins[kCopies][64];
     __shared__ uint64_t part[4];
     __shared__ uint32_t counts[4];
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int lane = threadIdx.x & 63, wave = static_cast<int>(uniform(threadIdx.x >> 6));
     const int64_t r = blockIdx.y, row = row0 + r, chunk = r * c.chunks + blockIdx.x;
     const typename T::raw *logits = static_cast<const typename T::raw *>(a.logits) + row * a.ld;
     const int base = static_cast<int>(blockIdx.x) * kChunk + (wave * 128 + lane) * 8;   // vectors at +0 and +512
-    uint32_t key[16], w[16];
-    load_keys<T>(logits, base, a.V, key);
-    load_keys<T>(logits, base + 512, a.V, key + 8);
+    float l[2][8];
+    load_logits<T>(logits, base, a.V, l[0]);
+    load_logits<T>(logits, base + 512, a.V, l[1]);
     const row_params p = params_of(a, row);
     const uint32_t top_key = row_top(c, r);
     if (!top_key) return;   // the whole row is empty
-    const float top = logit_of(top_key);
+    float top = logit_of(top_key);
+    if (is_infinite(top)) {
+        top = 0.0f;
+#pragma unroll
+        for (int e = 0; e < 16; ++e) l[e / 8][e % 8] = finite_of(l[e / 8][e % 8]);
+    }
     const bool filtered = p.k || p.p < 1u << 24;
 
     uint64_t mine = 0;
+    if (!filtered) {
 #pragma unroll
-    for (int e = 0; e < 16; ++e) {
-        w[e] = weight_of(key[e], top, p.per);
-        if (!filtered && p.min_e > 0.0f) w[e] = e_of(logit_of(key[e]), top, p.per) >= p.min_e ? w[e] : 0u;
-        mine += w[e];
+        for (int e = 0; e < 16; ++e) {
+            const float weight = e_of(z_of(l[e / 8][e % 8], top, p.per));
+            mine += whole_of(weight >= p.min_e ? weight * 0x1p31f : 0.0f);
+        }
+        mine = wave_total(mine);
+        if (lane == 0) part[wave] = mine;
+        __syncthreads();
+        if (threadIdx.x == 0) c.weight[chunk] = part[0] + part[1] + part[2] + part[3];
+        return;
     }
-    mine = wave_total(mine);
-    if (lane == 0) part[wave] = mine;
-    if (threadIdx.x < 64) bins[threadIdx.x] = 0;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) bins[wave * 4 + i][lane] = 0;
     __syncthreads();
-    if (threadIdx.x == 0) c.weight[chunk] = part[0] + part[1] + part[2] + part[3];
-    if (!filtered) return;
-
-    const float scale = fminf(2.0f * p.per, 3.4e38f);
     uint32_t bin[16];
 #pragma unroll
     for (int e = 0; e < 16; ++e) {
-        bin[e] = w[e] ? half_bit(key[e], top, scale) : 64u;
-        if (w[e]) atomicAdd(&bins[bin[e]], 1u);
+        const float z = z_of(l[e / 8][e % 8], top, p.per);
+        const uint32_t w = w_of(z);
+        bin[e] = w ? half_bit(z) : 64u;
+        if (w)
+            atomicAdd(reinterpret_cast<unsigned long long *>(&bins[wave * 4 + (lane & 3)][bin[e]]),
+                      (uint64_t{1} << kCountShift) + w);
     }
     __syncthreads();
-    const uint32_t upto = static_cast<uint32_t>(wave_scan(bins[lane]));
+    uint64_t sum = 0;   // of half-bit `lane`
+#pragma unroll
+    for (int i = 0; i < kCopies; ++i) sum += bins[i][lane];
+    if (wave == 0) {
+        c.bins[chunk * 64 + lane] = sum;
+        const uint64_t all = wave_total(sum & kWeightMask);
+        if (lane == 0) c.weight[chunk] = all;
+    }
+    const uint32_t upto = wave_scan(static_cast<uint32_t>(sum >> kCountShift));
     const int whole = __popcll(__ballot(upto <= static_cast<uint32_t>(c.cap))) - 1;   // upto does not fall with the lane
 
     // This thread's candidates in both vectors, counted before it in the wave.
     uint32_t own = 0;
 #pragma unroll
     for (int e = 0; e < 16; ++e) own += static_cast<int>(bin[e]) <= whole ? (e < 8 ? 1u : 0x10000u) : 0u;
-    const uint32_t through = static_cast<uint32_t>(wave_scan(own));   // no carry between the halves: at most 512 each
+    const uint32_t through = wave_scan(own);   // no carry between the halves: at most 512 each
     const uint32_t all = lane_value(through, 63);
     if (lane == 0) counts[wave] = (all & 0xFFFFu) + (all >> 16);
     __syncthreads();
     uint32_t first = 0;
     for (int i = 0; i < wave; ++i) first += counts[i];
-    uint32_t at[2] = {first + ((through - own) & 0xFFFFu), first + (all & 0xFFFFu) + ((through - own) >> 16)};
+    if (own) {
+        uint32_t at[2] = {first + ((through - own) & 0xFFFFu), first + (all & 0xFFFFu) + ((through - own) >> 16)};
 #pragma unroll
-    for (int e = 0; e < 16; ++e)
-        if (static_cast<int>(bin[e]) <= whole)
-            c.slot[chunk * c.cap + at[e / 8]++] = make_uint2(key[e], static_cast<uint32_t>(base + (e / 8) * 512 + e % 8));
+        for (int e = 0; e < 16; ++e)
+            if (static_cast<int>(bin[e]) <= whole)
+                c.slot[chunk * c.cap + at[e / 8]++] =
+                    make_uint2(__float_as_uint(l[e / 8][e % 8]), static_cast<uint32_t>(base + (e / 8) * 512 + e % 8));
+    }
     if (threadIdx.x == 0) {
         c.count[chunk] = counts[0] + counts[1] + counts[2] + counts[3];
         c.whole[chunk] = whole;
@@ -541,34 +702,43 @@ struct row_stream {
     const raw *logits;
     const int V;
     const float top, per;
+    const bool infinite;
     const int lane = threadIdx.x & 63, wave = static_cast<int>(uniform(threadIdx.x >> 6));
     const int run, begin, end;
     uint32_t K = 1, I = 0xFFFFFFFFu;
 
-    __device__ row_stream(lds &l, const raw *p, int n, float t, float f)
-        : s(l), logits(p), V(n), top(t), per(f), run((n + 8191) / 8192 * 512), begin(min(wave * run, n)),
+    __device__ row_stream(lds &l, const raw *p, int n, float t, float f, bool inf)
+        : s(l), logits(p), V(n), top(t), per(f), infinite(inf), run((n + 8191) / 8192 * 512), begin(min(wave * run, n)),
           end(min(begin + run, n)) {}
 
     __device__ bool kept(uint32_t key, int i) const {
         return (key > K) | ((key == K) & (static_cast<uint32_t>(i) <= I));
     }
 
-    // f(key, index) of every element of this wave's run that is ever drawn's key, or 0.
-    template <typename F>
-    __device__ void each(F &&f) {
-        for (int i = begin; i < end; i += 512) {
-            uint32_t key[8];
-            load_keys<T>(logits, i + lane * 8, V, key);
+    __device__ void load(int i, float (&l)[8]) {
+        load_logits<T>(logits, i + lane * 8, V, l);
+        if (infinite) {
 #pragma unroll
-            for (int e = 0; e < 8; ++e) f(key[e], i + lane * 8 + e);
+            for (int e = 0; e < 8; ++e) l[e] = finite_of(l[e]);
         }
     }
 
-    // The sum over the block of amount(key, index); each wave's in s.part.
+    // f(logit, index) of every element of this wave's run.
+    template <typename F>
+    __device__ void each(F &&f) {
+        for (int i = begin; i < end; i += 512) {
+            float l[8];
+            load(i, l);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) f(l[e], i + lane * 8 + e);
+        }
+    }
+
+    // The sum over the block of amount(logit, index); each wave's in s.part.
     template <typename A>
     __device__ uint64_t total(A &&amount) {
         uint64_t mine = 0;
-        each([&](uint32_t key, int i) { mine += amount(key, i); });
+        each([&](float l, int i) { mine += amount(l, i); });
         mine = wave_total(mine);
         __syncthreads();
         if (lane == 0) s.part[wave] = mine;
@@ -576,48 +746,46 @@ struct row_stream {
         return wave_total(lane < 16 ? s.part[lane] : 0);
     }
 
-    // After total(amount): hit(key, index) of the first element where the running sum exceeds t.
-    template <typename A, typename H>
-    __device__ void first_over(A &&amount, uint64_t t, H &&hit) {
+    // After total(amount): true in the thread of the first element where the
+    // running sum exceeds t, with its index and logit.
+    template <typename A>
+    __device__ bool first_over(A &&amount, uint64_t t, int &its_index, float &its_logit) {
         const uint64_t sums = wave_scan(lane < 16 ? s.part[lane] : 0);
         uint64_t before = wave ? lane_value(sums, wave - 1) : 0;
-        if (t < before || t >= lane_value(sums, wave)) return;
+        if (t < before || t >= lane_value(sums, wave)) return false;
         for (int i = begin; i < end; i += 512) {
-            uint32_t key[8];
-            load_keys<T>(logits, i + lane * 8, V, key);
+            float l[8];
+            load(i, l);
             uint64_t eight = 0;
 #pragma unroll
-            for (int e = 0; e < 8; ++e) eight += amount(key[e], i + lane * 8 + e);
+            for (int e = 0; e < 8; ++e) eight += amount(l[e], i + lane * 8 + e);
             const uint64_t upto = before + wave_scan(eight);
-            const uint64_t over = __ballot(upto > t);
-            if (over) {
-                if (lane == __builtin_ctzll(over)) {
-                    uint64_t sum = upto - eight;
-                    bool found = false;
-#pragma unroll
-                    for (int e = 0; e < 8; ++e) {
-                        sum += amount(key[e], i + lane * 8 + e);
-                        if (!found & (sum > t)) {
-                            found = true;
-                            hit(key[e], i + lane * 8 + e);
-                        }
-                    }
-                }
-                return;
-            }
             before = lane_value(upto, 63);
+            if (before <= t) continue;
+            uint64_t sum = upto - eight;
+            bool found = false;
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                const uint64_t next = sum + amount(l[e], i + lane * 8 + e);
+                const bool at = (sum <= t) & (next > t);
+                its_index = at ? i + lane * 8 + e : its_index;
+                its_logit = at ? l[e] : its_logit;
+                found |= at;
+                sum = next;
+            }
+            return found;
         }
+        return false;
     }
 
-    // As row_list::select, with 2048 bins (the first 1/64 of a bit wide).
+    // Narrows the kept set to its shortest prefix whose amounts (1, or the
+    // weights) reach `need`, as row_list does, with 2048 bins (the first 1/64
+    // of a bit wide); leaves it if they do not.
     __device__ void select(bool by_weight, uint64_t need) {
         uint32_t hi = 0xFFFFFFFFu, lo = 1;
         int shift = -1;
-        const float scale = fminf(64.0f * per, 3.4e38f);
-        const auto bin_of = [&](uint32_t key) {
-            const float l = logit_of(key);
-            return shift < 0 ? static_cast<uint32_t>(fminf((l == top ? 0.0f : top - l) * scale, 2047.0f))
-                             : (hi - key) >> shift;
+        const auto bin_of = [&](uint32_t key, float z) {
+            return shift < 0 ? min(whole_of(z * -64.0f), 2047u) : (hi - key) >> shift;
         };
         for (;;) {
             __syncthreads();
@@ -630,10 +798,11 @@ struct row_stream {
                 s.chosen = 0xFFFFFFFFu;
             }
             __syncthreads();
-            each([&](uint32_t key, int i) {
-                const uint32_t w = weight_of(key, top, per);
+            each([&](float l, int i) {
+                const float z = z_of(l, top, per);
+                const uint32_t w = w_of(z), key = key_of(l);
                 if ((w != 0) & (key >= lo) & (key <= hi) & kept(key, i))
-                    atomicAdd(reinterpret_cast<unsigned long long *>(&s.bins[bin_of(key)]), by_weight ? w : 1u);
+                    atomicAdd(reinterpret_cast<unsigned long long *>(&s.bins[bin_of(key, z)]), by_weight ? w : 1u);
             });
             __syncthreads();
             if (wave == 0) {   // 32 bins a lane, from the largest logits
@@ -660,9 +829,10 @@ struct row_stream {
             if (chosen == 0xFFFFFFFFu) return;
             need -= lane_value(s.before, 0);
             uint32_t high = 0, low = 0xFFFFFFFFu;
-            each([&](uint32_t key, int i) {
-                const uint32_t w = weight_of(key, top, per);
-                if ((w != 0) & (key >= lo) & (key <= hi) & kept(key, i) & (bin_of(key) == chosen)) {
+            each([&](float l, int i) {
+                const float z = z_of(l, top, per);
+                const uint32_t w = w_of(z), key = key_of(l);
+                if ((w != 0) & (key >= lo) & (key <= hi) & kept(key, i) & (bin_of(key, z) == chosen)) {
                     high = max(high, key);
                     low = min(low, key);
                     const uint32_t at = atomicAdd(&s.count, 1u);
@@ -703,9 +873,14 @@ struct row_stream {
         const uint32_t equal = lo;
         const uint64_t each_one = by_weight ? uniform(s.weight[0]) : 1u;
         const uint64_t count = (need + each_one - 1) / each_one;
-        const auto one = [&](uint32_t key, int i) -> uint64_t { return ((key == equal) & kept(key, i)) ? 1u : 0u; };
+        const auto one = [&](float l, int i) -> uint64_t {
+            const uint32_t key = key_of(l);
+            return ((key == equal) & kept(key, i)) ? 1u : 0u;
+        };
         total(one);
-        first_over(one, count - 1, [&](uint32_t, int i) { s.chosen = static_cast<uint32_t>(i); });
+        int at = 0;
+        float unused = 0.0f;
+        if (first_over(one, count - 1, at, unused)) s.chosen = static_cast<uint32_t>(at);
         __syncthreads();
         K = equal;
         I = uniform(s.chosen);
@@ -713,130 +888,230 @@ struct row_stream {
 };
 
 template <typename T>
+struct row_lds {
+    list_lds<16> list;
+    uint64_t sums[kMostChunks];   // kept weight of each chunk
+    union {
+        typename row_stream<T>::lds stream;
+        struct {
+            uint2 slot[kSlots];
+            uint32_t offset[kMostChunks];
+            uint64_t weight[64];
+            uint32_t count[64];
+        } wide;
+    };
+    uint64_t before;
+    int chunk;
+};
+
+template <typename T>
 __global__ __launch_bounds__(1024) void sample_row_kernel(sample_args a, chunk_store c, int64_t row0) {
-    using stream_t = row_stream<T>;
-    __shared__ union {
-        list_lds<16> list;
-        typename stream_t::lds stream;
-    } lds;
-    __shared__ uint64_t found_before;
-    __shared__ int found_chunk;
-    const int lane = threadIdx.x & 63;
+    __shared__ row_lds<T> s;
+    using raw = typename T::raw;
+    const int lane = threadIdx.x & 63, wave = static_cast<int>(uniform(threadIdx.x >> 6));
     const int64_t r = blockIdx.x, row = row0 + r, chunk0 = r * c.chunks;
-    const typename T::raw *logits = static_cast<const typename T::raw *>(a.logits) + row * a.ld;
+    const raw *logits = static_cast<const raw *>(a.logits) + row * a.ld;
     const row_params p = params_of(a, row);
+    row_list<16, 8, true> list(s.list);
     const uint32_t top_key = row_top(c, r);
     if (!top_key) {
         if (threadIdx.x == 0) write_empty(a, row);
         return;
     }
-    const float top = logit_of(top_key);
+    const bool infinite = is_infinite(logit_of(top_key));
+    const float top = infinite ? 0.0f : logit_of(top_key);
     const bool filtered = p.k || p.p < 1u << 24;
 
     // The row's weight, and for filtered rows the least half-bit given whole.
     int whole = 63;
     uint64_t weight = 0;
     for (int i = lane; i < c.chunks; i += 64) {
-        weight += c.weight[chunk0 + i];
+        const uint64_t w = c.weight[chunk0 + i];
+        weight += w;
+        if (wave == 0) s.sums[i] = w;
         if (filtered) whole = min(whole, c.whole[chunk0 + i]);
     }
     weight = wave_total(weight);
     whole = static_cast<int>(63u - wave_max(static_cast<uint32_t>(63 - whole)));
 
-    if (!filtered) {
-        // The chunk where the running weight exceeds t, and the draw in it: 4096 elements, 8 for each of 512 threads.
-        const uint64_t t = share(p.u, weight);
-        if (threadIdx.x < 64) {
-            uint64_t before = 0;
-            for (int i = 0; i < c.chunks; i += 64) {
-                const uint64_t upto = before + wave_scan(i + lane < c.chunks ? c.weight[chunk0 + i + lane] : 0);
-                const uint64_t over = __ballot(upto > t);
-                if (over) {
-                    const int owner = __builtin_ctzll(over);
-                    if (lane == owner) {
-                        found_chunk = i + lane;
-                        found_before = upto - c.weight[chunk0 + i + lane];
-                    }
-                    break;
-                }
-                before = lane_value(upto, 63);
-            }
-        }
-        __syncthreads();
-        const int base = static_cast<int>(uniform(static_cast<uint32_t>(found_chunk))) * kChunk;
-        const uint64_t rest = t - found_before;
-        row_list<16, 8> list(lds.list);
-        const int at = static_cast<int>(list.place(0));
-        load_keys<T>(logits, base + at, at < kChunk ? a.V : 0, list.key);
-        uint64_t mine = 0;
-#pragma unroll
-        for (int e = 0; e < 8; ++e) {
-            list.w[e] = weight_of(list.key[e], top, p.per);
-            if (p.min_e > 0.0f) list.w[e] = e_of(logit_of(list.key[e]), top, p.per) >= p.min_e ? list.w[e] : 0u;
-            mine += list.w[e];
-        }
-        list.total(mine);
-        list.first_over([&](int e) { return list.w[e]; }, rest, mine, [&](int e) {
-            a.token[row] = base + static_cast<int>(list.place(e));
-            if (a.logp) a.logp[row] = logp_of(z_of(logit_of(list.key[e]), top, p.per), weight);
-        });
-        return;
-    }
-
-    {
-        row_list<16, 8, true> list(lds.list);
-        const float scale = fminf(2.0f * p.per, 3.4e38f);
-        uint64_t count = 0;
+    uint32_t K = 1, I = 0xFFFFFFFFu;
+    if (filtered) {
         const int place = static_cast<int>(list.place(0)), chunk = place / c.cap, first = place % c.cap;
         const int n = chunk < c.chunks ? static_cast<int>(c.count[chunk0 + chunk]) - first : 0;
         const uint2 *slot = c.slot + (chunk0 + chunk) * c.cap + first;
+        uint64_t mine = 0;
+        uint32_t count = 0;
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
-            const uint2 s = e < n ? slot[e] : make_uint2(0, 0);
-            list.key[e] = static_cast<int>(half_bit(s.x, top, scale)) > whole ? 0u : s.x;
-            list.given[e] = s.y;
-            list.w[e] = weight_of(s.x, top, p.per);
+            const uint2 v = e < n ? slot[e] : make_uint2(0xFF800000u, 0);   // -infinity
+            const float l = __uint_as_float(v.x);
+            list.set(e, l, top, p.per, 0.0f, 8.0f);
+            list.given[e] = v.y;
+            if (static_cast<int>(half_bit(z_of(l, top, p.per))) > whole) list.key[e] = 0;
+            mine += list.key[e] ? list.w[e] : 0u;
             count += list.key[e] ? 1u : 0u;
         }
-        // Complete down to what the filters ask for?
-        const bool all = whole == 63;
-        bool enough = true;
-        if (p.k) enough = all || list.total(count) >= p.k;
-        uint64_t need = 0;
-        if (!p.k) {
-            need = share(p.p, weight);
-            enough = all || list.total(list.kept_weight()) >= (need ? need : 1);
-        }
+        // Do they hold the kept set?  They do if top-k ends in them; without
+        // top-k, if top-p does, or if min-p lets nothing below them through.
+        bool enough = whole == 63;
+        const uint64_t need = p.k ? p.k : max(share(p.p, weight), uint64_t{1});
+        const uint64_t have = list.total(p.k ? count : mine);   // (its barriers follow the clearing of the bins)
+        enough |= have >= need;
+        enough |= !p.k && e_of(-0.5f * static_cast<float>(whole + 1)) * 1.0001f < p.min_e;
         if (enough) {
-            if (p.k) list.select(false, p.k, top, p.per);
-            if (p.p < 1u << 24) {
-                if (p.k) need = share(p.p, list.total(list.kept_weight()));
-                list.select(true, need ? need : 1, top, p.per);
+            list.filter(p.k, p.k ? p.p : 1u << 24, p.k ? 0 : need);
+            list.draw(a, row, p, top, list.drop(p.min_e, top, p.per), 0, 0);
+            return;
+        }
+
+        // A wide set: the half-bit where the weight crosses `need`.
+        bool stream = p.k != 0;
+        uint32_t b = 0;
+        if (!stream) {
+            auto &wide = s.wide;
+            if (threadIdx.x < 64) {
+                wide.weight[threadIdx.x] = 0;
+                wide.count[threadIdx.x] = 0;
             }
-            list.draw(a, row, p, top);
+            __syncthreads();
+            uint64_t w = 0;
+            uint32_t n_b = 0;
+            for (int i = wave; i < c.chunks; i += 16) {
+                const uint64_t v = c.bins[(chunk0 + i) * 64 + lane];
+                w += v & kWeightMask;
+                n_b += static_cast<uint32_t>(v >> kCountShift);
+            }
+            atomicAdd(reinterpret_cast<unsigned long long *>(&wide.weight[lane]), w);
+            atomicAdd(&wide.count[lane], n_b);
+            __syncthreads();
+            const uint64_t upto = wave_scan(wide.weight[lane]);
+            b = static_cast<uint32_t>(__builtin_ctzll(__ballot(upto >= need)));
+            const uint64_t above = b ? lane_value(upto, static_cast<int>(b) - 1) : 0;
+            const uint32_t n_all = uniform(wide.count[b]);
+            stream = n_all > kSlots || (p.min_e > 0.0f && e_of(-0.5f * static_cast<float>(b + 1)) <= p.min_e * 1.0001f);
+            if (!stream) {
+                // Each chunk's weight above the half-bit, and where its elements of it go.
+                for (int i = wave; i < c.chunks; i += 16) {
+                    const uint64_t v = c.bins[(chunk0 + i) * 64 + lane];
+                    const uint64_t sum = wave_total(static_cast<uint32_t>(lane) < b ? v & kWeightMask : 0);
+                    if (lane == 0) {
+                        s.sums[i] = sum;
+                        wide.offset[i] = static_cast<uint32_t>(c.bins[(chunk0 + i) * 64 + b] >> kCountShift);
+                    }
+                }
+                __syncthreads();
+                if (wave == 0) {
+                    uint32_t before = 0;
+                    for (int i = 0; i < c.chunks; i += 64) {
+                        const uint32_t v = i + lane < c.chunks ? wide.offset[i + lane] : 0;
+                        const uint32_t through = before + wave_scan(v);
+                        if (i + lane < c.chunks) wide.offset[i + lane] = through - v;
+                        before = lane_value(through, 63);
+                    }
+                }
+                __syncthreads();
+                for (int i = wave; i < c.chunks; i += 16) {
+                    uint32_t at = uniform(wide.offset[i]);
+                    const uint32_t end = i + 1 < c.chunks ? uniform(wide.offset[i + 1]) : n_all;
+                    for (int v = 0; v < 8 && at < end; ++v) {
+                        const int index = i * kChunk + v * 512 + lane * 8;
+                        float l[8];
+                        load_logits<T>(logits, index, a.V, l);
+                        uint32_t in = 0;
+#pragma unroll
+                        for (int e = 0; e < 8; ++e) {
+                            if (infinite) l[e] = finite_of(l[e]);
+                            const float z = z_of(l[e], top, p.per);
+                            in |= ((half_bit(z) == b) & (w_of(z) != 0)) ? 1u << e : 0u;
+                        }
+                        const uint32_t through = wave_scan(static_cast<uint32_t>(__popc(in)));
+                        uint32_t to = at + through - static_cast<uint32_t>(__popc(in));
+#pragma unroll
+                        for (int e = 0; e < 8; ++e)
+                            if (in >> e & 1)
+                                wide.slot[to++] = make_uint2(__float_as_uint(l[e]), static_cast<uint32_t>(index + e));
+                        at += lane_value(through, 63);
+                    }
+                }
+                __syncthreads();
+                row_list<16, 8, true> part(s.list);
+                __syncthreads();
+#pragma unroll
+                for (int e = 0; e < 8; ++e) {
+                    const uint32_t at = part.place(e);
+                    const uint2 v = at < n_all ? wide.slot[at] : make_uint2(0xFF800000u, 0);
+                    // 1/512 of a bit a bin: the half-bit's part of z
+                    part.set(e, __uint_as_float(v.x), top, p.per, 0.5f * static_cast<float>(b), 512.0f);
+                    part.given[e] = v.y;
+                }
+                part.filter(0, 1u << 24, need - above);
+                K = part.K;
+                I = part.I;
+                __syncthreads();
+                weight = above + part.total(part.kept_weight());
+#pragma unroll
+                for (int e = 0; e < 8; ++e)
+                    if (part.kept(e))
+                        atomicAdd(reinterpret_cast<unsigned long long *>(&s.sums[part.given[e] / kChunk]), part.w[e]);
+            }
+        }
+        if (stream) {
+            __syncthreads();
+            row_stream<T> whole_row(s.stream, logits, a.V, top, p.per, infinite);
+            if (p.k) whole_row.select(false, p.k);
+            if (p.p < 1u << 24) {
+                const uint64_t of = whole_row.total([&](float l, int i) -> uint64_t {
+                    return whole_row.kept(key_of(l), i) ? w_of(z_of(l, top, p.per)) : 0u;
+                });
+                whole_row.select(true, max(share(p.p, of), uint64_t{1}));
+            }
+            const auto amount = [&](float l, int i) -> uint64_t {
+                const float e = e_of(z_of(l, top, p.per));
+                return (whole_row.kept(key_of(l), i) & (e >= p.min_e)) ? whole_of(e * 0x1p31f) : 0u;
+            };
+            const uint64_t total = whole_row.total(amount);
+            int at = 0;
+            float its = 0.0f;
+            if (!whole_row.first_over(amount, share(p.u, total), at, its)) return;
+            a.token[row] = at;
+            if (a.logp) a.logp[row] = logp_of(z_of(its, top, p.per), total);
             return;
         }
     }
 
+    // The chunk where the running weight exceeds t, and the draw in it.
     __syncthreads();
-    stream_t stream(lds.stream, logits, a.V, top, p.per);
-    if (p.k) stream.select(false, p.k);
-    if (p.p < 1u << 24) {
-        const uint64_t of = p.k ? stream.total([&](uint32_t key, int i) -> uint64_t {
-            return stream.kept(key, i) ? weight_of(key, top, p.per) : 0u;
-        }) : weight;
-        const uint64_t need = share(p.p, of);
-        stream.select(true, need ? need : 1);
+    const uint64_t t = share(p.u, weight);
+    if (wave == 0) {
+        uint64_t before = 0;
+        for (int i = 0; i < c.chunks; i += 64) {
+            const uint64_t v = i + lane < c.chunks ? s.sums[i + lane] : 0;
+            const uint64_t upto = before + wave_scan(v);
+            const uint64_t over = __ballot(upto > t);
+            if (over) {
+                if (lane == __builtin_ctzll(over)) {
+                    s.chunk = i + lane;
+                    s.before = upto - v;
+                }
+                break;
+            }
+            before = lane_value(upto, 63);
+        }
     }
-    const auto amount = [&](uint32_t key, int i) -> uint64_t {
-        const float e = e_of(logit_of(key), top, p.per);
-        return ((key != 0) & stream.kept(key, i) & (e >= p.min_e)) ? w_of(e) : 0u;
-    };
-    const uint64_t total = stream.total(amount);
-    stream.first_over(amount, share(p.u, total), [&](uint32_t key, int i) {
-        a.token[row] = i;
-        if (a.logp) a.logp[row] = logp_of(z_of(logit_of(key), top, p.per), total);
-    });
+    __syncthreads();
+    const int base = static_cast<int>(uniform(static_cast<uint32_t>(s.chunk))) * kChunk;
+    row_list<16, 8, true> drawn(s.list);
+    const int at = static_cast<int>(drawn.place(0));
+    float l[8];
+    load_logits<T>(logits, base + at, at < kChunk ? a.V : 0, l);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+        drawn.set(e, infinite ? finite_of(l[e]) : l[e], top, p.per, 0.0f, 8.0f);
+        drawn.given[e] = static_cast<uint32_t>(base + at + e);
+    }
+    drawn.K = K;
+    drawn.I = I;
+    drawn.draw(a, row, p, top, drawn.drop(p.min_e, top, p.per), weight, t - s.before);
 }
 
 template <typename T>
@@ -846,12 +1121,12 @@ aq_status launch_long(aq_ctx *ctx, const sample_args &a) {
     c.cap = kSlots / c.chunks / 8 * 8;
     const size_t rows = static_cast<size_t>(a.rows < kRowsAtOnce ? a.rows : kRowsAtOnce), n = rows * c.chunks;
     char *at = nullptr;
-    const size_t slots = n * c.cap * sizeof(uint2);
-    aq_status st = aq_ctx_scratch(ctx, 7, slots + n * 20, reinterpret_cast<void **>(&at));
+    aq_status st = aq_ctx_scratch(ctx, 7, n * (64 * 8 + 8 + c.cap * 8 + 12), reinterpret_cast<void **>(&at));
     if (st != AQ_OK) return st;
-    c.slot = reinterpret_cast<uint2 *>(at);
-    c.weight = reinterpret_cast<uint64_t *>(at + slots);
-    c.top = reinterpret_cast<uint32_t *>(c.weight + n);
+    c.bins = reinterpret_cast<uint64_t *>(at);
+    c.weight = c.bins + n * 64;
+    c.slot = reinterpret_cast<uint2 *>(c.weight + n);
+    c.top = reinterpret_cast<uint32_t *>(c.slot + n * c.cap);
     c.count = c.top + n;
     c.whole = reinterpret_cast<int32_t *>(c.count + n);
     for (int64_t row0 = 0; row0 < a.rows; row0 += kRowsAtOnce) {
