@@ -158,27 +158,35 @@ __device__ inline uint32_t wave_max(uint32_t v) {
 // takes every decision for itself from what lies in LDS, so a step needs no
 // barrier for its result.
 //
-// The filters.  256 bins by weight (of count and weight at once: 15 bits and
-// 46 of a word); the bin where the running count or weight crosses what is
+// The filters.  Bins by weight (of count and weight at once: 15 bits and 46
+// of a word); the bin where the running count or weight crosses what is
 // needed holds the end of the kept prefix.  If it has at most 64 elements, a
 // wave orders them by comparing all pairs; else it is divided again, in bins
 // linear in the key, which tells any two different logits apart after at most
-// four times; more than 64 equal ones are counted off in index order.
+// four times; more than 64 equal ones are counted off in index order.  There
+// are two bins a thread: with 256 for 8192 elements their atomics met in the
+// same words (13 000 cycles) and the ordering had dozens of elements.
 constexpr int kCountShift = 48;
 constexpr uint64_t kWeightMask = (uint64_t{1} << kCountShift) - 1;
 
+constexpr int bins_of(int waves) { return waves < 2 ? 256 : 128 * waves; }
+
 template <int WAVES>
 struct list_lds {
-    uint64_t bins[256];
+    uint64_t bins[bins_of(WAVES)];
     uint64_t part[WAVES];
+    uint32_t part_n[WAVES];
     uint32_t key[2][64], index[2][64], weight[2][64];
     uint32_t count[2], hi[2], lo[2], at, each;
+    // What one thread or wave found for all.
+    uint32_t bin[2], K, I;
+    uint64_t need[2], before, through;
 };
 
 template <int WAVES, int E, bool GIVEN = false>   // GIVEN: the elements bring their indices
 struct row_list {
-    static constexpr int kThreads = 64 * WAVES;
-    static constexpr int kNoBin = 256;
+    static constexpr int kThreads = 64 * WAVES, kBins = bins_of(WAVES), kPer = kBins / kThreads;
+    static constexpr float kBinsPerBit = kBins / 32.0f;   // weights span 31 bits
     list_lds<WAVES> &s;
     const int lane = threadIdx.x & 63, wave = static_cast<int>(uniform(threadIdx.x >> 6));
     uint32_t key[E], w[E], bin[E];
@@ -197,8 +205,7 @@ struct row_list {
 
     __device__ void clear() {
 #pragma unroll
-        for (int b = 0; b < 256; b += kThreads)
-            if (b + threadIdx.x < 256) s.bins[b + threadIdx.x] = 0;
+        for (int b = 0; b < kPer; ++b) s.bins[threadIdx.x + b * kThreads] = 0;
     }
 
     __device__ uint32_t place(int e) const {   // in the list
@@ -216,7 +223,7 @@ struct row_list {
         const float z = z_of(l, top, per);
         w[e] = w_of(z);
         key[e] = w[e] ? key_of(l) : 0;
-        bin[e] = min(whole_of((-z - z0) * scale), 255u);
+        bin[e] = min(whole_of((-z - z0) * scale), kBins - 1u);
     }
 
     // Each wave's sum of `mine` in s.part; the sum over the block.
@@ -267,13 +274,12 @@ struct row_list {
         return found;
     }
 
-    // Puts the end of the kept prefix into bin `chosen`, where `need` of the
-    // amounts (1, or the weights) are still to come; returns the weight kept
-    // of that bin.  `phase`: 0 and 1, each once after a clear.
-    __device__ uint64_t resolve(uint32_t chosen, int phase, bool by_weight, uint64_t need) {
+    // Into LDS: the elements that `in` names, up to 64, and the range of the others' keys.
+    template <typename P>
+    __device__ void gather(int phase, P &&in) {
 #pragma unroll
         for (int e = 0; e < E; ++e) {
-            if ((bin[e] != chosen) | !kept(e)) continue;
+            if (!in(e)) continue;
             const uint32_t at = atomicAdd(&s.count[phase], 1u);
             if (at < 64) {
                 s.key[phase][at] = key[e];
@@ -284,6 +290,13 @@ struct row_list {
                 atomicMin(&s.lo[phase], key[e]);
             }
         }
+    }
+
+    // Puts the end of the kept prefix into bin `chosen`, where `need` of the
+    // amounts (1, or the weights) are still to come; returns the weight kept
+    // of that bin.  `phase`: 0 and 1, each once after a clear.
+    __device__ uint64_t resolve(uint32_t chosen, int phase, bool by_weight, uint64_t need) {
+        gather(phase, [&](int e) { return (bin[e] == chosen) & kept(e); });
         __syncthreads();
         const uint32_t n = uniform(s.count[phase]);
         if (n <= 64) return order(phase, n, by_weight, need);
@@ -292,34 +305,118 @@ struct row_list {
         uint64_t mine = 0;
 #pragma unroll
         for (int e = 0; e < E; ++e) mine += ((bin[e] == chosen) & kept(e)) ? w[e] : 0u;
-        return by_weight ? 0 : total(mine);
+        return total(mine);
     }
 
-    // The end of the kept prefix among the n <= 64 elements of the short list.
+    // The end of the kept prefix among the n <= 64 elements of the short
+    // list.  Every wave finds it, or where they would share their SIMDs the
+    // first one for all.
     __device__ uint64_t order(int phase, uint32_t n, bool by_weight, uint64_t need) {
-        const bool there = static_cast<uint32_t>(lane) < n;
-        const uint32_t k = there ? s.key[phase][lane] : 0, at = there ? s.index[phase][lane] : 0;
-        const uint32_t weight = there ? s.weight[phase][lane] : 0;
-        uint64_t ahead_w = weight;
-        uint32_t ahead = 1;
-        for (uint32_t i = 0; i < n; ++i) {
-            const uint32_t ki = lane_value(k, i), ai = lane_value(at, i), wi = lane_value(weight, i);
-            const bool first = (ki > k) | ((ki == k) & (ai < at));
-            ahead_w += first ? wi : 0u;
-            ahead += first ? 1u : 0u;
+        uint64_t inside = 0;
+        if (WAVES <= 4 || wave == 0) {
+            const bool there = static_cast<uint32_t>(lane) < n;
+            const uint32_t k = there ? s.key[phase][lane] : 0, at = there ? s.index[phase][lane] : 0;
+            const uint32_t weight = there ? s.weight[phase][lane] : 0;
+            uint64_t through_w = weight;
+            uint32_t through_n = 1;
+            for (uint32_t i = 0; i < n; ++i) {
+                const uint32_t ki = lane_value(k, i), ai = lane_value(at, i), wi = lane_value(weight, i);
+                const bool first = (ki > k) | ((ki == k) & (ai < at));
+                through_w += first ? wi : 0u;
+                through_n += first ? 1u : 0u;
+            }
+            // The last one kept is the first through which the amount reaches `need`.
+            const uint64_t through = by_weight ? through_w : through_n, before = through - (by_weight ? weight : 1u);
+            const int last = __builtin_ctzll(__ballot(there & (before < need) & (through >= need)));
+            K = lane_value(k, last);
+            I = lane_value(at, last);
+            inside = lane_value(through_w, last);
         }
-        // Through this element; the last one kept is the first that reaches `need`.
-        const uint64_t through = by_weight ? ahead_w : ahead, before = through - (by_weight ? weight : 1u);
-        const int last = __builtin_ctzll(__ballot(there & (before < need) & (through >= need)));
-        K = lane_value(k, last);
-        I = lane_value(at, last);
-        return lane_value(ahead_w, last);
+        if (WAVES > 4) {
+            if (threadIdx.x == 0) {
+                s.K = K;
+                s.I = I;
+                s.through = inside;
+            }
+            __syncthreads();
+            K = uniform(s.K);
+            I = uniform(s.I);
+            inside = lane_value(s.through, 0);
+        }
+        return inside;
     }
 
-    // The same for more than 64 elements, the kept ones with keys from lo to hi.
+    // This thread's bins, the largest logits first: the sums of weight and
+    // count through the bins of the threads before it, and its own.
+    struct bin_sums {
+        uint64_t w[kPer], before_w, own_w, all_w;
+        uint32_t n[kPer], before_n, own_n, all_n;
+    };
+    __device__ void scan_bins(bin_sums &b) {
+        b.own_w = 0;
+        b.own_n = 0;
+#pragma unroll
+        for (int i = 0; i < kPer; ++i) {
+            const uint64_t v = s.bins[threadIdx.x * kPer + i];
+            b.own_w += b.w[i] = v & kWeightMask;
+            b.own_n += b.n[i] = static_cast<uint32_t>(v >> kCountShift);
+        }
+        const uint64_t w = wave_scan(b.own_w);
+        const uint32_t n = wave_scan(b.own_n);
+        b.before_w = w - b.own_w;
+        b.before_n = n - b.own_n;
+        b.all_w = lane_value(w, 63);
+        b.all_n = lane_value(n, 63);
+        if (WAVES > 1) {
+            if (lane == 63) {
+                s.part[wave] = w;
+                s.part_n[wave] = n;
+            }
+            __syncthreads();
+            b.all_w = 0;
+            b.all_n = 0;
+#pragma unroll
+            for (int i = 0; i < WAVES; ++i) {
+                b.before_w += i < wave ? s.part[i] : 0;
+                b.before_n += i < wave ? s.part_n[i] : 0;
+                b.all_w += s.part[i];
+                b.all_n += s.part_n[i];
+            }
+            b.all_w = lane_value(b.all_w, 0);
+            b.all_n = uniform(b.all_n);
+        }
+    }
+
+    // Where the running count (or weight) crosses `need`, which it reaches:
+    // the bin, what of `need` is left in it, and the weight before it.
+    __device__ void crossing(const bin_sums &b, int phase, bool by_weight, uint64_t &need, uint32_t &bin_at, uint64_t &weight) {
+        const uint64_t before = by_weight ? b.before_w : b.before_n, own = by_weight ? b.own_w : b.own_n;
+        if ((before < need) & (before + own >= need)) {
+            uint64_t sum = before, w_sum = b.before_w;
+            uint32_t at = 0;
+#pragma unroll
+            for (int i = 0; i + 1 < kPer; ++i) {
+                const uint64_t next = sum + (by_weight ? b.w[i] : b.n[i]);
+                const bool on = (at == static_cast<uint32_t>(i)) & (next < need);
+                sum = on ? next : sum;
+                w_sum += on ? b.w[i] : 0;
+                at += on ? 1u : 0u;
+            }
+            s.bin[phase] = threadIdx.x * kPer + at;
+            s.need[phase] = need - sum;
+            s.before = w_sum;
+        }
+        __syncthreads();
+        bin_at = uniform(s.bin[phase]);
+        need = lane_value(s.need[phase], 0);
+        weight = lane_value(s.before, 0);
+    }
+
+    // As resolve(), for more than 64 elements: the kept ones with keys from lo to hi.
     __device__ void refine(bool by_weight, uint64_t need, uint32_t hi, uint32_t lo) {
+        constexpr int kBits = 31 - __builtin_clz(static_cast<unsigned>(kBins));
         while (hi != lo) {
-            const int shift = max(0, 24 - __builtin_clz(hi - lo));
+            const int shift = max(0, 32 - kBits - __builtin_clz(hi - lo));
             __syncthreads();
             clear();
             if (threadIdx.x == 0) {
@@ -328,40 +425,19 @@ struct row_list {
                 s.lo[0] = 0xFFFFFFFFu;
             }
             __syncthreads();
+            const auto in = [&](int e) { return (key[e] >= lo) & (key[e] <= hi) & kept(e); };
 #pragma unroll
             for (int e = 0; e < E; ++e)
-                if ((key[e] >= lo) & (key[e] <= hi) & kept(e))
+                if (in(e))
                     atomicAdd(reinterpret_cast<unsigned long long *>(&s.bins[(hi - key[e]) >> shift]),
-                              by_weight ? w[e] : 1u);
+                              (uint64_t{1} << kCountShift) + w[e]);
             __syncthreads();
-            uint64_t four[4], sum = 0;
-#pragma unroll
-            for (int b = 0; b < 4; ++b) sum += four[b] = s.bins[4 * lane + b];
-            const uint64_t upto = wave_scan(sum);
-            const int owner = __builtin_ctzll(__ballot(upto >= need));
-            uint64_t before = upto - sum;
-            uint32_t b = 4 * lane;
-#pragma unroll
-            for (int i = 0; i < 3; ++i) {
-                const bool on = (b == static_cast<uint32_t>(4 * lane + i)) & (before + four[i] < need);
-                before += on ? four[i] : 0u;
-                b += on ? 1u : 0u;
-            }
-            const uint32_t chosen = lane_value(b, owner);
-            need -= lane_value(before, owner);
-#pragma unroll
-            for (int e = 0; e < E; ++e) {
-                if (!((key[e] >= lo) & (key[e] <= hi) & kept(e)) || (hi - key[e]) >> shift != chosen) continue;
-                const uint32_t at = atomicAdd(&s.count[0], 1u);
-                if (at < 64) {
-                    s.key[0][at] = key[e];
-                    s.index[0][at] = index(e);
-                    s.weight[0][at] = w[e];
-                } else {
-                    atomicMax(&s.hi[0], key[e]);
-                    atomicMin(&s.lo[0], key[e]);
-                }
-            }
+            bin_sums b;
+            scan_bins(b);
+            uint32_t chosen;
+            uint64_t unused;
+            crossing(b, 0, by_weight, need, chosen, unused);
+            gather(0, [&](int e) { return in(e) & ((hi - key[e]) >> shift == chosen); });
             __syncthreads();
             const uint32_t n = uniform(s.count[0]);
             if (n <= 64) {
@@ -373,7 +449,7 @@ struct row_list {
             lo = min(uniform(s.lo[0]), ~wave_max(~k));
         }
         // Equal logits: the first of them in index order.
-        uint64_t mine = 0;
+        uint64_t mine = 0, each = 1;
         uint32_t some = 0;
         const uint32_t equal = lo;
         const auto one = [&](int e) { return ((key[e] == equal) & kept(e)) ? 1u : 0u; };
@@ -382,15 +458,10 @@ struct row_list {
             mine += one(e);
             some = max(some, one(e) ? w[e] : 0u);
         }
-        uint64_t each = 1;
-        if (by_weight) {   // their weight, from whoever has one
-            if (some) s.each = some;
-        }
+        if (some) s.each = some;   // their weight, from whoever has one
         total(mine);
-        if (by_weight) {
-            if (WAVES == 1) __syncthreads();
-            each = uniform(s.each);
-        }
+        __syncthreads();
+        if (by_weight) each = uniform(s.each);
         uint32_t at = 0, unused = 0;
         if (first_over(one, (need + each - 1) / each - 1, mine, at, unused)) s.at = at;
         __syncthreads();
@@ -399,55 +470,30 @@ struct row_list {
     }
 
     // Top-k (k > 0), then top-p of the weight that leaves (p < 2^24), or
-    // until `need` > 0 of the weight is reached.
-    __device__ void filter(uint32_t k, uint32_t p, uint64_t need) {
+    // until `need` > 0 of the count or weight is reached.
+    __device__ uint64_t filter(uint32_t k, uint32_t p, uint64_t need, bool by_weight = true) {
 #pragma unroll
         for (int e = 0; e < E; ++e)
-            if (key[e])
+            if (kept(e))
                 atomicAdd(reinterpret_cast<unsigned long long *>(&s.bins[bin[e]]),
                           (uint64_t{1} << kCountShift) + w[e]);
         __syncthreads();
-        uint64_t w4[4], w_sum = 0;
-        uint32_t n4[4], n_sum = 0;
-#pragma unroll
-        for (int b = 0; b < 4; ++b) {   // bins 4 lane ..+3, the largest logits first
-            const uint64_t v = s.bins[4 * lane + b];
-            w_sum += w4[b] = v & kWeightMask;
-            n_sum += n4[b] = static_cast<uint32_t>(v >> kCountShift);
-        }
-        const uint32_t n_upto = wave_scan(n_sum);
-        const uint64_t w_upto = wave_scan(w_sum);
-        uint64_t weight = lane_value(w_upto, 63);   // kept
-        const uint64_t over_n = k ? __ballot(n_upto >= k) : 0;
-        if (over_n) {
-            const int owner = __builtin_ctzll(over_n);
-            uint32_t n = n_upto - n_sum, b = 4 * lane;
-            uint64_t before = w_upto - w_sum;
-#pragma unroll
-            for (int i = 0; i < 3; ++i) {
-                const bool on = (b == static_cast<uint32_t>(4 * lane + i)) & (n + n4[i] < k);
-                n += on ? n4[i] : 0u;
-                before += on ? w4[i] : 0u;
-                b += on ? 1u : 0u;
-            }
-            weight = lane_value(before, owner) + resolve(lane_value(b, owner), 0, false, k - lane_value(n, owner));
+        bin_sums b;
+        scan_bins(b);
+        uint64_t weight = b.all_w, before = 0;   // kept
+        uint32_t chosen = 0;
+        if (k && k <= b.all_n) {
+            uint64_t rest = k;
+            crossing(b, 0, false, rest, chosen, before);
+            weight = before + resolve(chosen, 0, false, rest);
         }
         if (p < 1u << 24) need = max(share(p, weight), uint64_t{1});
-        if (need) {
-            // (The sums of bins behind top-k's end are too large, but it is crossed before.)
-            const uint64_t over = __ballot(w_upto >= need);
-            if (!over) return;
-            const int owner = __builtin_ctzll(over);
-            uint64_t before = w_upto - w_sum;
-            uint32_t b = 4 * lane;
-#pragma unroll
-            for (int i = 0; i < 3; ++i) {
-                const bool on = (b == static_cast<uint32_t>(4 * lane + i)) & (before + w4[i] < need);
-                before += on ? w4[i] : 0u;
-                b += on ? 1u : 0u;
-            }
-            resolve(lane_value(b, owner), 1, true, need - lane_value(before, owner));
+        // (The sums of bins behind top-k's end are too large, but it is crossed before.)
+        if (need && need <= (by_weight ? b.all_w : b.all_n)) {
+            crossing(b, 1, by_weight, need, chosen, before);
+            weight = before + resolve(chosen, 1, by_weight, need);
         }
+        return weight;
     }
 
     __device__ uint64_t kept_weight() const {   // this thread's
@@ -537,7 +583,7 @@ __global__ __launch_bounds__(64 * WAVES) void sample_short_kernel(sample_args a)
         for (int e = 0; e < E; ++e) l[e / 8][e % 8] = finite_of(l[e / 8][e % 8]);
     }
 #pragma unroll
-    for (int e = 0; e < E; ++e) list.set(e, l[e / 8][e % 8], top, r.per, 0.0f, 8.0f);
+    for (int e = 0; e < E; ++e) list.set(e, l[e / 8][e % 8], top, r.per, 0.0f, list.kBinsPerBit);
     if (r.k || r.p < 1u << 24) list.filter(r.k, r.p, 0);
     list.draw(a, row, r, top, list.drop(r.min_e, top, r.per), 0, 0);
 }
@@ -552,13 +598,14 @@ __global__ __launch_bounds__(64 * WAVES) void sample_short_kernel(sample_args a)
 //  3. a block per row.  Without filters it finds the chunk that the draw falls
 //     into from the sums, and draws in it.  With filters it works on the
 //     candidates down to the least half-bit that every chunk has given whole,
-//     which hold the kept set unless that is wide.  A wide one ends, without
-//     top-k, in a half-bit that the sums tell: its elements are collected from
-//     the chunks and decide where, and the sums over what lies above it decide
-//     the chunk to draw in.  What is left (a top-k of thousands, min-p's end
-//     in a wide set, more than 8192 elements in half a bit) streams the row.
+//     which hold the kept set unless that is wide.  A wide one ends in a
+//     half-bit that the sums tell (top-k's end, then top-p's): its elements are
+//     collected from the chunks and decide where, and the sums over what lies
+//     above it decide the chunk to draw in.  What is left (min-p's end in a
+//     wide set, more than 8192 elements in half a bit) streams the row.
 constexpr int kChunk = 4096;          // 256 threads, 16 elements each
-constexpr int kSlots = 8192;          // candidates of a row: 1024 threads, 8 each
+constexpr int kSlots = 2048;          // candidates of a row: 256 threads, 8 each
+constexpr int kGathered = 8192;       // elements of a half-bit: 1024 threads, 8 each
 constexpr int kMostChunks = kMaxV / kChunk;
 constexpr int kRowsAtOnce = 256;
 
@@ -889,12 +936,15 @@ struct row_stream {
 
 template <typename T>
 struct row_lds {
-    list_lds<16> list;
+    union {
+        list_lds<4> narrow;
+        list_lds<16> list;
+    };
     uint64_t sums[kMostChunks];   // kept weight of each chunk
     union {
         typename row_stream<T>::lds stream;
         struct {
-            uint2 slot[kSlots];
+            uint2 slot[kGathered];
             uint32_t offset[kMostChunks];
             uint64_t weight[64];
             uint32_t count[64];
@@ -912,7 +962,6 @@ __global__ __launch_bounds__(1024) void sample_row_kernel(sample_args a, chunk_s
     const int64_t r = blockIdx.x, row = row0 + r, chunk0 = r * c.chunks;
     const raw *logits = static_cast<const raw *>(a.logits) + row * a.ld;
     const row_params p = params_of(a, row);
-    row_list<16, 8, true> list(s.list);
     const uint32_t top_key = row_top(c, r);
     if (!top_key) {
         if (threadIdx.x == 0) write_empty(a, row);
@@ -936,126 +985,150 @@ __global__ __launch_bounds__(1024) void sample_row_kernel(sample_args a, chunk_s
 
     uint32_t K = 1, I = 0xFFFFFFFFu;
     if (filtered) {
-        const int place = static_cast<int>(list.place(0)), chunk = place / c.cap, first = place % c.cap;
-        const int n = chunk < c.chunks ? static_cast<int>(c.count[chunk0 + chunk]) - first : 0;
-        const uint2 *slot = c.slot + (chunk0 + chunk) * c.cap + first;
-        uint64_t mine = 0;
-        uint32_t count = 0;
-#pragma unroll
-        for (int e = 0; e < 8; ++e) {
-            const uint2 v = e < n ? slot[e] : make_uint2(0xFF800000u, 0);   // -infinity
-            const float l = __uint_as_float(v.x);
-            list.set(e, l, top, p.per, 0.0f, 8.0f);
-            list.given[e] = v.y;
-            if (static_cast<int>(half_bit(z_of(l, top, p.per))) > whole) list.key[e] = 0;
-            mine += list.key[e] ? list.w[e] : 0u;
-            count += list.key[e] ? 1u : 0u;
+        // Do the candidates hold the kept set?  They do if top-k ends in
+        // them; without top-k, if top-p does, or if min-p lets nothing below
+        // them through.  (Their count and weight by the chunks' sums.)
+        if (threadIdx.x < 64) {
+            s.wide.weight[threadIdx.x] = 0;
+            s.wide.count[threadIdx.x] = 0;
         }
-        // Do they hold the kept set?  They do if top-k ends in them; without
-        // top-k, if top-p does, or if min-p lets nothing below them through.
-        bool enough = whole == 63;
+        __syncthreads();
+        {
+            uint64_t w = 0;
+            uint32_t n = 0;
+            for (int i = wave; i < c.chunks; i += 16) {
+                const uint64_t v = c.bins[(chunk0 + i) * 64 + lane];
+                w += v & kWeightMask;
+                n += static_cast<uint32_t>(v >> kCountShift);
+            }
+            if (n) {
+                atomicAdd(reinterpret_cast<unsigned long long *>(&s.wide.weight[lane]), w);
+                atomicAdd(&s.wide.count[lane], n);
+            }
+        }
+        __syncthreads();
+        const uint64_t upto_w = wave_scan(s.wide.weight[lane]);
+        const uint32_t upto_n = wave_scan(s.wide.count[lane]);
         const uint64_t need = p.k ? p.k : max(share(p.p, weight), uint64_t{1});
-        const uint64_t have = list.total(p.k ? count : mine);   // (its barriers follow the clearing of the bins)
-        enough |= have >= need;
+        bool enough = whole == 63;
+        if (whole >= 0) enough |= (p.k ? lane_value(upto_n, whole) : lane_value(upto_w, whole)) >= need;
         enough |= !p.k && e_of(-0.5f * static_cast<float>(whole + 1)) * 1.0001f < p.min_e;
         if (enough) {
+            if (wave >= 4) return;   // the first four waves hold the candidates; the others' end does not hold a barrier
+            row_list<4, 8, true> list(s.narrow);
+            const int place = static_cast<int>(list.place(0)), chunk = place / c.cap, first = place % c.cap;
+            const int n = chunk < c.chunks ? static_cast<int>(c.count[chunk0 + chunk]) - first : 0;
+            const uint4 *slot = reinterpret_cast<const uint4 *>(c.slot + (chunk0 + min(chunk, c.chunks - 1)) * c.cap + first);
+            uint4 v[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) v[i] = slot[i];
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                const float l = e < n ? __uint_as_float(e % 2 ? v[e / 2].z : v[e / 2].x) : -INFINITY;
+                list.set(e, l, top, p.per, 0.0f, list.kBinsPerBit);
+                list.given[e] = e % 2 ? v[e / 2].w : v[e / 2].y;
+                if (static_cast<int>(half_bit(z_of(l, top, p.per))) > whole) list.key[e] = 0;
+            }
+            __syncthreads();
             list.filter(p.k, p.k ? p.p : 1u << 24, p.k ? 0 : need);
             list.draw(a, row, p, top, list.drop(p.min_e, top, p.per), 0, 0);
             return;
         }
 
-        // A wide set: the half-bit where the weight crosses `need`.
-        bool stream = p.k != 0;
-        uint32_t b = 0;
-        if (!stream) {
+        // A wide set.  The end of the kept prefix lies in half-bit b, `rest`
+        // of the count or weight into it.
+        const auto end_in = [&](uint32_t b, bool by_weight, uint64_t rest) {
             auto &wide = s.wide;
-            if (threadIdx.x < 64) {
-                wide.weight[threadIdx.x] = 0;
-                wide.count[threadIdx.x] = 0;
-            }
-            __syncthreads();
-            uint64_t w = 0;
-            uint32_t n_b = 0;
+            const uint32_t n_all = uniform(wide.count[b]);
+            const uint64_t above = b ? lane_value(upto_w, static_cast<int>(b) - 1) : 0;
+            // Each chunk's weight above the half-bit, and where its elements of it go.
             for (int i = wave; i < c.chunks; i += 16) {
                 const uint64_t v = c.bins[(chunk0 + i) * 64 + lane];
-                w += v & kWeightMask;
-                n_b += static_cast<uint32_t>(v >> kCountShift);
+                const uint64_t sum = wave_total(static_cast<uint32_t>(lane) < b ? v & kWeightMask : 0);
+                if (lane == 0) {
+                    s.sums[i] = sum;
+                    wide.offset[i] = static_cast<uint32_t>(c.bins[(chunk0 + i) * 64 + b] >> kCountShift);
+                }
             }
-            atomicAdd(reinterpret_cast<unsigned long long *>(&wide.weight[lane]), w);
-            atomicAdd(&wide.count[lane], n_b);
             __syncthreads();
-            const uint64_t upto = wave_scan(wide.weight[lane]);
-            b = static_cast<uint32_t>(__builtin_ctzll(__ballot(upto >= need)));
-            const uint64_t above = b ? lane_value(upto, static_cast<int>(b) - 1) : 0;
-            const uint32_t n_all = uniform(wide.count[b]);
-            stream = n_all > kSlots || (p.min_e > 0.0f && e_of(-0.5f * static_cast<float>(b + 1)) <= p.min_e * 1.0001f);
-            if (!stream) {
-                // Each chunk's weight above the half-bit, and where its elements of it go.
-                for (int i = wave; i < c.chunks; i += 16) {
-                    const uint64_t v = c.bins[(chunk0 + i) * 64 + lane];
-                    const uint64_t sum = wave_total(static_cast<uint32_t>(lane) < b ? v & kWeightMask : 0);
-                    if (lane == 0) {
-                        s.sums[i] = sum;
-                        wide.offset[i] = static_cast<uint32_t>(c.bins[(chunk0 + i) * 64 + b] >> kCountShift);
-                    }
+            if (wave == 0) {
+                uint32_t before = 0;
+                for (int i = 0; i < c.chunks; i += 64) {
+                    const uint32_t v = i + lane < c.chunks ? wide.offset[i + lane] : 0;
+                    const uint32_t through = before + wave_scan(v);
+                    if (i + lane < c.chunks) wide.offset[i + lane] = through - v;
+                    before = lane_value(through, 63);
                 }
-                __syncthreads();
-                if (wave == 0) {
-                    uint32_t before = 0;
-                    for (int i = 0; i < c.chunks; i += 64) {
-                        const uint32_t v = i + lane < c.chunks ? wide.offset[i + lane] : 0;
-                        const uint32_t through = before + wave_scan(v);
-                        if (i + lane < c.chunks) wide.offset[i + lane] = through - v;
-                        before = lane_value(through, 63);
-                    }
-                }
-                __syncthreads();
-                for (int i = wave; i < c.chunks; i += 16) {
-                    uint32_t at = uniform(wide.offset[i]);
-                    const uint32_t end = i + 1 < c.chunks ? uniform(wide.offset[i + 1]) : n_all;
-                    for (int v = 0; v < 8 && at < end; ++v) {
-                        const int index = i * kChunk + v * 512 + lane * 8;
-                        float l[8];
-                        load_logits<T>(logits, index, a.V, l);
-                        uint32_t in = 0;
-#pragma unroll
-                        for (int e = 0; e < 8; ++e) {
-                            if (infinite) l[e] = finite_of(l[e]);
-                            const float z = z_of(l[e], top, p.per);
-                            in |= ((half_bit(z) == b) & (w_of(z) != 0)) ? 1u << e : 0u;
-                        }
-                        const uint32_t through = wave_scan(static_cast<uint32_t>(__popc(in)));
-                        uint32_t to = at + through - static_cast<uint32_t>(__popc(in));
-#pragma unroll
-                        for (int e = 0; e < 8; ++e)
-                            if (in >> e & 1)
-                                wide.slot[to++] = make_uint2(__float_as_uint(l[e]), static_cast<uint32_t>(index + e));
-                        at += lane_value(through, 63);
-                    }
-                }
-                __syncthreads();
-                row_list<16, 8, true> part(s.list);
-                __syncthreads();
-#pragma unroll
-                for (int e = 0; e < 8; ++e) {
-                    const uint32_t at = part.place(e);
-                    const uint2 v = at < n_all ? wide.slot[at] : make_uint2(0xFF800000u, 0);
-                    // 1/512 of a bit a bin: the half-bit's part of z
-                    part.set(e, __uint_as_float(v.x), top, p.per, 0.5f * static_cast<float>(b), 512.0f);
-                    part.given[e] = v.y;
-                }
-                part.filter(0, 1u << 24, need - above);
-                K = part.K;
-                I = part.I;
-                __syncthreads();
-                weight = above + part.total(part.kept_weight());
-#pragma unroll
-                for (int e = 0; e < 8; ++e)
-                    if (part.kept(e))
-                        atomicAdd(reinterpret_cast<unsigned long long *>(&s.sums[part.given[e] / kChunk]), part.w[e]);
             }
+            __syncthreads();
+            for (int i = wave; i < c.chunks; i += 16) {
+                uint32_t at = uniform(wide.offset[i]);
+                const uint32_t end = i + 1 < c.chunks ? uniform(wide.offset[i + 1]) : n_all;
+                for (int v = 0; v < 8 && at < end; ++v) {
+                    const int index = i * kChunk + v * 512 + lane * 8;
+                    float l[8];
+                    load_logits<T>(logits, index, a.V, l);
+                    uint32_t in = 0;
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) {
+                        if (infinite) l[e] = finite_of(l[e]);
+                        const float z = z_of(l[e], top, p.per);
+                        in |= ((half_bit(z) == b) & (w_of(z) != 0)) ? 1u << e : 0u;
+                    }
+                    const uint32_t through = wave_scan(static_cast<uint32_t>(__popc(in)));
+                    uint32_t to = at + through - static_cast<uint32_t>(__popc(in));
+#pragma unroll
+                    for (int e = 0; e < 8; ++e)
+                        if (in >> e & 1)
+                            wide.slot[to++] = make_uint2(__float_as_uint(l[e]), static_cast<uint32_t>(index + e));
+                    at += lane_value(through, 63);
+                }
+            }
+            __syncthreads();
+            row_list<16, 8, true> part(s.list);
+            __syncthreads();
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                const uint32_t at = part.place(e);
+                const uint2 v = at < n_all ? wide.slot[at] : make_uint2(0xFF800000u, 0);   // -infinity
+                // the bins over this half-bit's part of z
+                part.set(e, __uint_as_float(v.x), top, p.per, 0.5f * static_cast<float>(b), 64.0f * part.kBinsPerBit);
+                part.given[e] = v.y;
+            }
+            part.K = K;
+            part.I = I;
+            weight = above + part.filter(0, 1u << 24, rest, by_weight);
+            K = part.K;
+            I = part.I;
+#pragma unroll
+            for (int e = 0; e < 8; ++e)
+                if (part.kept(e))
+                    atomicAdd(reinterpret_cast<unsigned long long *>(&s.sums[part.given[e] / kChunk]), part.w[e]);
+            __syncthreads();
+        };
+        // The half-bit where the sums cross, if it may be taken that way.
+        const auto half_of = [&](uint64_t upto, uint64_t rest, uint32_t &b) {
+            b = static_cast<uint32_t>(__builtin_ctzll(__ballot(upto >= rest)));
+            return uniform(s.wide.count[b]) <= kGathered &&
+                   !(p.min_e > 0.0f && e_of(-0.5f * static_cast<float>(b + 1)) <= p.min_e * 1.0001f);
+        };
+        uint32_t b = 0;
+        bool done = true;
+        uint64_t want = need;
+        if (p.k) {
+            if (need <= lane_value(upto_n, 63)) {
+                done = half_of(upto_n, need, b);
+                if (done) end_in(b, false, need - (b ? lane_value(upto_n, static_cast<int>(b) - 1) : 0));
+            } else {
+                done = !(p.min_e > 0.0f);   // top-k leaves everything, and the sums are of everything
+            }
+            want = p.p < 1u << 24 ? max(share(p.p, weight), uint64_t{1}) : 0;
         }
-        if (stream) {
+        if (done && want) {
+            done = half_of(upto_w, want, b);
+            if (done) end_in(b, true, want - (b ? lane_value(upto_w, static_cast<int>(b) - 1) : 0));
+        }
+        if (!done) {
             __syncthreads();
             row_stream<T> whole_row(s.stream, logits, a.V, top, p.per, infinite);
             if (p.k) whole_row.select(false, p.k);
@@ -1150,7 +1223,6 @@ aq_status launch(aq_ctx *ctx, const sample_args &a) {
     else if (a.V <= 2048) in_registers(sample_short_kernel<T, 4, 8>, 4);
     else if (a.V <= 4096) in_registers(sample_short_kernel<T, 4, 16>, 4);
     else if (a.V <= 8192) in_registers(sample_short_kernel<T, 8, 16>, 8);
-    else if (a.V <= 16384) in_registers(sample_short_kernel<T, 16, 16>, 16);
     else return launch_long<T>(ctx, a);
     return AQ_OK;
 }
