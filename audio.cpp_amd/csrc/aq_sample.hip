@@ -18,11 +18,15 @@ struct sample_args {
     const void *logits;
     int64_t ld, rows;
     int V;
+    // [rows] each; those that the caller left out point to u and have no bit in `given`
     const float *u, *temperature, *top_p, *min_p;
     const int32_t *top_k;
+    uint32_t given;
     int32_t *token;
     float *logp;
 };
+
+enum : uint32_t { kTemperature = 1, kTopK = 2, kTopP = 4, kMinP = 8 };
 
 constexpr int kMaxV = 1 << 20;
 constexpr float kLog2e = 1.4426950408889634f;
@@ -36,18 +40,21 @@ struct row_params {
     uint32_t u;       // in 2^-24
 };
 
+// (All five loads at once: behind tests of the pointers each would wait for
+// the one before.)
 __device__ inline row_params params_of(const sample_args &a, int64_t row) {
+    const float u = a.u[row], temperature = a.temperature[row], top_p = a.top_p[row], min_p = a.min_p[row];
+    const int32_t top_k = a.top_k[row];
     row_params r;
-    const float t = a.temperature ? a.temperature[row] : 1.0f;
-    const bool greedy = !(t > 0.0f);
-    r.per = greedy ? kLog2e : fminf(kLog2e / t, 3.4e38f);
-    const int k = a.top_k ? a.top_k[row] : 0;
-    r.k = greedy ? 1u : k > 0 && k < a.V ? static_cast<uint32_t>(k) : 0u;
-    const float p = a.top_p ? a.top_p[row] : 1.0f;
+    const float degree = a.given & kTemperature ? temperature : 1.0f;
+    const bool greedy = !(degree > 0.0f);
+    r.per = greedy ? kLog2e : fminf(kLog2e / degree, 3.4e38f);
+    const int32_t k = a.given & kTopK ? top_k : 0;
+    r.k = greedy ? 1u : (k > 0) & (k < a.V) ? static_cast<uint32_t>(k) : 0u;
+    const float p = a.given & kTopP ? top_p : 1.0f;
     r.p = p < 1.0f ? static_cast<uint32_t>(fmaxf(p, 0.0f) * 0x1p24f) : 1u << 24;
-    const float m = a.min_p ? a.min_p[row] : 0.0f;
+    const float m = a.given & kMinP ? min_p : 0.0f;
     r.min_e = m > 0.0f ? fminf(m, 1.0f) : 0.0f;
-    const float u = a.u[row];
     r.u = static_cast<uint32_t>(fminf(fmaxf(u, 0.0f), 0x1.fffffep-1f) * 0x1p24f);   // NaN: 0
     return r;
 }
@@ -274,21 +281,36 @@ struct row_list {
         return found;
     }
 
-    // Into LDS: the elements that `in` names, up to 64, and the range of the others' keys.
+    // Into LDS: the elements that `in` names, up to 64, and the range of the
+    // others' keys.  One store of code for all of a thread's elements, taken in
+    // turn: code that runs once costs its fetch.
     template <typename P>
     __device__ void gather(int phase, P &&in) {
+        uint32_t left = 0;
 #pragma unroll
-        for (int e = 0; e < E; ++e) {
-            if (!in(e)) continue;
-            const uint32_t at = atomicAdd(&s.count[phase], 1u);
-            if (at < 64) {
-                s.key[phase][at] = key[e];
-                s.index[phase][at] = index(e);
-                s.weight[phase][at] = w[e];
-            } else {
-                atomicMax(&s.hi[phase], key[e]);
-                atomicMin(&s.lo[phase], key[e]);
+        for (int e = 0; e < E; ++e) left |= in(e) ? 1u << e : 0u;
+        while (__ballot(left != 0)) {
+            uint32_t k = 0, i = 0, weight = 0;
+            const uint32_t lowest = left & (0u - left);
+#pragma unroll
+            for (int e = 0; e < E; ++e) {
+                const bool it = lowest == 1u << e;
+                k = it ? key[e] : k;
+                i = it ? index(e) : i;
+                weight = it ? w[e] : weight;
             }
+            if (left) {
+                const uint32_t at = atomicAdd(&s.count[phase], 1u);
+                if (at < 64) {
+                    s.key[phase][at] = k;
+                    s.index[phase][at] = i;
+                    s.weight[phase][at] = weight;
+                } else {
+                    atomicMax(&s.hi[phase], k);
+                    atomicMin(&s.lo[phase], k);
+                }
+            }
+            left &= left - 1;
         }
     }
 
@@ -938,6 +960,7 @@ template <typename T>
 struct row_lds {
     union {
         list_lds<4> narrow;
+        list_lds<8> draw;
         list_lds<16> list;
     };
     uint64_t sums[kMostChunks];   // kept weight of each chunk
@@ -1061,27 +1084,32 @@ __global__ __launch_bounds__(1024) void sample_row_kernel(sample_args a, chunk_s
                 }
             }
             __syncthreads();
+            const float z_hi = -0.5f * static_cast<float>(b), z_lo = z_hi - 0.5f;   // z of the half-bit: z_lo < z <= z_hi
             for (int i = wave; i < c.chunks; i += 16) {
                 uint32_t at = uniform(wide.offset[i]);
                 const uint32_t end = i + 1 < c.chunks ? uniform(wide.offset[i + 1]) : n_all;
-                for (int v = 0; v < 8 && at < end; ++v) {
-                    const int index = i * kChunk + v * 512 + lane * 8;
-                    float l[8];
-                    load_logits<T>(logits, index, a.V, l);
-                    uint32_t in = 0;
+                for (int v0 = 0; v0 < 8 && at < end; v0 += 4) {
+                    float l[4][8];
 #pragma unroll
-                    for (int e = 0; e < 8; ++e) {
-                        if (infinite) l[e] = finite_of(l[e]);
-                        const float z = z_of(l[e], top, p.per);
-                        in |= ((half_bit(z) == b) & (w_of(z) != 0)) ? 1u << e : 0u;
+                    for (int v = 0; v < 4; ++v)
+                        load_logits<T>(logits, i * kChunk + (v0 + v) * 512 + lane * 8, a.V, l[v]);
+#pragma unroll
+                    for (int v = 0; v < 4; ++v) {
+                        uint32_t in = 0;
+#pragma unroll
+                        for (int e = 0; e < 8; ++e) {
+                            if (infinite) l[v][e] = finite_of(l[v][e]);
+                            const float z = z_of(l[v][e], top, p.per);
+                            in |= ((z <= z_hi) & (z > z_lo)) ? 1u << e : 0u;
+                        }
+                        const uint32_t through = wave_scan(static_cast<uint32_t>(__popc(in)));
+                        uint32_t to = at + through - static_cast<uint32_t>(__popc(in));
+                        at += lane_value(through, 63);
+                        const uint32_t index = static_cast<uint32_t>(i * kChunk + (v0 + v) * 512 + lane * 8);
+#pragma unroll
+                        for (int e = 0; e < 8; ++e)
+                            if (in >> e & 1) wide.slot[to++] = make_uint2(__float_as_uint(l[v][e]), index + e);
                     }
-                    const uint32_t through = wave_scan(static_cast<uint32_t>(__popc(in)));
-                    uint32_t to = at + through - static_cast<uint32_t>(__popc(in));
-#pragma unroll
-                    for (int e = 0; e < 8; ++e)
-                        if (in >> e & 1)
-                            wide.slot[to++] = make_uint2(__float_as_uint(l[e]), static_cast<uint32_t>(index + e));
-                    at += lane_value(through, 63);
                 }
             }
             __syncthreads();
@@ -1109,7 +1137,7 @@ __global__ __launch_bounds__(1024) void sample_row_kernel(sample_args a, chunk_s
         // The half-bit where the sums cross, if it may be taken that way.
         const auto half_of = [&](uint64_t upto, uint64_t rest, uint32_t &b) {
             b = static_cast<uint32_t>(__builtin_ctzll(__ballot(upto >= rest)));
-            return uniform(s.wide.count[b]) <= kGathered &&
+            return b < 61 && uniform(s.wide.count[b]) <= kGathered &&   // (61 and below: not all have a weight)
                    !(p.min_e > 0.0f && e_of(-0.5f * static_cast<float>(b + 1)) <= p.min_e * 1.0001f);
         };
         uint32_t b = 0;
@@ -1172,14 +1200,15 @@ __global__ __launch_bounds__(1024) void sample_row_kernel(sample_args a, chunk_s
         }
     }
     __syncthreads();
+    if (wave >= 8) return;   // a chunk is 8 elements for each of 512 threads
     const int base = static_cast<int>(uniform(static_cast<uint32_t>(s.chunk))) * kChunk;
-    row_list<16, 8, true> drawn(s.list);
+    row_list<8, 8, true> drawn(s.draw);
     const int at = static_cast<int>(drawn.place(0));
     float l[8];
-    load_logits<T>(logits, base + at, at < kChunk ? a.V : 0, l);
+    load_logits<T>(logits, base + at, a.V, l);
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
-        drawn.set(e, infinite ? finite_of(l[e]) : l[e], top, p.per, 0.0f, 8.0f);
+        drawn.set(e, infinite ? finite_of(l[e]) : l[e], top, p.per, 0.0f, drawn.kBinsPerBit);
         drawn.given[e] = static_cast<uint32_t>(base + at + e);
     }
     drawn.K = K;
@@ -1242,7 +1271,18 @@ extern "C" aq_status aq_sample(aq_ctx *ctx, int type, const void *logits, int64_
     if (!logits || !u || !token) return aq_fail(ctx, AQ_E_INVALID_ARG, "aq_sample: null logits, u or token");
     if (ld < V) return aq_fail(ctx, AQ_E_SHAPE, "aq_sample: row stride %lld is below V=%lld", (long long)ld, (long long)V);
     aq_device_guard g(ctx->device);
-    const sample_args a{logits, ld, rows, static_cast<int>(V), u, temperature, top_p, min_p, top_k, token, logp};
+    const sample_args a{logits,
+                        ld,
+                        rows,
+                        static_cast<int>(V),
+                        u,
+                        temperature ? temperature : u,
+                        top_p ? top_p : u,
+                        min_p ? min_p : u,
+                        top_k ? top_k : reinterpret_cast<const int32_t *>(u),
+                        (temperature ? kTemperature : 0u) | (top_k ? kTopK : 0u) | (top_p ? kTopP : 0u) | (min_p ? kMinP : 0u),
+                        token,
+                        logp};
     const aq_status st = type == AQ_T_F32   ? launch<f32>(ctx, a)
                          : type == AQ_T_F16 ? launch<f16>(ctx, a)
                                             : launch<bf16>(ctx, a);
