@@ -197,7 +197,7 @@ struct row_list {
     list_lds<WAVES> &s;
     const int lane = threadIdx.x & 63, wave = static_cast<int>(uniform(threadIdx.x >> 6));
     uint32_t key[E], w[E], bin[E];
-    uint32_t given[GIVEN ? E : 1];
+    uint32_t given[GIVEN ? E : 1], base = 0;
     uint32_t K = 1, I = 0xFFFFFFFFu;   // kept: key > K, or key == K and index <= I
 
     // Clears the bins: a barrier has to follow before filter().
@@ -218,7 +218,7 @@ struct row_list {
     __device__ uint32_t place(int e) const {   // in the list
         return static_cast<uint32_t>(((wave * (E / 8) + e / 8) * 64 + lane) * 8 + e % 8);
     }
-    __device__ uint32_t index(int e) const { return GIVEN ? given[e] : place(e); }
+    __device__ uint32_t index(int e) const { return GIVEN ? given[e] : base + place(e); }
 
     // No branches in the tests of elements: they are a few comparisons, and
     // ROCm 7.2's compiler has dropped the copy of a 64-bit value that a
@@ -502,18 +502,21 @@ struct row_list {
         __syncthreads();
         bin_sums b;
         scan_bins(b);
-        uint64_t weight = b.all_w, before = 0;   // kept
-        uint32_t chosen = 0;
-        if (k && k <= b.all_n) {
-            uint64_t rest = k;
-            crossing(b, 0, false, rest, chosen, before);
-            weight = before + resolve(chosen, 0, false, rest);
-        }
-        if (p < 1u << 24) need = max(share(p, weight), uint64_t{1});
-        // (The sums of bins behind top-k's end are too large, but it is crossed before.)
-        if (need && need <= (by_weight ? b.all_w : b.all_n)) {
-            crossing(b, 1, by_weight, need, chosen, before);
-            weight = before + resolve(chosen, 1, by_weight, need);
+        uint64_t weight = b.all_w;   // kept
+        // Phase 0: top-k's end; phase 1: top-p's (or that of `need`).  (The sums
+        // of bins behind top-k's end are too large then, but it is crossed
+        // before.)  One loop, so that the code is there, and fetched, once.
+#pragma unroll 1
+        for (int phase = 0; phase < 2; ++phase) {
+            uint64_t rest = need;
+            if (phase == 0) rest = k;
+            else if (p < 1u << 24) rest = max(share(p, weight), uint64_t{1});
+            const bool weights = phase && by_weight;
+            if (!rest || rest > (weights ? b.all_w : b.all_n)) continue;
+            uint32_t chosen = 0;
+            uint64_t before = 0;
+            crossing(b, phase, weights, rest, chosen, before);
+            weight = before + resolve(chosen, phase, weights, rest);
         }
         return weight;
     }
@@ -610,24 +613,27 @@ __global__ __launch_bounds__(64 * WAVES) void sample_short_kernel(sample_args a)
     list.draw(a, row, r, top, list.drop(r.min_e, top, r.per), 0, 0);
 }
 
-// Longer rows: chunks of 4096 elements, a block each, in three launches.
+// Longer rows: chunks of 4096 elements, a block each, in four launches.
 //
 //  1. the largest logit of each chunk;
 //  2. the weights, relative to the row's largest, and their sum over the
 //     chunk; for rows with filters also the chunk's count and weight per
 //     half-bit of weight, and its candidates: the elements of its largest
 //     half-bits, in index order, as many whole ones as fit its slots;
-//  3. a block per row.  Without filters it finds the chunk that the draw falls
-//     into from the sums, and draws in it.  With filters it works on the
+//  3. a small block per row.  Without filters it finds the chunk that the draw
+//     falls into from the sums, and draws in it.  With filters it works on the
 //     candidates down to the least half-bit that every chunk has given whole,
-//     which hold the kept set unless that is wide.  A wide one ends in a
-//     half-bit that the sums tell (top-k's end, then top-p's): its elements are
-//     collected from the chunks and decide where, and the sums over what lies
-//     above it decide the chunk to draw in.  What is left (min-p's end in a
-//     wide set, more than 8192 elements in half a bit) streams the row.
+//     which hold the kept set unless that is wide;
+//  4. where a row may be filtered, a large block per row that is left, if any.
+//     A wide set ends in a half-bit that the sums tell (top-k's end, then
+//     top-p's): its elements are collected from the chunks and decide where,
+//     and the sums over what lies above it decide the chunk to draw in.  What
+//     is left even then (min-p's end in a wide set, more than 8192 elements in
+//     half a bit) streams the row.
 constexpr int kChunk = 4096;          // 256 threads, 16 elements each
 constexpr int kSlots = 2048;          // candidates of a row: 256 threads, 8 each
-constexpr int kGathered = 8192;       // elements of a half-bit: 1024 threads, 8 each
+constexpr int kWideWaves = 8;         // of a block in the fourth launch: with twice as many its registers spill
+constexpr int kGathered = 8192;       // elements of a half-bit: 16 for each of its threads
 constexpr int kMostChunks = kMaxV / kChunk;
 constexpr int kRowsAtOnce = 256;
 
@@ -638,6 +644,7 @@ struct chunk_store {
     uint32_t *top;      // [rows][chunks] largest key
     uint32_t *count;    // [rows][chunks] candidates
     int32_t *whole;     // [rows][chunks] the last half-bit given whole, -1: none
+    uint32_t *left;     // [rows] 1: for the fourth launch
     int chunks, cap;
 };
 
@@ -754,7 +761,7 @@ __global__ __launch_bounds__(256) void sample_chunk_kernel(sample_args a, chunk_
     }
 }
 
-// A row streamed from memory by a block of 16 waves: wave w has the run of
+// A row streamed from memory by a block of 8 waves: wave w has the run of
 // whole vectors of 512 elements from w * run on, so that the waves' sums in
 // order give index order.
 template <typename T>
@@ -762,7 +769,7 @@ struct row_stream {
     using raw = typename T::raw;
     struct lds {
         uint64_t bins[2048];
-        uint64_t part[16];
+        uint64_t part[kWideWaves];
         uint32_t key[64], index[64], weight[64];
         uint32_t count, hi, lo, chosen;
         uint64_t before;
@@ -777,7 +784,7 @@ struct row_stream {
     uint32_t K = 1, I = 0xFFFFFFFFu;
 
     __device__ row_stream(lds &l, const raw *p, int n, float t, float f, bool inf)
-        : s(l), logits(p), V(n), top(t), per(f), infinite(inf), run((n + 8191) / 8192 * 512), begin(min(wave * run, n)),
+        : s(l), logits(p), V(n), top(t), per(f), infinite(inf), run((n + 512 * kWideWaves - 1) / (512 * kWideWaves) * 512), begin(min(wave * run, n)),
           end(min(begin + run, n)) {}
 
     __device__ bool kept(uint32_t key, int i) const {
@@ -812,14 +819,14 @@ struct row_stream {
         __syncthreads();
         if (lane == 0) s.part[wave] = mine;
         __syncthreads();
-        return wave_total(lane < 16 ? s.part[lane] : 0);
+        return wave_total(lane < kWideWaves ? s.part[lane] : 0);
     }
 
     // After total(amount): true in the thread of the first element where the
     // running sum exceeds t, with its index and logit.
     template <typename A>
     __device__ bool first_over(A &&amount, uint64_t t, int &its_index, float &its_logit) {
-        const uint64_t sums = wave_scan(lane < 16 ? s.part[lane] : 0);
+        const uint64_t sums = wave_scan(lane < kWideWaves ? s.part[lane] : 0);
         uint64_t before = wave ? lane_value(sums, wave - 1) : 0;
         if (t < before || t >= lane_value(sums, wave)) return false;
         for (int i = begin; i < end; i += 512) {
@@ -858,8 +865,7 @@ struct row_stream {
         };
         for (;;) {
             __syncthreads();
-            s.bins[threadIdx.x] = 0;
-            s.bins[threadIdx.x + 1024] = 0;
+            for (int b = threadIdx.x; b < 2048; b += 64 * kWideWaves) s.bins[b] = 0;
             if (threadIdx.x == 0) {
                 s.count = 0;
                 s.hi = 0;
@@ -956,36 +962,83 @@ struct row_stream {
     }
 };
 
-template <typename T>
-struct row_lds {
-    union {
-        list_lds<4> narrow;
-        list_lds<8> draw;
-        list_lds<16> list;
-    };
-    uint64_t sums[kMostChunks];   // kept weight of each chunk
-    union {
-        typename row_stream<T>::lds stream;
-        struct {
-            uint2 slot[kGathered];
-            uint32_t offset[kMostChunks];
-            uint64_t weight[64];
-            uint32_t count[64];
-        } wide;
-    };
-    uint64_t before;
-    int chunk;
+// The weight and count of a row's half-bits through half-bit `lane`, from its
+// chunks; every wave of a block takes part.
+struct half_bits {
+    uint64_t weight[64];
+    uint32_t count[64];
 };
+__device__ inline void sum_half_bits(const chunk_store &c, int64_t chunk0, half_bits &s, uint64_t &upto_w, uint32_t &upto_n) {
+    const int lane = threadIdx.x & 63, wave = static_cast<int>(uniform(threadIdx.x >> 6)), waves = blockDim.x >> 6;
+    if (threadIdx.x < 64) {
+        s.weight[threadIdx.x] = 0;
+        s.count[threadIdx.x] = 0;
+    }
+    __syncthreads();
+    uint64_t w = 0;
+    uint32_t n = 0;
+    for (int i = wave; i < c.chunks; i += waves) {
+        const uint64_t v = c.bins[(chunk0 + i) * 64 + lane];
+        w += v & kWeightMask;
+        n += static_cast<uint32_t>(v >> kCountShift);
+    }
+    if (n) {
+        atomicAdd(reinterpret_cast<unsigned long long *>(&s.weight[lane]), w);
+        atomicAdd(&s.count[lane], n);
+    }
+    __syncthreads();
+    upto_w = wave_scan(s.weight[lane]);
+    upto_n = wave_scan(s.count[lane]);
+}
+
+// The draw in the chunk where the running weight over `sums` (device or LDS,
+// one per chunk) exceeds share(u, weight), among what K and I keep.
+template <typename T, int WAVES, int E>
+__device__ inline void draw_in_chunk(const sample_args &a, const chunk_store &c, int64_t row, const row_params &p,
+                                     const uint64_t *sums, uint64_t weight, float top, bool infinite, uint32_t K,
+                                     uint32_t I, list_lds<WAVES> &lds) {
+    static_assert(64 * WAVES * E == kChunk, "");
+    row_list<WAVES, E> list(lds);
+    // Every wave finds the chunk for itself.
+    const uint64_t t = share(p.u, weight);
+    uint64_t before = 0;
+    int chunk = 0;
+    for (int i = 0; i < c.chunks; i += 64) {
+        const uint64_t v = i + list.lane < c.chunks ? sums[i + list.lane] : 0;
+        const uint64_t upto = before + wave_scan(v);
+        const uint64_t over = __ballot(upto > t);
+        if (over) {
+            const int owner = __builtin_ctzll(over);
+            chunk = i + owner;
+            before = lane_value(upto - v, owner);
+            break;
+        }
+        before = lane_value(upto, 63);
+    }
+    const int base = chunk * kChunk;
+    const typename T::raw *logits = static_cast<const typename T::raw *>(a.logits) + row * a.ld;
+#pragma unroll
+    for (int v = 0; v < E / 8; ++v) {
+        float l[8];
+        load_logits<T>(logits, base + static_cast<int>(list.place(8 * v)), a.V, l);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) list.set(8 * v + e, infinite ? finite_of(l[e]) : l[e], top, p.per, 0.0f, list.kBinsPerBit);
+    }
+    list.base = static_cast<uint32_t>(base);
+    list.K = K;
+    list.I = I;
+    list.draw(a, row, p, top, list.drop(p.min_e, top, p.per), weight, t - before);
+}
 
 template <typename T>
-__global__ __launch_bounds__(1024) void sample_row_kernel(sample_args a, chunk_store c, int64_t row0) {
-    __shared__ row_lds<T> s;
-    using raw = typename T::raw;
-    const int lane = threadIdx.x & 63, wave = static_cast<int>(uniform(threadIdx.x >> 6));
+__global__ __launch_bounds__(256) void sample_row_kernel(sample_args a, chunk_store c, int64_t row0) {
+    __shared__ list_lds<4> lds;
+    __shared__ half_bits sums;
+    const int lane = threadIdx.x & 63;
     const int64_t r = blockIdx.x, row = row0 + r, chunk0 = r * c.chunks;
-    const raw *logits = static_cast<const raw *>(a.logits) + row * a.ld;
     const row_params p = params_of(a, row);
     const uint32_t top_key = row_top(c, r);
+    if (threadIdx.x == 0) c.left[r] = 0;
     if (!top_key) {
         if (threadIdx.x == 0) write_empty(a, row);
         return;
@@ -998,74 +1051,114 @@ __global__ __launch_bounds__(1024) void sample_row_kernel(sample_args a, chunk_s
     int whole = 63;
     uint64_t weight = 0;
     for (int i = lane; i < c.chunks; i += 64) {
-        const uint64_t w = c.weight[chunk0 + i];
-        weight += w;
-        if (wave == 0) s.sums[i] = w;
+        weight += c.weight[chunk0 + i];
         if (filtered) whole = min(whole, c.whole[chunk0 + i]);
     }
     weight = wave_total(weight);
     whole = static_cast<int>(63u - wave_max(static_cast<uint32_t>(63 - whole)));
+    if (!filtered) {
+        draw_in_chunk<T, 4, 16>(a, c, row, p, c.weight + chunk0, weight, top, infinite, 1, 0xFFFFFFFFu, lds);
+        return;
+    }
 
+    // The candidates.
+    row_list<4, 8, true> list(lds);
+    const int place = static_cast<int>(list.place(0)), chunk = place / c.cap, first = place % c.cap;
+    const int n = chunk < c.chunks ? static_cast<int>(c.count[chunk0 + chunk]) - first : 0;
+    const uint4 *slot = reinterpret_cast<const uint4 *>(c.slot + (chunk0 + min(chunk, c.chunks - 1)) * c.cap + first);
+    uint4 v[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) v[i] = slot[i];
+    // Do they hold the kept set?  They do if top-k ends in them; without
+    // top-k, if top-p does, or if min-p lets nothing below them through.
+    uint64_t upto_w;
+    uint32_t upto_n;
+    sum_half_bits(c, chunk0, sums, upto_w, upto_n);
+    const uint64_t need = p.k ? p.k : max(share(p.p, weight), uint64_t{1});
+    bool enough = whole == 63;
+    if (whole >= 0) enough |= (p.k ? lane_value(upto_n, whole) : lane_value(upto_w, whole)) >= need;
+    enough |= !p.k && e_of(-0.5f * static_cast<float>(whole + 1)) * 1.0001f < p.min_e;
+    if (!enough) {
+        if (threadIdx.x == 0) c.left[r] = 1;
+        return;
+    }
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+        const float l = e < n ? __uint_as_float(e % 2 ? v[e / 2].z : v[e / 2].x) : -INFINITY;
+        list.set(e, l, top, p.per, 0.0f, list.kBinsPerBit);
+        list.given[e] = e % 2 ? v[e / 2].w : v[e / 2].y;
+        if (static_cast<int>(half_bit(z_of(l, top, p.per))) > whole) list.key[e] = 0;
+    }
+    list.filter(p.k, p.k ? p.p : 1u << 24, p.k ? 0 : need);
+    list.draw(a, row, p, top, list.drop(p.min_e, top, p.per), 0, 0);
+}
+
+template <typename T>
+struct wide_lds {
+    list_lds<kWideWaves> list;
+    uint64_t sums[kMostChunks];   // kept weight of each chunk
+    union {
+        typename row_stream<T>::lds stream;
+        struct {
+            uint2 slot[kGathered];
+            uint32_t offset[kMostChunks];
+            half_bits half;
+        } wide;
+    };
+};
+
+template <typename T>
+__global__ __launch_bounds__(64 * kWideWaves) void sample_wide_kernel(sample_args a, chunk_store c, int64_t row0) {
+    __shared__ wide_lds<T> s;
+    const int64_t r = blockIdx.x;
+    if (!c.left[r]) return;
+    using raw = typename T::raw;
+    const int lane = threadIdx.x & 63, wave = static_cast<int>(uniform(threadIdx.x >> 6));
+    const int64_t row = row0 + r, chunk0 = r * c.chunks;
+    const raw *logits = static_cast<const raw *>(a.logits) + row * a.ld;
+    const row_params p = params_of(a, row);
+    const uint32_t top_key = row_top(c, r);
+    const bool infinite = is_infinite(logit_of(top_key));
+    const float top = infinite ? 0.0f : logit_of(top_key);
+
+    uint64_t weight = 0;
+    for (int i = lane; i < c.chunks; i += 64) {
+        const uint64_t w = c.weight[chunk0 + i];
+        weight += w;
+        if (wave == 0) s.sums[i] = w;
+    }
+    weight = wave_total(weight);
+    uint64_t upto_w;
+    uint32_t upto_n;
+    sum_half_bits(c, chunk0, s.wide.half, upto_w, upto_n);
     uint32_t K = 1, I = 0xFFFFFFFFu;
-    if (filtered) {
-        // Do the candidates hold the kept set?  They do if top-k ends in
-        // them; without top-k, if top-p does, or if min-p lets nothing below
-        // them through.  (Their count and weight by the chunks' sums.)
-        if (threadIdx.x < 64) {
-            s.wide.weight[threadIdx.x] = 0;
-            s.wide.count[threadIdx.x] = 0;
-        }
-        __syncthreads();
-        {
-            uint64_t w = 0;
-            uint32_t n = 0;
-            for (int i = wave; i < c.chunks; i += 16) {
-                const uint64_t v = c.bins[(chunk0 + i) * 64 + lane];
-                w += v & kWeightMask;
-                n += static_cast<uint32_t>(v >> kCountShift);
+    {
+        // A wide set.  Phase 0: top-k's end; phase 1: top-p's.  The half-bit b
+        // where the sums cross holds it, `rest` of the count or weight into it.
+        bool done = true;
+#pragma unroll 1
+        for (int phase = 0; phase < 2; ++phase) {
+            const bool by_weight = phase != 0;
+            uint64_t rest = p.k;
+            if (phase == 1) rest = p.p < 1u << 24 ? max(share(p.p, weight), uint64_t{1}) : 0;
+            if (!rest) continue;
+            if (phase == 0 && rest > lane_value(upto_n, 63)) {   // top-k leaves everything, and the sums are of everything
+                done = !(p.min_e > 0.0f);
+                if (!done) break;
+                continue;
             }
-            if (n) {
-                atomicAdd(reinterpret_cast<unsigned long long *>(&s.wide.weight[lane]), w);
-                atomicAdd(&s.wide.count[lane], n);
-            }
-        }
-        __syncthreads();
-        const uint64_t upto_w = wave_scan(s.wide.weight[lane]);
-        const uint32_t upto_n = wave_scan(s.wide.count[lane]);
-        const uint64_t need = p.k ? p.k : max(share(p.p, weight), uint64_t{1});
-        bool enough = whole == 63;
-        if (whole >= 0) enough |= (p.k ? lane_value(upto_n, whole) : lane_value(upto_w, whole)) >= need;
-        enough |= !p.k && e_of(-0.5f * static_cast<float>(whole + 1)) * 1.0001f < p.min_e;
-        if (enough) {
-            if (wave >= 4) return;   // the first four waves hold the candidates; the others' end does not hold a barrier
-            row_list<4, 8, true> list(s.narrow);
-            const int place = static_cast<int>(list.place(0)), chunk = place / c.cap, first = place % c.cap;
-            const int n = chunk < c.chunks ? static_cast<int>(c.count[chunk0 + chunk]) - first : 0;
-            const uint4 *slot = reinterpret_cast<const uint4 *>(c.slot + (chunk0 + min(chunk, c.chunks - 1)) * c.cap + first);
-            uint4 v[4];
-#pragma unroll
-            for (int i = 0; i < 4; ++i) v[i] = slot[i];
-#pragma unroll
-            for (int e = 0; e < 8; ++e) {
-                const float l = e < n ? __uint_as_float(e % 2 ? v[e / 2].z : v[e / 2].x) : -INFINITY;
-                list.set(e, l, top, p.per, 0.0f, list.kBinsPerBit);
-                list.given[e] = e % 2 ? v[e / 2].w : v[e / 2].y;
-                if (static_cast<int>(half_bit(z_of(l, top, p.per))) > whole) list.key[e] = 0;
-            }
-            __syncthreads();
-            list.filter(p.k, p.k ? p.p : 1u << 24, p.k ? 0 : need);
-            list.draw(a, row, p, top, list.drop(p.min_e, top, p.per), 0, 0);
-            return;
-        }
-
-        // A wide set.  The end of the kept prefix lies in half-bit b, `rest`
-        // of the count or weight into it.
-        const auto end_in = [&](uint32_t b, bool by_weight, uint64_t rest) {
+            const uint64_t upto = by_weight ? upto_w : upto_n;
+            const uint32_t b = static_cast<uint32_t>(__builtin_ctzll(__ballot(upto >= rest)));
+            // (61 and below: not all have a weight)
+            done = b < 61 && uniform(s.wide.half.count[b]) <= kGathered &&
+                   !(p.min_e > 0.0f && e_of(-0.5f * static_cast<float>(b + 1)) <= p.min_e * 1.0001f);
+            if (!done) break;
+            rest -= b ? lane_value(upto, static_cast<int>(b) - 1) : 0;
             auto &wide = s.wide;
-            const uint32_t n_all = uniform(wide.count[b]);
+            const uint32_t n_all = uniform(wide.half.count[b]);
             const uint64_t above = b ? lane_value(upto_w, static_cast<int>(b) - 1) : 0;
             // Each chunk's weight above the half-bit, and where its elements of it go.
-            for (int i = wave; i < c.chunks; i += 16) {
+            for (int i = wave; i < c.chunks; i += kWideWaves) {
                 const uint64_t v = c.bins[(chunk0 + i) * 64 + lane];
                 const uint64_t sum = wave_total(static_cast<uint32_t>(lane) < b ? v & kWeightMask : 0);
                 if (lane == 0) {
@@ -1085,16 +1178,16 @@ __global__ __launch_bounds__(1024) void sample_row_kernel(sample_args a, chunk_s
             }
             __syncthreads();
             const float z_hi = -0.5f * static_cast<float>(b), z_lo = z_hi - 0.5f;   // z of the half-bit: z_lo < z <= z_hi
-            for (int i = wave; i < c.chunks; i += 16) {
+            for (int i = wave; i < c.chunks; i += kWideWaves) {
                 uint32_t at = uniform(wide.offset[i]);
                 const uint32_t end = i + 1 < c.chunks ? uniform(wide.offset[i + 1]) : n_all;
-                for (int v0 = 0; v0 < 8 && at < end; v0 += 4) {
-                    float l[4][8];
+                for (int v0 = 0; v0 < 8 && at < end; v0 += 2) {
+                    float l[2][8];
 #pragma unroll
-                    for (int v = 0; v < 4; ++v)
+                    for (int v = 0; v < 2; ++v)
                         load_logits<T>(logits, i * kChunk + (v0 + v) * 512 + lane * 8, a.V, l[v]);
 #pragma unroll
-                    for (int v = 0; v < 4; ++v) {
+                    for (int v = 0; v < 2; ++v) {
                         uint32_t in = 0;
 #pragma unroll
                         for (int e = 0; e < 8; ++e) {
@@ -1113,10 +1206,10 @@ __global__ __launch_bounds__(1024) void sample_row_kernel(sample_args a, chunk_s
                 }
             }
             __syncthreads();
-            row_list<16, 8, true> part(s.list);
+            row_list<kWideWaves, 16, true> part(s.list);
             __syncthreads();
 #pragma unroll
-            for (int e = 0; e < 8; ++e) {
+            for (int e = 0; e < 16; ++e) {
                 const uint32_t at = part.place(e);
                 const uint2 v = at < n_all ? wide.slot[at] : make_uint2(0xFF800000u, 0);   // -infinity
                 // the bins over this half-bit's part of z
@@ -1129,48 +1222,27 @@ __global__ __launch_bounds__(1024) void sample_row_kernel(sample_args a, chunk_s
             K = part.K;
             I = part.I;
 #pragma unroll
-            for (int e = 0; e < 8; ++e)
+            for (int e = 0; e < 16; ++e)
                 if (part.kept(e))
                     atomicAdd(reinterpret_cast<unsigned long long *>(&s.sums[part.given[e] / kChunk]), part.w[e]);
             __syncthreads();
-        };
-        // The half-bit where the sums cross, if it may be taken that way.
-        const auto half_of = [&](uint64_t upto, uint64_t rest, uint32_t &b) {
-            b = static_cast<uint32_t>(__builtin_ctzll(__ballot(upto >= rest)));
-            return b < 61 && uniform(s.wide.count[b]) <= kGathered &&   // (61 and below: not all have a weight)
-                   !(p.min_e > 0.0f && e_of(-0.5f * static_cast<float>(b + 1)) <= p.min_e * 1.0001f);
-        };
-        uint32_t b = 0;
-        bool done = true;
-        uint64_t want = need;
-        if (p.k) {
-            if (need <= lane_value(upto_n, 63)) {
-                done = half_of(upto_n, need, b);
-                if (done) end_in(b, false, need - (b ? lane_value(upto_n, static_cast<int>(b) - 1) : 0));
-            } else {
-                done = !(p.min_e > 0.0f);   // top-k leaves everything, and the sums are of everything
-            }
-            want = p.p < 1u << 24 ? max(share(p.p, weight), uint64_t{1}) : 0;
-        }
-        if (done && want) {
-            done = half_of(upto_w, want, b);
-            if (done) end_in(b, true, want - (b ? lane_value(upto_w, static_cast<int>(b) - 1) : 0));
         }
         if (!done) {
             __syncthreads();
             row_stream<T> whole_row(s.stream, logits, a.V, top, p.per, infinite);
-            if (p.k) whole_row.select(false, p.k);
-            if (p.p < 1u << 24) {
-                const uint64_t of = whole_row.total([&](float l, int i) -> uint64_t {
-                    return whole_row.kept(key_of(l), i) ? w_of(z_of(l, top, p.per)) : 0u;
-                });
-                whole_row.select(true, max(share(p.p, of), uint64_t{1}));
-            }
+            uint64_t total = 0;
+            float min_e = 0.0f;
             const auto amount = [&](float l, int i) -> uint64_t {
                 const float e = e_of(z_of(l, top, p.per));
-                return (whole_row.kept(key_of(l), i) & (e >= p.min_e)) ? whole_of(e * 0x1p31f) : 0u;
+                return (whole_row.kept(key_of(l), i) & (e >= min_e)) ? whole_of(e * 0x1p31f) : 0u;
             };
-            const uint64_t total = whole_row.total(amount);
+#pragma unroll 1
+            for (int phase = 0; phase < 3; ++phase) {   // top-k, top-p, the draw
+                if (phase == 2) min_e = p.min_e;
+                if (phase) total = whole_row.total(amount);
+                const uint64_t rest = phase == 0 ? p.k : phase == 1 && p.p < 1u << 24 ? max(share(p.p, total), uint64_t{1}) : 0;
+                if (rest) whole_row.select(phase != 0, rest);
+            }
             int at = 0;
             float its = 0.0f;
             if (!whole_row.first_over(amount, share(p.u, total), at, its)) return;
@@ -1180,40 +1252,8 @@ __global__ __launch_bounds__(1024) void sample_row_kernel(sample_args a, chunk_s
         }
     }
 
-    // The chunk where the running weight exceeds t, and the draw in it.
     __syncthreads();
-    const uint64_t t = share(p.u, weight);
-    if (wave == 0) {
-        uint64_t before = 0;
-        for (int i = 0; i < c.chunks; i += 64) {
-            const uint64_t v = i + lane < c.chunks ? s.sums[i + lane] : 0;
-            const uint64_t upto = before + wave_scan(v);
-            const uint64_t over = __ballot(upto > t);
-            if (over) {
-                if (lane == __builtin_ctzll(over)) {
-                    s.chunk = i + lane;
-                    s.before = upto - v;
-                }
-                break;
-            }
-            before = lane_value(upto, 63);
-        }
-    }
-    __syncthreads();
-    if (wave >= 8) return;   // a chunk is 8 elements for each of 512 threads
-    const int base = static_cast<int>(uniform(static_cast<uint32_t>(s.chunk))) * kChunk;
-    row_list<8, 8, true> drawn(s.draw);
-    const int at = static_cast<int>(drawn.place(0));
-    float l[8];
-    load_logits<T>(logits, base + at, a.V, l);
-#pragma unroll
-    for (int e = 0; e < 8; ++e) {
-        drawn.set(e, infinite ? finite_of(l[e]) : l[e], top, p.per, 0.0f, drawn.kBinsPerBit);
-        drawn.given[e] = static_cast<uint32_t>(base + at + e);
-    }
-    drawn.K = K;
-    drawn.I = I;
-    drawn.draw(a, row, p, top, drawn.drop(p.min_e, top, p.per), weight, t - s.before);
+    draw_in_chunk<T, kWideWaves, 8>(a, c, row, p, s.sums, weight, top, infinite, K, I, s.list);
 }
 
 template <typename T>
@@ -1223,7 +1263,7 @@ aq_status launch_long(aq_ctx *ctx, const sample_args &a) {
     c.cap = kSlots / c.chunks / 8 * 8;
     const size_t rows = static_cast<size_t>(a.rows < kRowsAtOnce ? a.rows : kRowsAtOnce), n = rows * c.chunks;
     char *at = nullptr;
-    aq_status st = aq_ctx_scratch(ctx, 7, n * (64 * 8 + 8 + c.cap * 8 + 12), reinterpret_cast<void **>(&at));
+    aq_status st = aq_ctx_scratch(ctx, 7, n * (64 * 8 + 8 + c.cap * 8 + 12) + rows * 4, reinterpret_cast<void **>(&at));
     if (st != AQ_OK) return st;
     c.bins = reinterpret_cast<uint64_t *>(at);
     c.weight = c.bins + n * 64;
@@ -1231,12 +1271,15 @@ aq_status launch_long(aq_ctx *ctx, const sample_args &a) {
     c.top = reinterpret_cast<uint32_t *>(c.slot + n * c.cap);
     c.count = c.top + n;
     c.whole = reinterpret_cast<int32_t *>(c.count + n);
+    c.left = c.count + 2 * n;
     for (int64_t row0 = 0; row0 < a.rows; row0 += kRowsAtOnce) {
         const uint32_t now = static_cast<uint32_t>(a.rows - row0 < kRowsAtOnce ? a.rows - row0 : kRowsAtOnce);
         const dim3 grid(static_cast<uint32_t>(c.chunks), now);
         aq_launch_timed(ctx, true, sample_top_kernel<T>, grid, dim3(256), 0u, a, c, row0);
         aq_launch_timed(ctx, true, sample_chunk_kernel<T>, grid, dim3(256), 0u, a, c, row0);
-        aq_launch_timed(ctx, true, sample_row_kernel<T>, dim3(now), dim3(1024), 0u, a, c, row0);
+        aq_launch_timed(ctx, true, sample_row_kernel<T>, dim3(now), dim3(256), 0u, a, c, row0);
+        if (a.given & (kTemperature | kTopK | kTopP))   // a temperature of 0 is a top-k of 1
+            aq_launch_timed(ctx, true, sample_wide_kernel<T>, dim3(now), dim3(64 * kWideWaves), 0u, a, c, row0);
     }
     return AQ_OK;
 }
