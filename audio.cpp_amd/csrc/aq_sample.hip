@@ -562,6 +562,37 @@ __device__ inline void load_logits(const typename T::raw *logits, int at, int V,
     load8<T>(logits, at, V, l, T::store(-INFINITY));
 }
 
+// The same in two steps, so that loads can be ahead of what is done with them.
+template <typename T>
+struct raw8 {
+    typedef uint32_t words __attribute__((ext_vector_type(4)));
+    typedef words any __attribute__((aligned(1)));
+    static constexpr int kWords = sizeof(typename T::raw) / 2;   // 16 bytes each
+    words w[kWords];
+    __device__ void load(const typename T::raw *logits, int at, int V) {
+        if (at + 8 <= V) {
+#pragma unroll
+            for (int i = 0; i < kWords; ++i) w[i] = reinterpret_cast<const any *>(logits + at)[i];
+        } else {
+            float l[8];
+            load_logits<T>(logits, at, V, l);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                const uint32_t bits = bits_of(T::store(l[i]));
+                if (kWords == 2) w[i / 4][i % 4] = bits;
+                else w[0][i / 2] = i % 2 ? w[0][i / 2] | bits << 16 : bits;
+            }
+        }
+    }
+    __device__ void get(float (&l)[8]) const {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            if constexpr (kWords == 2) l[i] = __uint_as_float(w[i / 4][i % 4]);
+            else l[i] = T::load(static_cast<typename T::raw>(w[0][i / 2] >> (i % 2 * 16)));
+        }
+    }
+};
+
 __device__ inline uint32_t largest_key(const float (&l)[8]) {
     float top = l[0];
 #pragma unroll
@@ -613,43 +644,48 @@ __global__ __launch_bounds__(64 * WAVES) void sample_short_kernel(sample_args a)
     list.draw(a, row, r, top, list.drop(r.min_e, top, r.per), 0, 0);
 }
 
-// Longer rows: chunks of 4096 elements, a block each, in four launches.
+// Longer rows: chunks of 8192 elements, a block each, in four launches.
 //
-//  1. the largest logit of each chunk;
+//  1. the largest logit of each chunk, and the row's parameters;
 //  2. the weights, relative to the row's largest, and their sum over the
 //     chunk; for rows with filters also the chunk's count and weight per
-//     half-bit of weight, and its candidates: the elements of its largest
-//     half-bits, in index order, as many whole ones as fit its slots;
+//     quarter of a bit of weight (63 of them, and of all that is below), and
+//     its candidates: the elements of its largest quarters, in index order, as
+//     many whole ones as fit its slots;
 //  3. a small block per row.  Without filters it finds the chunk that the draw
 //     falls into from the sums, and draws in it.  With filters it works on the
-//     candidates down to the least half-bit that every chunk has given whole,
+//     candidates down to the least quarter that every chunk has given whole,
 //     which hold the kept set unless that is wide;
 //  4. where a row may be filtered, a large block per row that is left, if any.
-//     A wide set ends in a half-bit that the sums tell (top-k's end, then
+//     A wide set ends in a quarter that the sums tell (top-k's end, then
 //     top-p's): its elements are collected from the chunks and decide where,
 //     and the sums over what lies above it decide the chunk to draw in.  What
 //     is left even then (min-p's end in a wide set, more than 8192 elements in
-//     half a bit) streams the row.
-constexpr int kChunk = 4096;          // 256 threads, 16 elements each
+//     a quarter, an end below them all) streams the row.
+constexpr int kChunk = 8192;          // 256 threads, 32 elements each
 constexpr int kSlots = 2048;          // candidates of a row: 256 threads, 8 each
 constexpr int kWideWaves = 8;         // of a block in the fourth launch: with twice as many its registers spill
-constexpr int kGathered = 8192;       // elements of a half-bit: 16 for each of its threads
+constexpr int kGathered = 8192;       // elements of a quarter: 16 for each of its threads
 constexpr int kMostChunks = kMaxV / kChunk;
 constexpr int kRowsAtOnce = 256;
 
 struct chunk_store {
-    uint64_t *bins;     // [rows][chunks][64] count and weight of each half-bit, as kCountShift has them
+    uint64_t *bins;     // [rows][chunks][64] count and weight of each quarter, as kCountShift has them
     uint64_t *weight;   // [rows][chunks] sum of weights (of those that min-p leaves, for rows without other filters)
     uint2 *slot;        // [rows][chunks][cap] logit's bits, index
     uint32_t *top;      // [rows][chunks] largest key
     uint32_t *count;    // [rows][chunks] candidates
-    int32_t *whole;     // [rows][chunks] the last half-bit given whole, -1: none
+    int32_t *whole;     // [rows][chunks] the last quarter given whole, -1: none
     uint32_t *left;     // [rows] 1: for the fourth launch
+    row_params *params; // [rows]
     int chunks, cap;
 };
 
-// The half-bit of weight below the largest, 0 to 63.
-__device__ inline uint32_t half_bit(float z) { return min(whole_of(z * -2.0f), 63u); }
+// The quarter of a bit of weight below the largest: 63 for the largest itself,
+// 62 for those above -1/4, and so on; 0: all at or below -15.5 (and a NaN).
+// One fused product and sum, and it does not fall with z.
+__device__ inline uint32_t step_of(float z) { return whole_of(__fmaf_rn(z, 4.0f, 63.0f)); }
+__device__ inline uint32_t quarter(float z) { return 63u - step_of(z); }
 
 template <typename T>
 __global__ __launch_bounds__(256) void sample_top_kernel(sample_args a, chunk_store c, int64_t row0) {
@@ -657,13 +693,18 @@ __global__ __launch_bounds__(256) void sample_top_kernel(sample_args a, chunk_st
     const int64_t r = blockIdx.y;
     const typename T::raw *logits = static_cast<const typename T::raw *>(a.logits) + (row0 + r) * a.ld;
     const int at = static_cast<int>(blockIdx.x) * kChunk + static_cast<int>(threadIdx.x) * 8;
-    float l[2][8];
-    load_logits<T>(logits, at, a.V, l[0]);
-    load_logits<T>(logits, at + 2048, a.V, l[1]);
-    const uint32_t top = wave_max(max(largest_key(l[0]), largest_key(l[1])));
+    float l[4][8];
+#pragma unroll
+    for (int v = 0; v < 4; ++v) load_logits<T>(logits, at + 2048 * v, a.V, l[v]);
+    uint32_t top = 0;
+#pragma unroll
+    for (int v = 0; v < 4; ++v) top = max(top, largest_key(l[v]));
+    top = wave_max(top);
     if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = top;
     __syncthreads();
-    if (threadIdx.x == 0) c.top[r * c.chunks + blockIdx.x] = max(max(part[0], part[1]), max(part[2], part[3]));
+    if (threadIdx.x != 0) return;
+    c.top[r * c.chunks + blockIdx.x] = max(max(part[0], part[1]), max(part[2], part[3]));
+    if (blockIdx.x == 0) c.params[r] = params_of(a, row0 + r);
 }
 
 // The largest key of a row from its chunks'; every wave for itself.
@@ -678,31 +719,32 @@ __global__ __launch_bounds__(256) void sample_chunk_kernel(sample_args a, chunk_
     // Copies of the bins for every wave and every fourth lane: lanes of one
     // wave often meet in a bin.
     constexpr int kCopies = 16;
-    __shared__ uint64_t bins[kCopies][64];
+    __shared__ uint64_t bins[64][kCopies];
     __shared__ uint64_t part[4];
     __shared__ uint32_t counts[4];
+    __shared__ int whole;
     const int lane = threadIdx.x & 63, wave = static_cast<int>(uniform(threadIdx.x >> 6));
     const int64_t r = blockIdx.y, row = row0 + r, chunk = r * c.chunks + blockIdx.x;
     const typename T::raw *logits = static_cast<const typename T::raw *>(a.logits) + row * a.ld;
-    const int base = static_cast<int>(blockIdx.x) * kChunk + (wave * 128 + lane) * 8;   // vectors at +0 and +512
-    float l[2][8];
-    load_logits<T>(logits, base, a.V, l[0]);
-    load_logits<T>(logits, base + 512, a.V, l[1]);
-    const row_params p = params_of(a, row);
+    const int base = static_cast<int>(blockIdx.x) * kChunk + (wave * 256 + lane) * 8;   // four vectors, 512 apart
+    float l[4][8];
+#pragma unroll
+    for (int v = 0; v < 4; ++v) load_logits<T>(logits, base + 512 * v, a.V, l[v]);
+    const row_params p = c.params[r];
     const uint32_t top_key = row_top(c, r);
     if (!top_key) return;   // the whole row is empty
     float top = logit_of(top_key);
     if (is_infinite(top)) {
         top = 0.0f;
 #pragma unroll
-        for (int e = 0; e < 16; ++e) l[e / 8][e % 8] = finite_of(l[e / 8][e % 8]);
+        for (int e = 0; e < 32; ++e) l[e / 8][e % 8] = finite_of(l[e / 8][e % 8]);
     }
     const bool filtered = p.k || p.p < 1u << 24;
 
     uint64_t mine = 0;
     if (!filtered) {
 #pragma unroll
-        for (int e = 0; e < 16; ++e) {
+        for (int e = 0; e < 32; ++e) {
             const float weight = e_of(z_of(l[e / 8][e % 8], top, p.per));
             mine += whole_of(weight >= p.min_e ? weight * 0x1p31f : 0.0f);
         }
@@ -712,53 +754,73 @@ __global__ __launch_bounds__(256) void sample_chunk_kernel(sample_args a, chunk_
         if (threadIdx.x == 0) c.weight[chunk] = part[0] + part[1] + part[2] + part[3];
         return;
     }
+    // Vector instructions are what this kernel takes its time for, so what is
+    // not for an element is for 32 of them, or left to one wave.
 #pragma unroll
-    for (int i = 0; i < 4; ++i) bins[wave * 4 + i][lane] = 0;
+    for (int i = 0; i < 4; ++i) bins[lane][wave * 4 + i] = 0;
     __syncthreads();
-    uint32_t bin[16];
+    uint32_t step[32];
 #pragma unroll
-    for (int e = 0; e < 16; ++e) {
+    for (int e = 0; e < 32; ++e) {
         const float z = z_of(l[e / 8][e % 8], top, p.per);
         const uint32_t w = w_of(z);
-        bin[e] = w ? half_bit(z) : 64u;
-        if (w)
-            atomicAdd(reinterpret_cast<unsigned long long *>(&bins[wave * 4 + (lane & 3)][bin[e]]),
+        step[e] = step_of(z);
+        mine += w;
+        if (step[e])   // not so far below that only the sum counts
+            atomicAdd(reinterpret_cast<unsigned long long *>(&bins[step[e]][wave * 4 + (lane & 3)]),
                       (uint64_t{1} << kCountShift) + w);
     }
+    mine = wave_total(mine);
+    if (lane == 0) part[wave] = mine;
     __syncthreads();
-    uint64_t sum = 0;   // of half-bit `lane`
-#pragma unroll
-    for (int i = 0; i < kCopies; ++i) sum += bins[i][lane];
     if (wave == 0) {
-        c.bins[chunk * 64 + lane] = sum;
-        const uint64_t all = wave_total(sum & kWeightMask);
-        if (lane == 0) c.weight[chunk] = all;
-    }
-    const uint32_t upto = wave_scan(static_cast<uint32_t>(sum >> kCountShift));
-    const int whole = __popcll(__ballot(upto <= static_cast<uint32_t>(c.cap))) - 1;   // upto does not fall with the lane
-
-    // This thread's candidates in both vectors, counted before it in the wave.
-    uint32_t own = 0;
+        uint64_t sum = 0;   // of quarter `lane`
 #pragma unroll
-    for (int e = 0; e < 16; ++e) own += static_cast<int>(bin[e]) <= whole ? (e < 8 ? 1u : 0x10000u) : 0u;
-    const uint32_t through = wave_scan(own);   // no carry between the halves: at most 512 each
-    const uint32_t all = lane_value(through, 63);
-    if (lane == 0) counts[wave] = (all & 0xFFFFu) + (all >> 16);
+        for (int i = 0; i < kCopies; ++i) sum += bins[63 - lane][(i + lane) % kCopies];
+        // What is below all quarters is what they leave of the chunk's weight;
+        // its count matters only as none, or more than any slots hold.
+        const uint64_t all = part[0] + part[1] + part[2] + part[3], above = wave_total(sum & kWeightMask);
+        if (lane == 63) sum = all > above ? (uint64_t{kChunk} << kCountShift) + (all - above) : 0;
+        c.bins[chunk * 64 + lane] = sum;
+        const uint32_t upto = wave_scan(static_cast<uint32_t>(sum >> kCountShift));
+        const int last = __popcll(__ballot(upto <= static_cast<uint32_t>(c.cap))) - 1;   // upto does not fall with the lane
+        if (lane == 0) {
+            c.weight[chunk] = all;
+            c.whole[chunk] = last;
+            whole = last;
+        }
+    }
+    __syncthreads();
+    const uint32_t least = static_cast<uint32_t>(max(63 - whole, 1));   // step of the last quarter given (0 has no weight then)
+
+    // This thread's candidates, 8 bits a vector from the highest down, and how
+    // many of the wave's are before those of each vector.
+    uint32_t in = 0;
+#pragma unroll
+    for (int e = 0; e < 32; ++e) in = in + in + (step[e] >= least ? 1u : 0u);
+    const uint32_t own01 = static_cast<uint32_t>(__popc(in >> 24) | __popc(in >> 16 & 255u) << 16);
+    const uint32_t own23 = static_cast<uint32_t>(__popc(in >> 8 & 255u) | __popc(in & 255u) << 16);
+    const uint32_t to01 = wave_scan(own01), to23 = wave_scan(own23);   // no carry between the halves: at most 512 each
+    const uint32_t all01 = lane_value(to01, 63), all23 = lane_value(to23, 63);
+    const uint32_t n0 = all01 & 0xFFFFu, n1 = n0 + (all01 >> 16), n2 = n1 + (all23 & 0xFFFFu), n3 = n2 + (all23 >> 16);
+    if (lane == 0) counts[wave] = n3;
     __syncthreads();
     uint32_t first = 0;
     for (int i = 0; i < wave; ++i) first += counts[i];
-    if (own) {
-        uint32_t at[2] = {first + ((through - own) & 0xFFFFu), first + (all & 0xFFFFu) + ((through - own) >> 16)};
-#pragma unroll
-        for (int e = 0; e < 16; ++e)
-            if (static_cast<int>(bin[e]) <= whole)
-                c.slot[chunk * c.cap + at[e / 8]++] =
-                    make_uint2(__float_as_uint(l[e / 8][e % 8]), static_cast<uint32_t>(base + (e / 8) * 512 + e % 8));
+    const uint32_t at[4] = {first + ((to01 - own01) & 0xFFFFu), first + n0 + ((to01 - own01) >> 16),
+                            first + n1 + ((to23 - own23) & 0xFFFFu), first + n2 + ((to23 - own23) >> 16)};
+    uint2 *slot = c.slot + chunk * c.cap;
+    uint32_t left = in;
+    while (__ballot(left != 0)) {
+        if (left) {
+            const int bit = 31 - __builtin_clz(left), v = 3 - bit / 8, index = base + v * 512 + 7 - bit % 8;
+            const uint32_t before = static_cast<uint32_t>(__popc(in >> bit & (255u >> bit % 8))) - 1;   // own of this vector
+            const uint32_t to = (v == 0 ? at[0] : v == 1 ? at[1] : v == 2 ? at[2] : at[3]) + before;
+            slot[to] = make_uint2(bits_of(static_cast<float>(T::load(logits[index]))), static_cast<uint32_t>(index));
+            left ^= 1u << bit;
+        }
     }
-    if (threadIdx.x == 0) {
-        c.count[chunk] = counts[0] + counts[1] + counts[2] + counts[3];
-        c.whole[chunk] = whole;
-    }
+    if (threadIdx.x == 0) c.count[chunk] = counts[0] + counts[1] + counts[2] + counts[3];
 }
 
 // A row streamed from memory by a block of 8 waves: wave w has the run of
@@ -962,13 +1024,13 @@ struct row_stream {
     }
 };
 
-// The weight and count of a row's half-bits through half-bit `lane`, from its
+// The weight and count of a row's quarters through quarter `lane`, from its
 // chunks; every wave of a block takes part.
-struct half_bits {
+struct quarter_sums {
     uint64_t weight[64];
     uint32_t count[64];
 };
-__device__ inline void sum_half_bits(const chunk_store &c, int64_t chunk0, half_bits &s, uint64_t &upto_w, uint32_t &upto_n) {
+__device__ inline void sum_quarters(const chunk_store &c, int64_t chunk0, quarter_sums &s, uint64_t &upto_w, uint32_t &upto_n) {
     const int lane = threadIdx.x & 63, wave = static_cast<int>(uniform(threadIdx.x >> 6)), waves = blockDim.x >> 6;
     if (threadIdx.x < 64) {
         s.weight[threadIdx.x] = 0;
@@ -1033,10 +1095,10 @@ __device__ inline void draw_in_chunk(const sample_args &a, const chunk_store &c,
 template <typename T>
 __global__ __launch_bounds__(256) void sample_row_kernel(sample_args a, chunk_store c, int64_t row0) {
     __shared__ list_lds<4> lds;
-    __shared__ half_bits sums;
+    __shared__ quarter_sums sums;
     const int lane = threadIdx.x & 63;
     const int64_t r = blockIdx.x, row = row0 + r, chunk0 = r * c.chunks;
-    const row_params p = params_of(a, row);
+    const row_params p = c.params[r];
     const uint32_t top_key = row_top(c, r);
     if (threadIdx.x == 0) c.left[r] = 0;
     if (!top_key) {
@@ -1047,7 +1109,7 @@ __global__ __launch_bounds__(256) void sample_row_kernel(sample_args a, chunk_st
     const float top = infinite ? 0.0f : logit_of(top_key);
     const bool filtered = p.k || p.p < 1u << 24;
 
-    // The row's weight, and for filtered rows the least half-bit given whole.
+    // The row's weight, and for filtered rows the least quarter given whole.
     int whole = 63;
     uint64_t weight = 0;
     for (int i = lane; i < c.chunks; i += 64) {
@@ -1057,7 +1119,7 @@ __global__ __launch_bounds__(256) void sample_row_kernel(sample_args a, chunk_st
     weight = wave_total(weight);
     whole = static_cast<int>(63u - wave_max(static_cast<uint32_t>(63 - whole)));
     if (!filtered) {
-        draw_in_chunk<T, 4, 16>(a, c, row, p, c.weight + chunk0, weight, top, infinite, 1, 0xFFFFFFFFu, lds);
+        draw_in_chunk<T, 4, 32>(a, c, row, p, c.weight + chunk0, weight, top, infinite, 1, 0xFFFFFFFFu, lds);
         return;
     }
 
@@ -1073,21 +1135,23 @@ __global__ __launch_bounds__(256) void sample_row_kernel(sample_args a, chunk_st
     // top-k, if top-p does, or if min-p lets nothing below them through.
     uint64_t upto_w;
     uint32_t upto_n;
-    sum_half_bits(c, chunk0, sums, upto_w, upto_n);
+    sum_quarters(c, chunk0, sums, upto_w, upto_n);
     const uint64_t need = p.k ? p.k : max(share(p.p, weight), uint64_t{1});
     bool enough = whole == 63;
     if (whole >= 0) enough |= (p.k ? lane_value(upto_n, whole) : lane_value(upto_w, whole)) >= need;
-    enough |= !p.k && e_of(-0.5f * static_cast<float>(whole + 1)) * 1.0001f < p.min_e;
+    enough |= !p.k && e_of(-0.25f * static_cast<float>(whole)) * 1.0001f < p.min_e;
     if (!enough) {
         if (threadIdx.x == 0) c.left[r] = 1;
         return;
     }
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
-        const float l = e < n ? __uint_as_float(e % 2 ? v[e / 2].z : v[e / 2].x) : -INFINITY;
+        float l = __uint_as_float(e % 2 ? v[e / 2].z : v[e / 2].x);
+        if (infinite) l = finite_of(l);
+        l = e < n ? l : -INFINITY;
         list.set(e, l, top, p.per, 0.0f, list.kBinsPerBit);
         list.given[e] = e % 2 ? v[e / 2].w : v[e / 2].y;
-        if (static_cast<int>(half_bit(z_of(l, top, p.per))) > whole) list.key[e] = 0;
+        if (static_cast<int>(quarter(z_of(l, top, p.per))) > whole) list.key[e] = 0;
     }
     list.filter(p.k, p.k ? p.p : 1u << 24, p.k ? 0 : need);
     list.draw(a, row, p, top, list.drop(p.min_e, top, p.per), 0, 0);
@@ -1100,9 +1164,9 @@ struct wide_lds {
     union {
         typename row_stream<T>::lds stream;
         struct {
-            uint2 slot[kGathered];
+            uint32_t slot[kGathered];   // indices
             uint32_t offset[kMostChunks];
-            half_bits half;
+            quarter_sums quarters;
         } wide;
     };
 };
@@ -1116,7 +1180,7 @@ __global__ __launch_bounds__(64 * kWideWaves) void sample_wide_kernel(sample_arg
     const int lane = threadIdx.x & 63, wave = static_cast<int>(uniform(threadIdx.x >> 6));
     const int64_t row = row0 + r, chunk0 = r * c.chunks;
     const raw *logits = static_cast<const raw *>(a.logits) + row * a.ld;
-    const row_params p = params_of(a, row);
+    const row_params p = c.params[r];
     const uint32_t top_key = row_top(c, r);
     const bool infinite = is_infinite(logit_of(top_key));
     const float top = infinite ? 0.0f : logit_of(top_key);
@@ -1130,10 +1194,10 @@ __global__ __launch_bounds__(64 * kWideWaves) void sample_wide_kernel(sample_arg
     weight = wave_total(weight);
     uint64_t upto_w;
     uint32_t upto_n;
-    sum_half_bits(c, chunk0, s.wide.half, upto_w, upto_n);
+    sum_quarters(c, chunk0, s.wide.quarters, upto_w, upto_n);
     uint32_t K = 1, I = 0xFFFFFFFFu;
     {
-        // A wide set.  Phase 0: top-k's end; phase 1: top-p's.  The half-bit b
+        // A wide set.  Phase 0: top-k's end; phase 1: top-p's.  The quarter b
         // where the sums cross holds it, `rest` of the count or weight into it.
         bool done = true;
 #pragma unroll 1
@@ -1149,15 +1213,14 @@ __global__ __launch_bounds__(64 * kWideWaves) void sample_wide_kernel(sample_arg
             }
             const uint64_t upto = by_weight ? upto_w : upto_n;
             const uint32_t b = static_cast<uint32_t>(__builtin_ctzll(__ballot(upto >= rest)));
-            // (61 and below: not all have a weight)
-            done = b < 61 && uniform(s.wide.half.count[b]) <= kGathered &&
-                   !(p.min_e > 0.0f && e_of(-0.5f * static_cast<float>(b + 1)) <= p.min_e * 1.0001f);
+            done = b < 63 && uniform(s.wide.quarters.count[b]) <= kGathered &&
+                   !(p.min_e > 0.0f && e_of(-0.25f * static_cast<float>(b)) <= p.min_e * 1.0001f);
             if (!done) break;
             rest -= b ? lane_value(upto, static_cast<int>(b) - 1) : 0;
             auto &wide = s.wide;
-            const uint32_t n_all = uniform(wide.half.count[b]);
+            const uint32_t n_all = uniform(wide.quarters.count[b]);
             const uint64_t above = b ? lane_value(upto_w, static_cast<int>(b) - 1) : 0;
-            // Each chunk's weight above the half-bit, and where its elements of it go.
+            // Each chunk's weight above the quarter, and where its elements of it go.
             for (int i = wave; i < c.chunks; i += kWideWaves) {
                 const uint64_t v = c.bins[(chunk0 + i) * 64 + lane];
                 const uint64_t sum = wave_total(static_cast<uint32_t>(lane) < b ? v & kWeightMask : 0);
@@ -1177,31 +1240,46 @@ __global__ __launch_bounds__(64 * kWideWaves) void sample_wide_kernel(sample_arg
                 }
             }
             __syncthreads();
-            const float z_hi = -0.5f * static_cast<float>(b), z_lo = z_hi - 0.5f;   // z of the half-bit: z_lo < z <= z_hi
             for (int i = wave; i < c.chunks; i += kWideWaves) {
                 uint32_t at = uniform(wide.offset[i]);
                 const uint32_t end = i + 1 < c.chunks ? uniform(wide.offset[i + 1]) : n_all;
-                for (int v0 = 0; v0 < 8 && at < end; v0 += 2) {
-                    float l[2][8];
+                raw8<T> ahead[4];
+                const auto load4 = [&](int v0) {
 #pragma unroll
-                    for (int v = 0; v < 2; ++v)
-                        load_logits<T>(logits, i * kChunk + (v0 + v) * 512 + lane * 8, a.V, l[v]);
+                    for (int v = 0; v < 4; ++v) ahead[v].load(logits, i * kChunk + (v0 + v) * 512 + lane * 8, a.V);
+                };
+                load4(0);
+                for (int v0 = 0; v0 < kChunk / 512 && at < end; v0 += 4) {
+                    uint32_t in = 0;   // 8 bits a vector from the highest down
 #pragma unroll
-                    for (int v = 0; v < 2; ++v) {
-                        uint32_t in = 0;
+                    for (int v = 0; v < 4; ++v) {
+                        float l[8];
+                        ahead[v].get(l);
 #pragma unroll
                         for (int e = 0; e < 8; ++e) {
-                            if (infinite) l[v][e] = finite_of(l[v][e]);
-                            const float z = z_of(l[v][e], top, p.per);
-                            in |= ((z <= z_hi) & (z > z_lo)) ? 1u << e : 0u;
+                            const float z = z_of(infinite ? finite_of(l[e]) : l[e], top, p.per);
+                            in = in + in + (step_of(z) == 63 - b ? 1u : 0u);
                         }
-                        const uint32_t through = wave_scan(static_cast<uint32_t>(__popc(in)));
-                        uint32_t to = at + through - static_cast<uint32_t>(__popc(in));
-                        at += lane_value(through, 63);
-                        const uint32_t index = static_cast<uint32_t>(i * kChunk + (v0 + v) * 512 + lane * 8);
-#pragma unroll
-                        for (int e = 0; e < 8; ++e)
-                            if (in >> e & 1) wide.slot[to++] = make_uint2(__float_as_uint(l[v][e]), index + e);
+                    }
+                    if (v0 + 4 < kChunk / 512) load4(v0 + 4);
+                    const uint32_t own01 = static_cast<uint32_t>(__popc(in >> 24) | __popc(in >> 16 & 255u) << 16);
+                    const uint32_t own23 = static_cast<uint32_t>(__popc(in >> 8 & 255u) | __popc(in & 255u) << 16);
+                    const uint32_t to01 = wave_scan(own01), to23 = wave_scan(own23);
+                    const uint32_t all01 = lane_value(to01, 63), all23 = lane_value(to23, 63);
+                    const uint32_t n0 = all01 & 0xFFFFu, n1 = n0 + (all01 >> 16), n2 = n1 + (all23 & 0xFFFFu);
+                    const uint32_t to[4] = {at + ((to01 - own01) & 0xFFFFu), at + n0 + ((to01 - own01) >> 16),
+                                            at + n1 + ((to23 - own23) & 0xFFFFu), at + n2 + ((to23 - own23) >> 16)};
+                    at += n2 + (all23 >> 16);
+                    const uint32_t index = static_cast<uint32_t>(i * kChunk + v0 * 512 + lane * 8);
+                    uint32_t left = in;
+                    while (__ballot(left != 0)) {
+                        if (left) {
+                            const uint32_t bit = 31u - static_cast<uint32_t>(__builtin_clz(left)), v = 3 - bit / 8;
+                            const uint32_t before = static_cast<uint32_t>(__popc(in >> bit & (255u >> bit % 8))) - 1;
+                            wide.slot[(v == 0 ? to[0] : v == 1 ? to[1] : v == 2 ? to[2] : to[3]) + before] =
+                                index + v * 512 + 7 - bit % 8;
+                            left ^= 1u << bit;
+                        }
                     }
                 }
             }
@@ -1211,10 +1289,13 @@ __global__ __launch_bounds__(64 * kWideWaves) void sample_wide_kernel(sample_arg
 #pragma unroll
             for (int e = 0; e < 16; ++e) {
                 const uint32_t at = part.place(e);
-                const uint2 v = at < n_all ? wide.slot[at] : make_uint2(0xFF800000u, 0);   // -infinity
-                // the bins over this half-bit's part of z
-                part.set(e, __uint_as_float(v.x), top, p.per, 0.5f * static_cast<float>(b), 64.0f * part.kBinsPerBit);
-                part.given[e] = v.y;
+                const uint32_t given = wide.slot[min(at, n_all - 1)];
+                float l = T::load(logits[given]);
+                if (infinite) l = finite_of(l);
+                l = at < n_all ? l : -INFINITY;
+                // the bins over this quarter's part of z: -b/4 <= z < (1 - b)/4
+                part.set(e, l, top, p.per, 0.25f * (static_cast<float>(b) - 1.0f), 128.0f * part.kBinsPerBit);
+                part.given[e] = given;
             }
             part.K = K;
             part.I = I;
@@ -1253,7 +1334,7 @@ __global__ __launch_bounds__(64 * kWideWaves) void sample_wide_kernel(sample_arg
     }
 
     __syncthreads();
-    draw_in_chunk<T, kWideWaves, 8>(a, c, row, p, s.sums, weight, top, infinite, K, I, s.list);
+    draw_in_chunk<T, kWideWaves, 16>(a, c, row, p, s.sums, weight, top, infinite, K, I, s.list);
 }
 
 template <typename T>
@@ -1263,7 +1344,7 @@ aq_status launch_long(aq_ctx *ctx, const sample_args &a) {
     c.cap = kSlots / c.chunks / 8 * 8;
     const size_t rows = static_cast<size_t>(a.rows < kRowsAtOnce ? a.rows : kRowsAtOnce), n = rows * c.chunks;
     char *at = nullptr;
-    aq_status st = aq_ctx_scratch(ctx, 7, n * (64 * 8 + 8 + c.cap * 8 + 12) + rows * 4, reinterpret_cast<void **>(&at));
+    aq_status st = aq_ctx_scratch(ctx, 7, n * (64 * 8 + 8 + c.cap * 8 + 12) + rows * (4 + sizeof(row_params)), reinterpret_cast<void **>(&at));
     if (st != AQ_OK) return st;
     c.bins = reinterpret_cast<uint64_t *>(at);
     c.weight = c.bins + n * 64;
@@ -1272,6 +1353,7 @@ aq_status launch_long(aq_ctx *ctx, const sample_args &a) {
     c.count = c.top + n;
     c.whole = reinterpret_cast<int32_t *>(c.count + n);
     c.left = c.count + 2 * n;
+    c.params = reinterpret_cast<row_params *>(c.left + rows);
     for (int64_t row0 = 0; row0 < a.rows; row0 += kRowsAtOnce) {
         const uint32_t now = static_cast<uint32_t>(a.rows - row0 < kRowsAtOnce ? a.rows - row0 : kRowsAtOnce);
         const dim3 grid(static_cast<uint32_t>(c.chunks), now);
