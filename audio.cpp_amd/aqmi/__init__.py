@@ -123,17 +123,23 @@ def _dptr(t) -> int | None:
     return t.data_ptr()
 
 
+_DTYPES: dict = {}   # torch.dtype -> aq_dtype
+
+
+def _torch_dtypes() -> dict:
+    import torch
+
+    _DTYPES.update({torch.float32: T_F32, torch.float16: T_F16, torch.bfloat16: T_BF16, torch.int8: T_I8,
+                    torch.float8_e4m3fn: T_E4M3})
+    return _DTYPES
+
+
 def _dtype(t) -> int:
     """aq_dtype of a torch tensor."""
-    name = str(t.dtype)
-    try:
-        return _DTYPES[name]
-    except KeyError:
-        raise TypeError(f"{name} is no element type of the library") from None
-
-
-_DTYPES = {"torch.float32": T_F32, "torch.float16": T_F16, "torch.bfloat16": T_BF16, "torch.int8": T_I8,
-           "torch.float8_e4m3fn": T_E4M3}
+    code = (_DTYPES or _torch_dtypes()).get(t.dtype)
+    if code is None:
+        raise TypeError(f"{t.dtype} is no element type of the library")
+    return code
 
 
 def _rows(t, rows: int, cols: int, dtype: int | None = None):
@@ -144,7 +150,7 @@ def _rows(t, rows: int, cols: int, dtype: int | None = None):
     if not t.is_cuda or t.shape != (rows, cols) or (strides[1] != 1 and cols > 1):
         raise ValueError(f"expected a device matrix [{rows}, {cols}] with adjacent row elements, got "
                          f"{tuple(t.shape)} strides {strides}")
-    if dtype is not None and _DTYPES.get(str(t.dtype)) != dtype:
+    if dtype is not None and _dtype(t) != dtype:
         raise TypeError(f"expected element type {dtype}, got {t.dtype}")
     return t.data_ptr(), strides[0] if rows > 1 else cols
 
@@ -623,10 +629,9 @@ def sample(ctx: Context, logits, u, token, temperature=None, top_k=None, top_p=N
     temperature, top_p, min_p, logp float32 and top_k, token int32, all of
     `rows` elements (token may be [B, Q] with B * Q rows)."""
     rows, V = logits.shape
-    for t, want in ((u, "torch.float32"), (token, "torch.int32"), (temperature, "torch.float32"),
-                    (top_k, "torch.int32"), (top_p, "torch.float32"), (min_p, "torch.float32"),
-                    (logp, "torch.float32")):
-        if t is not None and (t.numel() != rows or str(t.dtype) != want):
+    f32, i32 = ctx.torch.float32, ctx.torch.int32
+    for t, want in ((u, f32), (token, i32), (temperature, f32), (top_k, i32), (top_p, f32), (min_p, f32), (logp, f32)):
+        if t is not None and (t.dtype is not want or t.numel() != rows):
             raise ValueError(f"expected {rows} elements of {want}, got {tuple(t.shape)} of {t.dtype}")
     ctx.use_current_stream()
     ctx.check(ctx.lib.aq_sample(ctx.h, _dtype(logits), *_rows(logits, rows, V), rows, V, _dptr(u), _dptr(temperature),

@@ -59,6 +59,8 @@ template <> struct words<4> {
         typedef u32x4 any __attribute__((aligned(1)));
         v = *static_cast<const any *>(p);
     }
+    // Read once: an aligned load that is the first to leave the caches.
+    __device__ inline void stream(const void *p) { v = __builtin_nontemporal_load(static_cast<const u32x4 *>(p)); }
     __device__ inline uint32_t operator[](int i) const { return v[i]; }
     __device__ inline void set(int i, uint32_t w) { v[i] = w; }
 };
@@ -237,7 +239,14 @@ __global__ __launch_bounds__(PACKED || RT > 1 ? 256 : 512) void q4_product_kerne
 
     const auto load_codes = [&](int kb, words<4> (&w)[RT]) {
 #pragma unroll
-        for (int r = 0; r < RT; ++r) w[r].load(a.codes + ((tile[r] + kb) * 64 + lane) * 16);
+        for (int r = 0; r < RT; ++r) {
+            const uint8_t *from = a.codes + ((tile[r] + kb) * 64 + lane) * 16;
+            // A long matrix passes the caches once (26.2 us for 8192 x 28672,
+            // 27.5 with plain loads); a small one, or one that several rows of
+            // blocks read, is better left in them.
+            if constexpr (!PACKED && RT > 1) w[r].stream(from);
+            else w[r].load(from);
+        }
     };
     const auto load_x = [&](int kb, int part, x_t &x) {
 #pragma unroll

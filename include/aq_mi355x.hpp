@@ -270,6 +270,48 @@ private:
     aq_moss_quantizer *q_ = nullptr;
 };
 
+// A matrix with 4-bit weights and group scales (aq_q4_*).
+class Q4Linear {
+public:
+    // codes [out][ceil(in / 2)], scale (F16 bits) and zero [out][ceil(in / group)];
+    // zero and bias may be null.
+    Q4Linear(Context &ctx, int64_t out_features, int64_t in_features, int64_t group, const uint8_t *codes,
+             const uint16_t *scale, const uint8_t *zero = nullptr, const float *bias = nullptr)
+        : ctx_(&ctx) {
+        ctx.check(aq_q4_upload(ctx.get(), out_features, in_features, group, codes, scale, zero, bias, &w_));
+    }
+    Q4Linear(const Q4Linear &) = delete;
+    Q4Linear &operator=(const Q4Linear &) = delete;
+    Q4Linear(Q4Linear &&o) noexcept : ctx_(o.ctx_), w_(std::exchange(o.w_, nullptr)) {}
+    ~Q4Linear() {
+        if (w_) aq_q4_release(w_);
+    }
+
+    // Device pointers: y [M, out] = x [M, in] W^T + bias.
+    void forward(aq_dtype x_type, const void *x, int64_t x_ld, int64_t M, aq_dtype y_type, void *y, int64_t y_ld,
+                 const float *x_scale = nullptr, int64_t x_group = 0) const {
+        ctx_->check(aq_q4_forward(ctx_->get(), w_, x_type, x, x_ld, x_scale, x_group, M, y_type, y, y_ld));
+    }
+
+private:
+    Context *ctx_;
+    aq_q4 *w_ = nullptr;
+};
+
+// What aq_sample draws with, per row (device pointers; null: off).
+struct SampleFilters {
+    const float *temperature = nullptr;
+    const int32_t *top_k = nullptr;
+    const float *top_p = nullptr;
+    const float *min_p = nullptr;
+};
+
+// One index per row of device logits [rows, V], from the random numbers u [rows].
+inline void sample(Context &ctx, aq_dtype type, const void *logits, int64_t ld, int64_t rows, int64_t V, const float *u,
+                   const SampleFilters &f, int32_t *token, float *logp = nullptr) {
+    ctx.check(aq_sample(ctx.get(), type, logits, ld, rows, V, u, f.temperature, f.top_k, f.top_p, f.min_p, token, logp));
+}
+
 namespace engine::runtime {
 
 // engine::runtime::VectorQuantizer on the MI355X: the nearest codeword of
