@@ -291,11 +291,20 @@ void launch(aq_ctx *ctx, const norm_args &a) {
         const uint32_t grid = static_cast<uint32_t>(waves == 1 ? (a.M + 3) / 4 : a.M);
         aq_launch_timed(ctx, true, kernel, dim3(grid), dim3(waves == 1 ? 256 : 64 * waves), 0u, a);
     };
+    // A wave a row needs no barrier, and two vectors a thread cost less than
+    // twice the waves, once there are rows for all of the card: 4096 bf16 rows
+    // of 1024 take 10.4 us with <1, 2>, 11.4 with <4, 1>, of 4096 26.6 with
+    // <4, 2>, 27.8 with <8, 1>, of 8192 55.6 with <8, 2>, 61.4 with <16, 1>.
+    // Before that a row's own time counts: one takes 4.2 and 3.2, 4.7 and
+    // 3.7, 5.0 and 4.4 us; the two meet at about 512 to 1024 rows.
+    const bool few = a.M <= 512;
     if (nv <= 64) go(add_rmsnorm_kernel<T, 1, 1>, 1);
-    else if (nv <= 128) go(add_rmsnorm_kernel<T, 1, 2>, 1);
+    else if (nv <= 128 && !few) go(add_rmsnorm_kernel<T, 1, 2>, 1);
     else if (nv <= 256) go(add_rmsnorm_kernel<T, 4, 1>, 4);
-    else if (nv <= 512) go(add_rmsnorm_kernel<T, 4, 2>, 4);
-    else if (nv <= 1024) go(add_rmsnorm_kernel<T, 4, 4>, 4);
+    else if (nv <= 512 && !few) go(add_rmsnorm_kernel<T, 4, 2>, 4);
+    else if (nv <= 512) go(add_rmsnorm_kernel<T, 8, 1>, 8);
+    else if (nv <= 1024 && !few) go(add_rmsnorm_kernel<T, 8, 2>, 8);
+    else if (nv <= 1024) go(add_rmsnorm_kernel<T, 16, 1>, 16);
     else if (nv <= 2048) go(add_rmsnorm_kernel<T, 16, 2>, 16);
     else if (nv <= 4096) go(add_rmsnorm_kernel<T, 16, 4>, 16);
     else go(add_rmsnorm_long_kernel<T>, 16);

@@ -207,9 +207,11 @@ struct scales {
     float x[MT], x1[MT];   // a packed x's scale, and its sum over the group
 };
 
-// PACKED: x and its sums are what q4_pack_kernel wrote.
-template <typename X, bool PACKED, bool AHEAD, int SUBS, int RT, int MT, int J>
-__global__ __launch_bounds__(PACKED || RT > 1 ? 256 : 512) void q4_product_kernel(args a) {
+// PACKED: x and its sums are what q4_pack_kernel wrote.  STREAM: the codes pass
+// the caches once (8192 x 28672: 26.2 us, 27.5 with plain loads); a small
+// matrix, or one that several rows of blocks read, is better left in them.
+template <typename X, bool PACKED, bool AHEAD, bool STREAM, int SUBS, int RT, int MT, int J>
+__global__ __launch_bounds__(PACKED || RT > 2 ? 256 : 512) void q4_product_kernel(args a) {
     using x_t = x_step<X, PACKED, MT, J>;
     extern __shared__ float red[];   // [waves][RT * MT][64][4]
     using frag = typename X::frag;
@@ -241,10 +243,7 @@ __global__ __launch_bounds__(PACKED || RT > 1 ? 256 : 512) void q4_product_kerne
 #pragma unroll
         for (int r = 0; r < RT; ++r) {
             const uint8_t *from = a.codes + ((tile[r] + kb) * 64 + lane) * 16;
-            // A long matrix passes the caches once (26.2 us for 8192 x 28672,
-            // 27.5 with plain loads); a small one, or one that several rows of
-            // blocks read, is better left in them.
-            if constexpr (!PACKED && RT > 1) w[r].stream(from);
+            if constexpr (STREAM) w[r].stream(from);
             else w[r].load(from);
         }
     };
@@ -487,11 +486,11 @@ __global__ __launch_bounds__(256) void q4_pack_kernel(args a, void *to, float *s
     }
 }
 
-template <typename X, bool PACKED, bool AHEAD, int SUBS, int RT, int MT, int J>
+template <typename X, bool PACKED, bool AHEAD, bool STREAM, int SUBS, int RT, int MT, int J>
 aq_status launch_shape(aq_ctx *ctx, const args &a, int waves) {
     if (waves > a.kblocks) waves = a.kblocks;
     const uint32_t lds = static_cast<uint32_t>(waves * RT * MT * 1024);
-    auto kernel = q4_product_kernel<X, PACKED, AHEAD, SUBS, RT, MT, J>;
+    auto kernel = q4_product_kernel<X, PACKED, AHEAD, STREAM, SUBS, RT, MT, J>;
     aq_status st = aq_launch_lds(ctx, reinterpret_cast<const void *>(kernel), lds, "aq_q4_forward");
     if (st != AQ_OK) return st;
     const dim3 grid(static_cast<uint32_t>((a.tiles + RT - 1) / RT), static_cast<uint32_t>((a.M + 16 * MT - 1) / (16 * MT)));
@@ -502,16 +501,29 @@ aq_status launch_shape(aq_ctx *ctx, const args &a, int waves) {
 
 template <typename X, int SUBS>
 aq_status launch_subs(aq_ctx *ctx, const args &a) {
-    // Up to 16 rows of x: bound by the codes' way from memory.  A long matrix
-    // takes several tiles a wave (x is loaded once for them) with loads ahead:
-    // 8192 x 28672, one int8 row: 27.8 us with four, 35.8 with one.  Where
-    // that leaves compute units idle, one tile; where a wave has no second
-    // k-block, no loads ahead: 1000 x 4099, five fp32 rows: 6.0 us, 8.2 with.
-    constexpr int kTiles = SUBS == 4 ? 2 : 4;   // as many as the registers hold with each group's scales
+    // Up to 16 rows of x.  Bound by the codes' way from memory, and where a
+    // wave has few of them by latency: all in one, 8192 x 28672 takes an int8
+    // row at 4.6 TB/s.  Several tiles a block load x once for all of them, but
+    // leave fewer blocks.  In us, for 1 and 16 rows at K = 4096, group 128:
+    //                        int8          bf16
+    //    512 tiles, one     7.5  13.4     7.5  12.0
+    //               two     7.5   9.6     8.3   9.5
+    //   1024 tiles, two    10.7  15.4    11.3  14.5
+    //               four   11.4  12.4    14.4  14.7
+    // and at K = 8192, 1792 tiles: two 30.3 and 47.2, 33.3 and 43.0, four 28.4
+    // and 31.8, 36.3 and 34.5.  With 32 columns a scale four tiles' scales do
+    // not fit the registers; there one row (bf16, 1792 tiles) takes 49 us with
+    // one tile, 67 with two, 16 rows 74 and 70.
     if (a.M <= 16) {
-        if (a.kblocks <= 8) return launch_shape<X, false, false, SUBS, 1, 1, 4>(ctx, a, 8);
-        if (a.tiles < 256 * kTiles) return launch_shape<X, false, true, SUBS, 1, 1, 4>(ctx, a, 8);
-        return launch_shape<X, false, true, SUBS, kTiles, 1, 4>(ctx, a, 4);
+        const bool few = a.M <= 4;
+        // A wave has one k-block: no loads ahead, less code to fetch (1000 x
+        // 4099, five fp32 rows: 6.0 us, 8.2 with them).
+        if (a.kblocks <= 8) return launch_shape<X, false, false, false, SUBS, 1, 1, 4>(ctx, a, 8);
+        if (a.tiles < 512) return launch_shape<X, false, true, false, SUBS, 1, 1, 4>(ctx, a, 8);
+        if (a.tiles < (few ? 1536 : 1024)) return launch_shape<X, false, true, true, SUBS, 2, 1, 4>(ctx, a, 8);
+        if constexpr (SUBS < 4) return launch_shape<X, false, true, true, SUBS, 4, 1, 4>(ctx, a, 4);
+        else if (few) return launch_shape<X, false, true, true, SUBS, 1, 1, 4>(ctx, a, 4);
+        else return launch_shape<X, false, true, true, SUBS, 2, 1, 4>(ctx, a, 4);
     }
     // Packed batches of rows, at most 64 MB of them (but 64 rows).
     const int64_t row_bytes = static_cast<int64_t>(a.kblocks) * 16 * sizeof(typename X::frag) * X::kParts;
@@ -534,10 +546,13 @@ aq_status launch_subs(aq_ctx *ctx, const args &a) {
         aq_launch_timed(ctx, false, q4_pack_kernel<X>, grid, dim3(256), 0u, b, static_cast<void *>(packed), sums, SUBS);
         b.x = packed;
         b.x_sum = sums;
-        // 64 rows of x at once where the registers hold their sums, else 32.
+        // 64 rows of x at once where the registers hold their sums and that
+        // leaves two blocks a compute unit, else 32: 64 rows, K = 4096, bf16:
+        // 14.2 and 10.7 us for 4096 columns, 19.5 and 20.2 for 16384.
         constexpr bool kWide = SUBS != 4 && X::kParts == 1;
-        if (kWide && b.M > 32) st = launch_shape<X, true, true, SUBS, 2, kWide ? 4 : 2, 1>(ctx, b, 4);
-        else st = launch_shape<X, true, true, SUBS, 2, 2, X::kParts == 1 ? 2 : 1>(ctx, b, 4);
+        const int64_t blocks = static_cast<int64_t>((a.tiles + 1) / 2) * ((b.M + 63) / 64);
+        if (kWide && blocks >= 512 && b.M > 32) st = launch_shape<X, true, true, false, SUBS, 2, kWide ? 4 : 2, 1>(ctx, b, 4);
+        else st = launch_shape<X, true, true, false, SUBS, 2, 2, X::kParts == 1 ? 2 : 1>(ctx, b, 4);
         if (st != AQ_OK) return st;
     }
     return AQ_OK;

@@ -1375,7 +1375,7 @@ aq_status launch(aq_ctx *ctx, const sample_args &a) {
     if (a.V <= 512) in_registers(sample_short_kernel<T, 1, 8>, 1);
     else if (a.V <= 1024) in_registers(sample_short_kernel<T, 2, 8>, 2);
     else if (a.V <= 2048) in_registers(sample_short_kernel<T, 4, 8>, 4);
-    else if (a.V <= 4096) in_registers(sample_short_kernel<T, 4, 16>, 4);
+    else if (a.V <= 4096) in_registers(sample_short_kernel<T, 8, 8>, 8);
     else if (a.V <= 8192) in_registers(sample_short_kernel<T, 8, 16>, 8);
     else return launch_long<T>(ctx, a);
     return AQ_OK;

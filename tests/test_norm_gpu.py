@@ -77,6 +77,15 @@ def test_against_64_bits(ctx, t, kind, group, M, D):
 
 
 @pytest.mark.parametrize("t", TYPES)
+@pytest.mark.parametrize("D", [1000, 3000, 8000])
+def test_batches_of_rows(ctx, t, D):
+    """More rows than the few that get a wider block each."""
+    x, r, w = make(515, D, t, D)
+    check(ctx, x, r, w, t, "i8", 32)
+    check(ctx, x, None, w, t, "e4m3", 0)
+
+
+@pytest.mark.parametrize("t", TYPES)
 @pytest.mark.parametrize("D,ld", [(100, 103), (1024, 1025), (2050, 2064), (40000, 40003)])
 def test_strided_rows_in_place(ctx, t, D, ld):
     """x read at odd offsets; h written over x, y over the residual."""

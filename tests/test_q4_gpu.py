@@ -103,6 +103,19 @@ def test_types_and_strides(ctx, t, out):
     check(ctx, 64, 384, 128, 20, t, out)
 
 
+@pytest.mark.parametrize("t", TYPES)
+@pytest.mark.parametrize("G", [32, 64, 128])
+@pytest.mark.parametrize("N,M", [(8203, 1), (8203, 6), (16397, 5), (24601, 2)])
+def test_long_matrices(ctx, t, G, N, M):
+    """Sizes where a block takes one, two or four tiles of rows, the last one with fewer."""
+    check(ctx, N, 1100, G, M, t, zeros=True)
+
+
+@pytest.mark.parametrize("t", TYPES)
+def test_long_matrices_and_many_rows(ctx, t):
+    check(ctx, 16401, 300, 128, 70, t, bias=True)
+
+
 def test_many_rows_of_x(ctx):
     check(ctx, 48, 256, 64, 1000, "bf16", "bf16")
 
