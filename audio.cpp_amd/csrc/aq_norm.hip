@@ -10,6 +10,11 @@
 // A row of D columns is nv = ceil(D / 8) vectors of 8; vector v of a row
 // belongs to thread v % threads, so 4, 8 or 16 adjacent lanes hold a group of
 // 32, 64 or 128 columns and its maximum is a butterfly within them.
+//
+// Bound by memory: 16384 bf16 rows of 8192 with every output (1.2 GB) take
+// 219 us, 5.5 TB/s, 6000 f16 rows of 4096 without y (172 MB) 35.5 us, 4.8
+// TB/s; a copy of 2 GB runs at 4.8 TB/s on the same card.  A single row is
+// latency: 3.2 us for 1024 columns, the launch, a load, a reduction.
 #include "aq_device_math.hpp"
 #include "aq_internal.hpp"
 #include "aq_types.hpp"

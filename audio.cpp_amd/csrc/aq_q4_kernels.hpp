@@ -18,6 +18,13 @@
 // 8-bit x.  Whole numbers stay whole: the nibbles as bytes against x's bytes,
 // and zero * sum(x) taken off (all below 2^24, so exact in fp32 as well).
 // e4m3 converts to f16 exactly.
+//
+// What bounds it.  Up to 16 rows of x, the codes' way from memory: 8192 x
+// 28672, one int8 row, 121 MB in 26 us, 4.7 TB/s, where a copy of 2 GB runs
+// at 4.8.  Small matrices, latency: 1024 x 12288, one bf16 row, 5.6 us.  Many
+// rows, the waits of few waves with many registers: 64 rows of f16 by 4096 x
+// 16384 18.7 us with 3 us of packing, 37.7 MB and 8.6 GFLOP, of which the
+// matrix instructions take 37 % of the time and the codes' conversion as much.
 #pragma once
 #include "aq_internal.hpp"
 #include "aq_q4.hpp"
@@ -442,7 +449,8 @@ __global__ __launch_bounds__(PACKED || RT > 2 ? 256 : 512) void q4_product_kerne
 // zeros past M and K: [16 rows][k-block][4 steps][parts][64 lanes].  A lane of
 // the product reads 16 (or 8) bytes next to its neighbour's, where a row of x
 // gives it 16 bytes of each of 16 rows: for many rows that, not the
-// arithmetic, was what the product waited for.
+// arithmetic, was what the product waited for (64 rows, 4096 x 16384: 39 us,
+// and 19 with the packing).
 // With them the sums of x over each of a k-block's `subs` parts, [16 rows]
 // [k-block][subs][16], as the products' groups need them.
 template <typename X>

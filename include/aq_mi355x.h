@@ -17,6 +17,9 @@
  * differ from this library's (tests/test_oracle.py
  * test_reference_cpu_view_bug_is_real shows it on ggml itself).
  *
+ * The operators at the end ("Answering with codes") have no reference: they
+ * compute what their own comments say.
+ *
  * Conventions
  *  - Plain C types only.  Every entry point returns aq_status; a message for
  *    the last failure on a context is available from aq_last_error().
@@ -514,7 +517,8 @@ typedef enum aq_dtype { AQ_T_F32 = 0, AQ_T_F16 = 1, AQ_T_BF16 = 2, AQ_T_I8 = 3, 
  *             sum is the same buffer.
  *   q_type    I8 or E4M3; q device [M, D] contiguous, or NULL: no 8-bit output
  *   scale     device [M, ceil(D / group)] (group 0: [M]); with q
- * Any D from 1 to 2^30.  Sums are held in fp32. */
+ * Any D from 1 to 2^30.  Sums are held in fp32; their order depends on the
+ * type, M and D alone. */
 aq_status aq_add_rmsnorm(aq_ctx *ctx, int type, const void *x, int64_t x_ld, const void *residual,
                          int64_t residual_ld, const void *weight, int64_t M, int64_t D, float eps, void *sum,
                          int64_t sum_ld, void *y, int64_t y_ld, int q_type, int64_t group, void *q, float *scale);
@@ -546,7 +550,8 @@ aq_status aq_q4_upload(aq_ctx *ctx, int64_t out_features, int64_t in_features, i
  * Products and sums are fp32, exact whole numbers for I8; an F32 x enters
  * with all its 24 bits.  A row of x with a value that is not finite (or above
  * 2^112, where a group's sum may not be) gives a row of NaN.  The order of a
- * sum depends on M and the matrix alone. */
+ * sum depends on the types, M and the matrix alone.  For M above 16 x is laid
+ * out in the context's scratch first. */
 aq_status aq_q4_forward(aq_ctx *ctx, const aq_q4 *w, int x_type, const void *x, int64_t x_ld, const float *x_scale,
                         int64_t x_group, int64_t M, int y_type, void *y, int64_t y_ld);
 aq_status aq_q4_release(aq_q4 *w);
@@ -574,7 +579,8 @@ aq_status aq_q4_release(aq_q4 *w);
  *   min_p        device [rows] or NULL; <= 0 or NaN: off; above 1 counts as 1
  *   token        device [rows] int32; [B, Q] codes are rows = B * Q
  *   logp         device [rows] or NULL
- * V from 1 to 2^20, rows up to 2^21. */
+ * V from 1 to 2^20, rows up to 2^21.  Rows longer than 8192 use the context's
+ * scratch. */
 aq_status aq_sample(aq_ctx *ctx, int type, const void *logits, int64_t ld, int64_t rows, int64_t V, const float *u,
                     const float *temperature, const int32_t *top_k, const float *top_p, const float *min_p,
                     int32_t *token, float *logp);
