@@ -25,6 +25,13 @@ struct aq_ctx {
     // exact scan takes, 7: largest logits and candidates of sampled rows,
     // 8: rows of x in operand order).
     static constexpr int kScratchSlots = 9;
+    // Slots from here on (tens of MB at most, but for rows of millions of
+    // columns) at least double when they grow, and leave the buffers that they
+    // outgrow allocated until the context ends: a captured graph of a call
+    // goes on using its own.
+    static constexpr int kFirstKept = 7;
+    void *outgrown[(kScratchSlots - kFirstKept) * 64] = {};   // a size doubles fewer than 64 times
+    int outgrown_count = 0;
     // Per-stage counters of the last Euclidean encode on this context (in
     // slot 1, or in the no-allocation scratch).
     int32_t *euclid_counts = nullptr;
@@ -54,7 +61,8 @@ inline void aq_launch_timed(aq_ctx *ctx, bool may_time, F kernel, dim3 grid, dim
 }
 
 // Device buffer `slot` of at least `bytes` (grows it, waiting for the stream
-// first; bytes == 0 returns the current buffer, possibly null).
+// first if the old one is freed; bytes == 0 returns the current buffer,
+// possibly null).
 aq_status aq_ctx_scratch(aq_ctx *ctx, int slot, size_t bytes, void **out);
 
 // LDS of a gfx950 compute unit: a block's static and dynamic LDS together

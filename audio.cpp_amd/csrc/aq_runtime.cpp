@@ -20,6 +20,16 @@ aq_status aq_ctx_scratch(aq_ctx *ctx, int slot, size_t bytes, void **out) {
     if (!ctx || !out || slot < 0 || slot >= aq_ctx::kScratchSlots) return AQ_E_INVALID_ARG;
     if (bytes > ctx->scratch_bytes[slot]) {
         aq_device_guard g(ctx->device);
+        if (slot >= aq_ctx::kFirstKept) {
+            void *grown = nullptr;
+            if (bytes < 2 * ctx->scratch_bytes[slot]) bytes = 2 * ctx->scratch_bytes[slot];
+            if (hipMalloc(&grown, bytes) != hipSuccess)
+                return aq_fail(ctx, AQ_E_NOMEM, "work buffer of %zu bytes could not be allocated", bytes);
+            if (ctx->scratch[slot]) ctx->outgrown[ctx->outgrown_count++] = ctx->scratch[slot];
+            ctx->scratch_bytes[slot] = bytes;
+            *out = ctx->scratch[slot] = grown;
+            return AQ_OK;
+        }
         AQ_HIP(ctx, hipStreamSynchronize(ctx->stream));
         if (ctx->scratch[slot]) (void)hipFree(ctx->scratch[slot]);
         ctx->scratch[slot] = nullptr;
@@ -123,6 +133,7 @@ aq_status aq_ctx_destroy(aq_ctx *ctx) {
         if (ctx->d_flags) (void)hipFree(ctx->d_flags);
         for (int i = 0; i < aq_ctx::kScratchSlots; ++i)
             if (ctx->scratch[i]) (void)hipFree(ctx->scratch[i]);
+        for (int i = 0; i < ctx->outgrown_count; ++i) (void)hipFree(ctx->outgrown[i]);
         for (hipEvent_t e : ctx->ev_start) (void)hipEventDestroy(e);
         for (hipEvent_t e : ctx->ev_stop) (void)hipEventDestroy(e);
     }

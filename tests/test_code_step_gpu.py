@@ -88,3 +88,47 @@ def test_captured_in_a_graph():
         torch.cuda.synchronize()
         for a, b in zip(got, (stream, step.codes, step.logp, step.logits, token)):
             assert torch.equal(a, b)
+
+
+def test_graph_keeps_its_scratch():
+    """A later call that needs more scratch leaves a captured one what it uses."""
+    ctx = aqmi.Context(0)
+    g = torch.Generator(device="cuda").manual_seed(5)
+    logits = 3 * torch.randn((3, 9000), generator=g, device="cuda")
+    u, top_p = torch.rand(3, generator=g, device="cuda"), torch.full((3,), 0.95, device="cuda")
+    token = torch.empty(3, dtype=torch.int32, device="cuda")
+    r = np.random.default_rng(5)
+    linears = [aqmi.Q4Linear(ctx, r.integers(0, 256, (n, k // 2), dtype=np.uint8),
+                             r.uniform(0.01, 0.02, (n, k // 64)).astype(np.float16), k, 64) for n, k in ((96, 256), (64, 2048))]
+    x, y = torch.randn((20, 256), generator=g, device="cuda").half(), torch.empty((20, 96), device="cuda")
+
+    def work():
+        linears[0].forward(x, y)
+        aqmi.sample(ctx, logits, u, token, top_p=top_p)
+
+    def larger():
+        aqmi.sample(ctx, 3 * torch.randn((40, 50000), generator=g, device="cuda"), torch.rand(40, device="cuda"),
+                    torch.empty(40, dtype=torch.int32, device="cuda"), top_p=torch.full((40,), 0.9, device="cuda"))
+        linears[1].forward(torch.randn((200, 2048), generator=g, device="cuda").half(),
+                           torch.empty((200, 64), device="cuda"))
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        work()
+    torch.cuda.synchronize()
+    want = token.clone(), y.clone()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=side):
+        work()
+    for _ in range(3):
+        larger()
+        torch.cuda.synchronize()
+        fill = [torch.full((1 << 20,), -1, dtype=torch.int32, device="cuda") for _ in range(8)]
+        torch.cuda.synchronize()
+        token.fill_(-7)
+        y.fill_(-7)
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(token, want[0]) and torch.equal(y, want[1])
+        assert all(bool((f == -1).all()) for f in fill)
