@@ -653,9 +653,8 @@ __global__ __launch_bounds__(64 * WAVES) void sample_short_kernel(sample_args a)
 //  1. the largest logit of each chunk, and the row's parameters;
 //  2. the weights, relative to the row's largest, and their sum over the
 //     chunk; for rows with filters also the chunk's count and weight per
-//     quarter of a bit of weight (63 of them, and of all that is below), and
-//     its candidates: the elements of its largest quarters, in index order, as
-//     many whole ones as fit its slots;
+//     quarter of a bit of weight, and its candidates: the elements of its
+//     largest quarters, in index order, as many whole ones as fit its slots;
 //  3. a small block per row.  Without filters it finds the chunk that the draw
 //     falls into from the sums, and draws in it.  With filters it works on the
 //     candidates down to the least quarter that every chunk has given whole,
@@ -665,7 +664,13 @@ __global__ __launch_bounds__(64 * WAVES) void sample_short_kernel(sample_args a)
 //     top-p's): its elements are collected from the chunks and decide where,
 //     and the sums over what lies above it decide the chunk to draw in.  What
 //     is left even then (min-p's end in a wide set, more than 8192 elements in
-//     a quarter, an end below them all) streams the row.
+//     a quarter) streams the row.
+//
+// 256 rows of 160000 bf16 logits under top-p take 14, 31, 12 and 47 us (82 MB,
+// 17 us at a copy's rate): the first reads at 6 TB/s; the second's time is
+// vector instructions, some 20 an element; the third's and fourth's the
+// latency of one block's steps, the fourth's with the row read again.  One row
+// of 131071: 2.5, 6, 9 and 1.
 constexpr int kChunk = 8192;          // 256 threads, 32 elements each
 constexpr int kSlots = 2048;          // candidates of a row: 256 threads, 8 each
 constexpr int kWideWaves = 8;         // of a block in the fourth launch: with twice as many its registers spill
@@ -674,7 +679,7 @@ constexpr int kMostChunks = kMaxV / kChunk;
 constexpr int kRowsAtOnce = 256;
 
 struct chunk_store {
-    uint64_t *bins;     // [rows][chunks][64] count and weight of each quarter, as kCountShift has them
+    uint64_t *bins;     // [rows][chunks][kBinned] count and weight of each quarter, as kCountShift has them
     uint64_t *weight;   // [rows][chunks] sum of weights (of those that min-p leaves, for rows without other filters)
     uint2 *slot;        // [rows][chunks][cap] logit's bits, index
     uint32_t *top;      // [rows][chunks] largest key
@@ -685,11 +690,46 @@ struct chunk_store {
     int chunks, cap;
 };
 
-// The quarter of a bit of weight below the largest: 63 for the largest itself,
-// 62 for those above -1/4, and so on; 0: all at or below -15.5 (and a NaN).
-// One fused product and sum, and it does not fall with z.
-__device__ inline uint32_t step_of(float z) { return whole_of(__fmaf_rn(z, 4.0f, 63.0f)); }
-__device__ inline uint32_t quarter(float z) { return 63u - step_of(z); }
+// The quarter of a bit of weight below the largest, counted from below: 125 for
+// the largest itself, 124 for those above -1/4, down to 1 from -31 on; 0: no
+// weight (or a NaN).  One fused product and sum, and it does not fall with z.
+// Quarter 0 is the largest itself, 124 the last with weights.
+constexpr int kQuarters = 125, kBinned = 128;   // bins, two a lane; the last ones stay empty
+__device__ inline uint32_t step_of(float z) { return whole_of(__fmaf_rn(z, 4.0f, 125.0f)); }
+__device__ inline uint32_t quarter(float z) { return kQuarters - step_of(z); }
+
+// Elements that a wave picks from 2048 of a row, in index order: bit 31 - (8 v +
+// e) of `in` is element e of this lane's 8 in vector v, and vector v's come
+// before v + 1's.  `to`: the places of each vector's first one of this lane.
+// Returns how many the wave has.  (Sums of two vectors in a word: no carry, at
+// most 512 each.)
+__device__ inline uint32_t places_of(uint32_t in, uint32_t (&to)[4]) {
+    const uint32_t own01 = static_cast<uint32_t>(__popc(in >> 24) | __popc(in >> 16 & 255u) << 16);
+    const uint32_t own23 = static_cast<uint32_t>(__popc(in >> 8 & 255u) | __popc(in & 255u) << 16);
+    const uint32_t to01 = wave_scan(own01), to23 = wave_scan(own23);
+    const uint32_t all01 = lane_value(to01, 63), all23 = lane_value(to23, 63);
+    const uint32_t n0 = all01 & 0xFFFFu, n1 = n0 + (all01 >> 16), n2 = n1 + (all23 & 0xFFFFu);
+    to[0] = (to01 - own01) & 0xFFFFu;
+    to[1] = n0 + ((to01 - own01) >> 16);
+    to[2] = n1 + ((to23 - own23) & 0xFFFFu);
+    to[3] = n2 + ((to23 - own23) >> 16);
+    return n2 + (all23 >> 16);
+}
+
+// f(place, offset of the element from the wave's first) for each of them.
+template <typename F>
+__device__ inline void each_picked(uint32_t in, const uint32_t (&to)[4], F &&f) {
+    const uint32_t lane8 = (threadIdx.x & 63) * 8;
+    uint32_t left = in;
+    while (__ballot(left != 0)) {
+        if (left) {
+            const uint32_t bit = 31u - static_cast<uint32_t>(__builtin_clz(left)), v = 3 - bit / 8;
+            const uint32_t before = static_cast<uint32_t>(__popc(in >> bit & (255u >> bit % 8))) - 1;   // own of this vector
+            f((v == 0 ? to[0] : v == 1 ? to[1] : v == 2 ? to[2] : to[3]) + before, v * 512 + lane8 + 7 - bit % 8);
+            left ^= 1u << bit;
+        }
+    }
+}
 
 template <typename T>
 __global__ __launch_bounds__(256) void sample_top_kernel(sample_args a, chunk_store c, int64_t row0) {
@@ -720,10 +760,12 @@ __device__ inline uint32_t row_top(const chunk_store &c, int64_t r) {
 
 template <typename T>
 __global__ __launch_bounds__(256) void sample_chunk_kernel(sample_args a, chunk_store c, int64_t row0) {
-    // Copies of the bins for every wave and every fourth lane: lanes of one
-    // wave often meet in a bin.
-    constexpr int kCopies = 16;
-    __shared__ uint64_t bins[64][kCopies];
+    // Copies of the bins for every eighth lane, since lanes of one wave often
+    // meet in a bin, and a row's length that puts its neighbours into other
+    // banks.  256 rows of 160000 bf16 logits: 31 us; with 16 copies 39, for the
+    // room that they take, and 45 without the added word.
+    constexpr int kCopies = 8;
+    __shared__ uint64_t bins[kBinned][kCopies + 1];
     __shared__ uint64_t part[4];
     __shared__ uint32_t counts[4];
     __shared__ int whole;
@@ -758,10 +800,10 @@ __global__ __launch_bounds__(256) void sample_chunk_kernel(sample_args a, chunk_
         if (threadIdx.x == 0) c.weight[chunk] = part[0] + part[1] + part[2] + part[3];
         return;
     }
-    // Vector instructions are what this kernel takes its time for, so what is
-    // not for an element is for 32 of them, or left to one wave.
+    // Vector instructions are what this takes its time for, so what is not for
+    // an element is for 32 of them, or left to one wave.
 #pragma unroll
-    for (int i = 0; i < 4; ++i) bins[lane][wave * 4 + i] = 0;
+    for (int i = 0; i < kBinned * kCopies / 256; ++i) bins[lane + i % 2 * 64][wave * (kCopies / 4) + i / 2] = 0;
     __syncthreads();
     uint32_t step[32];
 #pragma unroll
@@ -769,25 +811,27 @@ __global__ __launch_bounds__(256) void sample_chunk_kernel(sample_args a, chunk_
         const float z = z_of(l[e / 8][e % 8], top, p.per);
         const uint32_t w = w_of(z);
         step[e] = step_of(z);
-        mine += w;
-        if (step[e])   // not so far below that only the sum counts
-            atomicAdd(reinterpret_cast<unsigned long long *>(&bins[step[e]][wave * 4 + (lane & 3)]),
+        if (step[e])
+            atomicAdd(reinterpret_cast<unsigned long long *>(&bins[step[e]][lane % kCopies]),
                       (uint64_t{1} << kCountShift) + w);
     }
-    mine = wave_total(mine);
-    if (lane == 0) part[wave] = mine;
     __syncthreads();
     if (wave == 0) {
-        uint64_t sum = 0;   // of quarter `lane`
+        const int q = 2 * lane;   // and q + 1
+        ulonglong2 sum = make_ulonglong2(0, 0);
+        if (q < kQuarters) {
 #pragma unroll
-        for (int i = 0; i < kCopies; ++i) sum += bins[63 - lane][(i + lane) % kCopies];
-        // What is below all quarters is what they leave of the chunk's weight;
-        // its count matters only as none, or more than any slots hold.
-        const uint64_t all = part[0] + part[1] + part[2] + part[3], above = wave_total(sum & kWeightMask);
-        if (lane == 63) sum = all > above ? (uint64_t{kChunk} << kCountShift) + (all - above) : 0;
-        c.bins[chunk * 64 + lane] = sum;
-        const uint32_t upto = wave_scan(static_cast<uint32_t>(sum >> kCountShift));
-        const int last = __popcll(__ballot(upto <= static_cast<uint32_t>(c.cap))) - 1;   // upto does not fall with the lane
+            for (int i = 0; i < kCopies; ++i) {
+                sum.x += bins[kQuarters - q][(i + lane) % kCopies];
+                sum.y += q + 1 < kQuarters ? bins[kQuarters - q - 1][(i + lane) % kCopies] : 0;
+            }
+        }
+        *reinterpret_cast<ulonglong2 *>(c.bins + chunk * kBinned + q) = sum;
+        const uint64_t all = wave_total((sum.x & kWeightMask) + (sum.y & kWeightMask));
+        const uint32_t n1 = static_cast<uint32_t>(sum.y >> kCountShift);
+        const uint32_t upto = wave_scan(static_cast<uint32_t>(sum.x >> kCountShift) + n1);   // through q + 1; it does not fall
+        const uint32_t cap = static_cast<uint32_t>(c.cap);
+        const int last = __popcll(__ballot(upto <= cap)) + __popcll(__ballot(upto - n1 <= cap)) - 1;
         if (lane == 0) {
             c.weight[chunk] = all;
             c.whole[chunk] = last;
@@ -795,35 +839,21 @@ __global__ __launch_bounds__(256) void sample_chunk_kernel(sample_args a, chunk_
         }
     }
     __syncthreads();
-    const uint32_t least = static_cast<uint32_t>(max(63 - whole, 1));   // step of the last quarter given (0 has no weight then)
+    const uint32_t least = static_cast<uint32_t>(max(kQuarters - whole, 1));   // step of the last quarter given
 
-    // This thread's candidates, 8 bits a vector from the highest down, and how
-    // many of the wave's are before those of each vector.
-    uint32_t in = 0;
+    // The candidates.
+    uint32_t in = 0, to[4];
 #pragma unroll
     for (int e = 0; e < 32; ++e) in = in + in + (step[e] >= least ? 1u : 0u);
-    const uint32_t own01 = static_cast<uint32_t>(__popc(in >> 24) | __popc(in >> 16 & 255u) << 16);
-    const uint32_t own23 = static_cast<uint32_t>(__popc(in >> 8 & 255u) | __popc(in & 255u) << 16);
-    const uint32_t to01 = wave_scan(own01), to23 = wave_scan(own23);   // no carry between the halves: at most 512 each
-    const uint32_t all01 = lane_value(to01, 63), all23 = lane_value(to23, 63);
-    const uint32_t n0 = all01 & 0xFFFFu, n1 = n0 + (all01 >> 16), n2 = n1 + (all23 & 0xFFFFu), n3 = n2 + (all23 >> 16);
-    if (lane == 0) counts[wave] = n3;
+    const uint32_t n = places_of(in, to);
+    if (lane == 0) counts[wave] = n;
     __syncthreads();
-    uint32_t first = 0;
-    for (int i = 0; i < wave; ++i) first += counts[i];
-    const uint32_t at[4] = {first + ((to01 - own01) & 0xFFFFu), first + n0 + ((to01 - own01) >> 16),
-                            first + n1 + ((to23 - own23) & 0xFFFFu), first + n2 + ((to23 - own23) >> 16)};
     uint2 *slot = c.slot + chunk * c.cap;
-    uint32_t left = in;
-    while (__ballot(left != 0)) {
-        if (left) {
-            const int bit = 31 - __builtin_clz(left), v = 3 - bit / 8, index = base + v * 512 + 7 - bit % 8;
-            const uint32_t before = static_cast<uint32_t>(__popc(in >> bit & (255u >> bit % 8))) - 1;   // own of this vector
-            const uint32_t to = (v == 0 ? at[0] : v == 1 ? at[1] : v == 2 ? at[2] : at[3]) + before;
-            slot[to] = make_uint2(bits_of(static_cast<float>(T::load(logits[index]))), static_cast<uint32_t>(index));
-            left ^= 1u << bit;
-        }
-    }
+    for (int i = 0; i < wave; ++i) slot += counts[i];
+    const uint32_t index0 = blockIdx.x * kChunk + static_cast<uint32_t>(wave) * 2048;
+    each_picked(in, to, [&](uint32_t at, uint32_t offset) {
+        slot[at] = make_uint2(bits_of(static_cast<float>(T::load(logits[index0 + offset]))), index0 + offset);
+    });
     if (threadIdx.x == 0) c.count[chunk] = counts[0] + counts[1] + counts[2] + counts[3];
 }
 
@@ -1028,34 +1058,77 @@ struct row_stream {
     }
 };
 
-// The weight and count of a row's quarters through quarter `lane`, from its
-// chunks; every wave of a block takes part.
-struct quarter_sums {
-    uint64_t weight[64];
-    uint32_t count[64];
+// The weight and count of a row's quarters through 2 * lane and the next, from
+// its chunks; every wave of a block takes part.
+struct quarter_lds {
+    uint64_t weight[kBinned];
+    uint32_t count[kBinned];
 };
-__device__ inline void sum_quarters(const chunk_store &c, int64_t chunk0, quarter_sums &s, uint64_t &upto_w, uint32_t &upto_n) {
-    const int lane = threadIdx.x & 63, wave = static_cast<int>(uniform(threadIdx.x >> 6)), waves = blockDim.x >> 6;
-    if (threadIdx.x < 64) {
-        s.weight[threadIdx.x] = 0;
-        s.count[threadIdx.x] = 0;
+struct quarter_sums {
+    uint64_t w_even, w_odd;
+    uint32_t n_even, n_odd;
+    __device__ inline __attribute__((always_inline)) quarter_sums(const chunk_store &c, int64_t chunk0, quarter_lds &s) {
+        const int lane = threadIdx.x & 63, wave = static_cast<int>(uniform(threadIdx.x >> 6)), waves = blockDim.x >> 6;
+        if (threadIdx.x < kBinned) {
+            s.weight[threadIdx.x] = 0;
+            s.count[threadIdx.x] = 0;
+        }
+        __syncthreads();
+        uint64_t w0 = 0, w1 = 0;
+        uint32_t n0 = 0, n1 = 0;
+        for (int i = wave; i < c.chunks; i += waves) {
+            const ulonglong2 v = *reinterpret_cast<const ulonglong2 *>(c.bins + (chunk0 + i) * kBinned + 2 * lane);
+            w0 += v.x & kWeightMask;
+            w1 += v.y & kWeightMask;
+            n0 += static_cast<uint32_t>(v.x >> kCountShift);
+            n1 += static_cast<uint32_t>(v.y >> kCountShift);
+        }
+        if (n0 + n1) {
+            atomicAdd(reinterpret_cast<unsigned long long *>(&s.weight[2 * lane]), w0);
+            atomicAdd(reinterpret_cast<unsigned long long *>(&s.weight[2 * lane + 1]), w1);
+            atomicAdd(&s.count[2 * lane], n0);
+            atomicAdd(&s.count[2 * lane + 1], n1);
+        }
+        __syncthreads();
+        w1 = s.weight[2 * lane + 1];
+        n1 = s.count[2 * lane + 1];
+        w_odd = wave_scan(s.weight[2 * lane] + w1);
+        n_odd = wave_scan(s.count[2 * lane] + n1);
+        w_even = w_odd - w1;
+        n_even = n_odd - n1;
     }
-    __syncthreads();
-    uint64_t w = 0;
-    uint32_t n = 0;
-    for (int i = wave; i < c.chunks; i += waves) {
-        const uint64_t v = c.bins[(chunk0 + i) * 64 + lane];
-        w += v & kWeightMask;
-        n += static_cast<uint32_t>(v >> kCountShift);
+    // Through quarter b.
+    __device__ uint64_t weight(int b) const {
+        const uint64_t even = lane_value(w_even, b >> 1), odd = lane_value(w_odd, b >> 1);
+        return b & 1 ? odd : even;
     }
-    if (n) {
-        atomicAdd(reinterpret_cast<unsigned long long *>(&s.weight[lane]), w);
-        atomicAdd(&s.count[lane], n);
+    __device__ uint32_t count(int b) const {
+        const uint32_t even = lane_value(n_even, b >> 1), odd = lane_value(n_odd, b >> 1);
+        return b & 1 ? odd : even;
     }
-    __syncthreads();
-    upto_w = wave_scan(s.weight[lane]);
-    upto_n = wave_scan(s.count[lane]);
-}
+};
+
+// Where a wide set ends by count (top-k) or by weight (top-p of `weight`):
+// the quarter, what is needed of it, and whether it can be worked on, with
+// nothing kept that min-p may drop.
+struct wide_end {
+    uint64_t rest = 0;
+    uint32_t quarter = 0, count = 0;
+    bool usable = false;
+    __device__ inline __attribute__((always_inline)) wide_end(const row_params &p, uint64_t weight, const quarter_sums &sums, const quarter_lds &s, bool by_weight) {
+        rest = by_weight ? max(share(p.p, weight), uint64_t{1}) : p.k;
+        const uint64_t over0 = by_weight ? __ballot(sums.w_even >= rest) : __ballot(sums.n_even >= rest);
+        const uint64_t over1 = by_weight ? __ballot(sums.w_odd >= rest) : __ballot(sums.n_odd >= rest);
+        if (!over1) return;
+        const int in1 = 2 * __builtin_ctzll(over1) + 1, in0 = over0 ? 2 * __builtin_ctzll(over0) : in1;
+        const int b = min(in0, in1);
+        quarter = static_cast<uint32_t>(b);
+        count = uniform(s.count[b]);
+        usable = (count <= kGathered) &
+                 !((p.min_e > 0.0f) & (e_of(-0.25f * static_cast<float>(b)) <= p.min_e * 1.0001f));
+        if (b) rest -= by_weight ? sums.weight(b - 1) : sums.count(b - 1);
+    }
+};
 
 // The draw in the chunk where the running weight over `sums` (device or LDS,
 // one per chunk) exceeds share(u, weight), among what K and I keep.
@@ -1099,7 +1172,7 @@ __device__ inline void draw_in_chunk(const sample_args &a, const chunk_store &c,
 template <typename T>
 __global__ __launch_bounds__(256) void sample_row_kernel(sample_args a, chunk_store c, int64_t row0) {
     __shared__ list_lds<4> lds;
-    __shared__ quarter_sums sums;
+    __shared__ quarter_lds quarters;
     const int lane = threadIdx.x & 63;
     const int64_t r = blockIdx.x, row = row0 + r, chunk0 = r * c.chunks;
     const row_params p = c.params[r];
@@ -1114,14 +1187,14 @@ __global__ __launch_bounds__(256) void sample_row_kernel(sample_args a, chunk_st
     const bool filtered = p.k || p.p < 1u << 24;
 
     // The row's weight, and for filtered rows the least quarter given whole.
-    int whole = 63;
+    int whole = kBinned - 1;
     uint64_t weight = 0;
     for (int i = lane; i < c.chunks; i += 64) {
         weight += c.weight[chunk0 + i];
         if (filtered) whole = min(whole, c.whole[chunk0 + i]);
     }
     weight = wave_total(weight);
-    whole = static_cast<int>(63u - wave_max(static_cast<uint32_t>(63 - whole)));
+    whole = kBinned - 1 - static_cast<int>(wave_max(static_cast<uint32_t>(kBinned - 1 - whole)));
     if (!filtered) {
         draw_in_chunk<T, 4, 32>(a, c, row, p, c.weight + chunk0, weight, top, infinite, 1, 0xFFFFFFFFu, lds);
         return;
@@ -1137,12 +1210,10 @@ __global__ __launch_bounds__(256) void sample_row_kernel(sample_args a, chunk_st
     for (int i = 0; i < 4; ++i) v[i] = slot[i];
     // Do they hold the kept set?  They do if top-k ends in them; without
     // top-k, if top-p does, or if min-p lets nothing below them through.
-    uint64_t upto_w;
-    uint32_t upto_n;
-    sum_quarters(c, chunk0, sums, upto_w, upto_n);
+    const quarter_sums sums(c, chunk0, quarters);
     const uint64_t need = p.k ? p.k : max(share(p.p, weight), uint64_t{1});
-    bool enough = whole == 63;
-    if (whole >= 0) enough |= (p.k ? lane_value(upto_n, whole) : lane_value(upto_w, whole)) >= need;
+    bool enough = whole >= kQuarters - 1;
+    if (whole >= 0) enough |= (p.k ? sums.count(whole) : sums.weight(whole)) >= need;
     enough |= !p.k && e_of(-0.25f * static_cast<float>(whole)) * 1.0001f < p.min_e;
     if (!enough) {
         if (threadIdx.x == 0) c.left[r] = 1;
@@ -1170,7 +1241,7 @@ struct wide_lds {
         struct {
             uint32_t slot[kGathered];   // indices
             uint32_t offset[kMostChunks];
-            quarter_sums quarters;
+            quarter_lds quarters;
         } wide;
     };
 };
@@ -1196,42 +1267,35 @@ __global__ __launch_bounds__(64 * kWideWaves) void sample_wide_kernel(sample_arg
         if (wave == 0) s.sums[i] = w;
     }
     weight = wave_total(weight);
-    uint64_t upto_w;
-    uint32_t upto_n;
-    sum_quarters(c, chunk0, s.wide.quarters, upto_w, upto_n);
+    const quarter_sums sums(c, chunk0, s.wide.quarters);
     uint32_t K = 1, I = 0xFFFFFFFFu;
     {
-        // A wide set.  Phase 0: top-k's end; phase 1: top-p's.  The quarter b
-        // where the sums cross holds it, `rest` of the count or weight into it.
+        // A wide set.  Phase 0: top-k's end; phase 1: top-p's.  (Where the sums
+        // cross, so there is one: both are at most the row's.)
         bool done = true;
 #pragma unroll 1
         for (int phase = 0; phase < 2; ++phase) {
             const bool by_weight = phase != 0;
-            uint64_t rest = p.k;
-            if (phase == 1) rest = p.p < 1u << 24 ? max(share(p.p, weight), uint64_t{1}) : 0;
-            if (!rest) continue;
-            if (phase == 0 && rest > lane_value(upto_n, 63)) {   // top-k leaves everything, and the sums are of everything
+            if (by_weight ? p.p >= 1u << 24 : !p.k) continue;
+            if (!by_weight && p.k > sums.count(kQuarters - 1)) {   // top-k leaves everything, and the sums are of everything
                 done = !(p.min_e > 0.0f);
                 if (!done) break;
                 continue;
             }
-            const uint64_t upto = by_weight ? upto_w : upto_n;
-            const uint32_t b = static_cast<uint32_t>(__builtin_ctzll(__ballot(upto >= rest)));
-            done = b < 63 && uniform(s.wide.quarters.count[b]) <= kGathered &&
-                   !(p.min_e > 0.0f && e_of(-0.25f * static_cast<float>(b)) <= p.min_e * 1.0001f);
+            const wide_end ends(p, weight, sums, s.wide.quarters, by_weight);
+            done = ends.usable;
             if (!done) break;
-            rest -= b ? lane_value(upto, static_cast<int>(b) - 1) : 0;
+            const uint32_t b = ends.quarter, n_all = ends.count;
+            const uint64_t rest = ends.rest;
             auto &wide = s.wide;
-            const uint32_t n_all = uniform(wide.quarters.count[b]);
-            const uint64_t above = b ? lane_value(upto_w, static_cast<int>(b) - 1) : 0;
+            const uint64_t above = b ? sums.weight(static_cast<int>(b) - 1) : 0;
             // Each chunk's weight above the quarter, and where its elements of it go.
             for (int i = wave; i < c.chunks; i += kWideWaves) {
-                const uint64_t v = c.bins[(chunk0 + i) * 64 + lane];
-                const uint64_t sum = wave_total(static_cast<uint32_t>(lane) < b ? v & kWeightMask : 0);
-                if (lane == 0) {
-                    s.sums[i] = sum;
-                    wide.offset[i] = static_cast<uint32_t>(c.bins[(chunk0 + i) * 64 + b] >> kCountShift);
-                }
+                const ulonglong2 v = *reinterpret_cast<const ulonglong2 *>(c.bins + (chunk0 + i) * kBinned + 2 * lane);
+                const uint32_t q = 2 * static_cast<uint32_t>(lane);
+                const uint64_t sum = wave_total((q < b ? v.x & kWeightMask : 0) + (q + 1 < b ? v.y & kWeightMask : 0));
+                if (lane == 0) s.sums[i] = sum;
+                if (q == (b & ~1u)) wide.offset[i] = static_cast<uint32_t>((b & 1 ? v.y : v.x) >> kCountShift);
             }
             __syncthreads();
             if (wave == 0) {
@@ -1262,44 +1326,32 @@ __global__ __launch_bounds__(64 * kWideWaves) void sample_wide_kernel(sample_arg
 #pragma unroll
                         for (int e = 0; e < 8; ++e) {
                             const float z = z_of(infinite ? finite_of(l[e]) : l[e], top, p.per);
-                            in = in + in + (step_of(z) == 63 - b ? 1u : 0u);
+                            in = in + in + (step_of(z) == kQuarters - b ? 1u : 0u);
                         }
                     }
                     if (v0 + 4 < kChunk / 512) load4(v0 + 4);
-                    const uint32_t own01 = static_cast<uint32_t>(__popc(in >> 24) | __popc(in >> 16 & 255u) << 16);
-                    const uint32_t own23 = static_cast<uint32_t>(__popc(in >> 8 & 255u) | __popc(in & 255u) << 16);
-                    const uint32_t to01 = wave_scan(own01), to23 = wave_scan(own23);
-                    const uint32_t all01 = lane_value(to01, 63), all23 = lane_value(to23, 63);
-                    const uint32_t n0 = all01 & 0xFFFFu, n1 = n0 + (all01 >> 16), n2 = n1 + (all23 & 0xFFFFu);
-                    const uint32_t to[4] = {at + ((to01 - own01) & 0xFFFFu), at + n0 + ((to01 - own01) >> 16),
-                                            at + n1 + ((to23 - own23) & 0xFFFFu), at + n2 + ((to23 - own23) >> 16)};
-                    at += n2 + (all23 >> 16);
-                    const uint32_t index = static_cast<uint32_t>(i * kChunk + v0 * 512 + lane * 8);
-                    uint32_t left = in;
-                    while (__ballot(left != 0)) {
-                        if (left) {
-                            const uint32_t bit = 31u - static_cast<uint32_t>(__builtin_clz(left)), v = 3 - bit / 8;
-                            const uint32_t before = static_cast<uint32_t>(__popc(in >> bit & (255u >> bit % 8))) - 1;
-                            wide.slot[(v == 0 ? to[0] : v == 1 ? to[1] : v == 2 ? to[2] : to[3]) + before] =
-                                index + v * 512 + 7 - bit % 8;
-                            left ^= 1u << bit;
-                        }
-                    }
+                    uint32_t to[4];
+                    const uint32_t n = places_of(in, to);
+                    const uint32_t index0 = static_cast<uint32_t>(i * kChunk + v0 * 512);
+                    each_picked(in, to, [&](uint32_t place, uint32_t offset) { wide.slot[at + place] = index0 + offset; });
+                    at += n;
                 }
             }
             __syncthreads();
             row_list<kWideWaves, 16, true> part(s.list);
             __syncthreads();
+            float l[16];
 #pragma unroll
             for (int e = 0; e < 16; ++e) {
-                const uint32_t at = part.place(e);
-                const uint32_t given = wide.slot[min(at, n_all - 1)];
-                float l = T::load(logits[given]);
-                if (infinite) l = finite_of(l);
-                l = at < n_all ? l : -INFINITY;
+                part.given[e] = wide.slot[min(part.place(e), n_all - 1)];
+                l[e] = T::load(logits[part.given[e]]);
+            }
+#pragma unroll
+            for (int e = 0; e < 16; ++e) {
+                if (infinite) l[e] = finite_of(l[e]);
+                l[e] = part.place(e) < n_all ? l[e] : -INFINITY;
                 // the bins over this quarter's part of z: -b/4 <= z < (1 - b)/4
-                part.set(e, l, top, p.per, 0.25f * (static_cast<float>(b) - 1.0f), 128.0f * part.kBinsPerBit);
-                part.given[e] = given;
+                part.set(e, l[e], top, p.per, 0.25f * (static_cast<float>(b) - 1.0f), 128.0f * part.kBinsPerBit);
             }
             part.K = K;
             part.I = I;
@@ -1348,10 +1400,10 @@ aq_status launch_long(aq_ctx *ctx, const sample_args &a) {
     c.cap = kSlots / c.chunks / 8 * 8;
     const size_t rows = static_cast<size_t>(a.rows < kRowsAtOnce ? a.rows : kRowsAtOnce), n = rows * c.chunks;
     char *at = nullptr;
-    aq_status st = aq_ctx_scratch(ctx, 7, n * (64 * 8 + 8 + c.cap * 8 + 12) + rows * (4 + sizeof(row_params)), reinterpret_cast<void **>(&at));
+    aq_status st = aq_ctx_scratch(ctx, 7, n * (kBinned * 8 + 8 + c.cap * 8 + 12) + rows * (4 + sizeof(row_params)), reinterpret_cast<void **>(&at));
     if (st != AQ_OK) return st;
     c.bins = reinterpret_cast<uint64_t *>(at);
-    c.weight = c.bins + n * 64;
+    c.weight = c.bins + n * kBinned;
     c.slot = reinterpret_cast<uint2 *>(c.weight + n);
     c.top = reinterpret_cast<uint32_t *>(c.slot + n * c.cap);
     c.count = c.top + n;
