@@ -806,13 +806,14 @@ __global__ __launch_bounds__(256) void sample_chunk_kernel(sample_args a, chunk_
     for (int i = 0; i < kBinned * kCopies / 256; ++i) bins[lane + i % 2 * 64][wave * (kCopies / 4) + i / 2] = 0;
     __syncthreads();
     uint32_t step[32];
+    char *own = reinterpret_cast<char *>(&bins[0][lane % kCopies]);
 #pragma unroll
     for (int e = 0; e < 32; ++e) {
         const float z = z_of(l[e / 8][e % 8], top, p.per);
         const uint32_t w = w_of(z);
         step[e] = step_of(z);
         if (step[e])
-            atomicAdd(reinterpret_cast<unsigned long long *>(&bins[step[e]][lane % kCopies]),
+            atomicAdd(reinterpret_cast<unsigned long long *>(own + __umul24(step[e], sizeof(bins[0]))),
                       (uint64_t{1} << kCountShift) + w);
     }
     __syncthreads();

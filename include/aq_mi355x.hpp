@@ -270,6 +270,27 @@ private:
     aq_moss_quantizer *q_ = nullptr;
 };
 
+// What aq_add_rmsnorm writes, on the device (null: not).  q and scale go
+// together; group: columns per scale, 0 one a row.
+struct NormOutputs {
+    void *sum = nullptr;
+    int64_t sum_ld = 0;
+    void *y = nullptr;
+    int64_t y_ld = 0;
+    aq_dtype q_type = AQ_T_I8;
+    int64_t group = 0;
+    void *q = nullptr;
+    float *scale = nullptr;
+};
+
+// Device rows x (+ residual) [M, D] normalised by their root mean square;
+// residual and weight may be null.
+inline void add_rmsnorm(Context &ctx, aq_dtype type, const void *x, int64_t x_ld, const void *residual,
+                        int64_t residual_ld, const void *weight, int64_t M, int64_t D, float eps, const NormOutputs &o) {
+    ctx.check(aq_add_rmsnorm(ctx.get(), type, x, x_ld, residual, residual_ld, weight, M, D, eps, o.sum, o.sum_ld, o.y,
+                             o.y_ld, o.q_type, o.group, o.q, o.scale));
+}
+
 // A matrix with 4-bit weights and group scales (aq_q4_*).
 class Q4Linear {
 public:
