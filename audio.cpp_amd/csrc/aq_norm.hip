@@ -289,12 +289,28 @@ __global__ __launch_bounds__(1024) void add_rmsnorm_long_kernel(norm_args a) {
     }
 }
 
+// Rows of one launch: a grid has fewer than 2^32 threads.
+constexpr int64_t kRowsAtOnce = int64_t{1} << 21;
+
 template <typename T>
 void launch(aq_ctx *ctx, const norm_args &a) {
-    const int64_t nv = (a.D + 7) / 8;
+    using raw = typename T::raw;
+    const int64_t nv = (a.D + 7) / 8, scales = a.group ? (a.D + a.group - 1) / a.group : 1;
     const auto go = [&](auto kernel, int waves) {
-        const uint32_t grid = static_cast<uint32_t>(waves == 1 ? (a.M + 3) / 4 : a.M);
-        aq_launch_timed(ctx, true, kernel, dim3(grid), dim3(waves == 1 ? 256 : 64 * waves), 0u, a);
+        for (int64_t m = 0; m < a.M; m += kRowsAtOnce) {
+            norm_args b = a;
+            b.M = a.M - m < kRowsAtOnce ? a.M - m : kRowsAtOnce;
+            b.x = static_cast<const raw *>(a.x) + m * a.x_ld;
+            if (a.residual) b.residual = static_cast<const raw *>(a.residual) + m * a.residual_ld;
+            if (a.sum) b.sum = static_cast<raw *>(a.sum) + m * a.sum_ld;
+            if (a.y) b.y = static_cast<raw *>(a.y) + m * a.y_ld;
+            if (a.q) {
+                b.q = static_cast<uint8_t *>(a.q) + m * a.D;
+                b.scale = a.scale + m * scales;
+            }
+            const uint32_t grid = static_cast<uint32_t>(waves == 1 ? (b.M + 3) / 4 : b.M);
+            aq_launch_timed(ctx, true, kernel, dim3(grid), dim3(waves == 1 ? 256 : 64 * waves), 0u, b);
+        }
     };
     // A wave a row needs no barrier, and two vectors a thread cost less than
     // twice the waves, once there are rows for all of the card: 4096 bf16 rows

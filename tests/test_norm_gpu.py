@@ -85,6 +85,26 @@ def test_batches_of_rows(ctx, t, D):
     check(ctx, x, None, w, t, "e4m3", 0)
 
 
+def test_more_rows_than_a_grid_takes(ctx):
+    """Two launches; the last rows against the same rows alone."""
+    M, D = (1 << 21) + 5, 40
+    g = torch.Generator(device="cuda").manual_seed(7)
+    x = torch.randn((M, D), generator=g, device="cuda").bfloat16()
+    r = torch.randn((M, D), generator=g, device="cuda").bfloat16()
+    w = (1 + 0.3 * torch.randn(D, generator=g, device="cuda")).bfloat16()
+
+    def run(x, r):
+        y, q = torch.empty_like(x), torch.empty(x.shape, dtype=torch.int8, device="cuda")
+        h, scale = torch.empty_like(x), torch.empty((len(x), 2), device="cuda")
+        aqmi.add_rmsnorm(ctx, x, w, 1e-6, residual=r, sum=h, y=y, q=q, scale=scale, group=32)
+        return h, y, q, scale
+
+    for whole, part in zip(run(x, r), run(x[-9:], r[-9:])):
+        assert torch.equal(whole[-9:], part)
+    for whole, part in zip(run(x, r), run(x[:7], r[:7])):
+        assert torch.equal(whole[:7], part)
+
+
 @pytest.mark.parametrize("t", TYPES)
 @pytest.mark.parametrize("D,ld", [(100, 103), (1024, 1025), (2050, 2064), (40000, 40003)])
 def test_strided_rows_in_place(ctx, t, D, ld):
