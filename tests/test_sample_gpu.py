@@ -123,6 +123,40 @@ def test_flat_and_peaked_rows(ctx, V, spread):
     check(ctx, l.bfloat16(), 0.5, 700, 0.9, 0.1, seed=5)
 
 
+@pytest.mark.parametrize("V", [5000, 9001, 70000])
+@pytest.mark.parametrize("ahead", [9.0, 14.0, 20.0])
+def test_ends_in_a_far_tail(ctx, V, ahead):
+    """One logit so far ahead that the kept set ends many bits below it."""
+    l = normal(4, V, "f32", V, 1.5)
+    l[:, V // 3] = ahead
+    for p in (0.5, 0.97, 0.9999, 1 - 2.0 ** -24):
+        check(ctx, l, 1.0, None, p, seed=1)
+    check(ctx, l, 1.4, V // 3, 0.999, seed=2)
+    check(ctx, l, 1.0, V // 2, None, 2.0 ** -22, seed=3)
+    check(ctx, l, 1.2, V - 3, 0.999, 1e-5, seed=4)
+    check(ctx, l, 1.0, V - 1, seed=5, u=1.0)
+
+
+@pytest.mark.parametrize("V", [700, 9000, 40000])
+def test_weights_at_the_edges_of_quarter_bits(ctx, V):
+    """z in whole quarters down to below the last weight: a temperature of
+    log2(e) makes z the logits' own difference."""
+    l = -0.25 * (torch.arange(V) * 37 % 133).float().repeat(3, 1)
+    l[1] *= 0.5
+    l[2, : V // 2] = -31.0
+    l[2, V // 2 :] = -31.000002
+    l[2, V // 5] = 0.0
+    l = l.cuda()
+    t = 1.44269504
+    some = int((l[0] >= -31).sum())
+    check(ctx, l, t, seed=1)
+    for k in (some - 1, some, some + 1, V - 1):
+        check(ctx, l, t, k, seed=k, u=0.9999999)
+    for p in (0.5, 0.999999, 1 - 2.0 ** -24):
+        check(ctx, l, t, None, p, seed=2)
+        check(ctx, l, t, V // 2, p, 2.0 ** -30, seed=3)
+
+
 @pytest.mark.parametrize("V", [100, 2000, 6000, 33000, 70000])
 def test_masks(ctx, V):
     lowest = torch.finfo(torch.float32).min
