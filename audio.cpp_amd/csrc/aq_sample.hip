@@ -666,7 +666,7 @@ __global__ __launch_bounds__(64 * WAVES) void sample_short_kernel(sample_args a)
 //     is left even then (min-p's end in a wide set, more than 8192 elements in
 //     a quarter) streams the row.
 //
-// 256 rows of 160000 bf16 logits under top-p take 14, 31, 12 and 47 us (82 MB,
+// 256 rows of 160000 bf16 logits under top-p take 14, 31, 12 and 45 us (82 MB,
 // 17 us at a copy's rate): the first reads at 6 TB/s; the second's time is
 // vector instructions, some 20 an element; the third's and fourth's the
 // latency of one block's steps, the fourth's with the row read again.  One row
@@ -1319,18 +1319,18 @@ __global__ __launch_bounds__(64 * kWideWaves) void sample_wide_kernel(sample_arg
                 };
                 load4(0);
                 for (int v0 = 0; v0 < kChunk / 512 && at < end; v0 += 4) {
+                    float l[4][8];
+#pragma unroll
+                    for (int v = 0; v < 4; ++v) ahead[v].get(l[v]);
+                    if (v0 + 4 < kChunk / 512) load4(v0 + 4);
+                    if (infinite) {
+#pragma unroll
+                        for (int e = 0; e < 32; ++e) l[e / 8][e % 8] = finite_of(l[e / 8][e % 8]);
+                    }
                     uint32_t in = 0;   // 8 bits a vector from the highest down
 #pragma unroll
-                    for (int v = 0; v < 4; ++v) {
-                        float l[8];
-                        ahead[v].get(l);
-#pragma unroll
-                        for (int e = 0; e < 8; ++e) {
-                            const float z = z_of(infinite ? finite_of(l[e]) : l[e], top, p.per);
-                            in = in + in + (step_of(z) == kQuarters - b ? 1u : 0u);
-                        }
-                    }
-                    if (v0 + 4 < kChunk / 512) load4(v0 + 4);
+                    for (int e = 0; e < 32; ++e)
+                        in = in + in + (step_of(z_of(l[e / 8][e % 8], top, p.per)) == kQuarters - b ? 1u : 0u);
                     uint32_t to[4];
                     const uint32_t n = places_of(in, to);
                     const uint32_t index0 = static_cast<uint32_t>(i * kChunk + v0 * 512);
