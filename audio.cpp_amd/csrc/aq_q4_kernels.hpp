@@ -13,7 +13,10 @@
 // instruction with ones for codes, shared by all tiles of rows: no code is
 // converted or corrected on its own.  It is scaled in fp32.  An fp32 x is
 // split into three bf16 parts (8 bits of the mantissa each, by truncation,
-// exact).
+// exact).  The upper part's sums have few bits and are nearly exact; the lower
+// parts have sums of their own, since next to the upper ones, which the offset
+// of 16 + q makes several times the result, they would be rounded at that size
+// (5 x 1000 x 4099, rows of mean 2: 1.4e-6 of the result, and 2e-7 apart).
 //
 // 8-bit x.  Whole numbers stay whole: the nibbles as bytes against x's bytes,
 // and zero * sum(x) taken off (all below 2^24, so exact in fp32 as well).
@@ -85,13 +88,14 @@ template <> struct words<8> {
 };
 
 // What a type of x needs: its element, the operand fragment of 8 columns
-// (PARTS of them for a split x), the operand of a dword of codes and of the
-// correction, and the matrix instruction.
+// (kParts of them for a split x, whose sums go to kSums accumulators: the
+// first part to the first, the others to the last), the operand of a dword of
+// codes and of the correction, and the matrix instruction.
 struct x_f16 {
     using elem = uint16_t;
     using frag = f16x8;
     using acc = f32x4;
-    static constexpr int kParts = 1;
+    static constexpr int kParts = 1, kSums = 1;
     static constexpr bool kScaled = false;
     static __device__ inline void x8(const words<4> &v, frag (&f)[kParts]) { f[0] = __builtin_bit_cast(frag, v.v); }
     static __device__ inline frag codes(uint32_t w) {
@@ -113,7 +117,7 @@ struct x_bf16 {
     using elem = uint16_t;
     using frag = bf16x8;
     using acc = f32x4;
-    static constexpr int kParts = 1;
+    static constexpr int kParts = 1, kSums = 1;
     static constexpr bool kScaled = false;
     static __device__ inline void x8(const words<4> &v, frag (&f)[kParts]) { f[0] = __builtin_bit_cast(frag, v.v); }
     static __device__ inline frag codes(uint32_t w) {
@@ -133,7 +137,7 @@ struct x_bf16 {
 
 struct x_f32 : x_bf16 {
     using elem = float;
-    static constexpr int kParts = 3;
+    static constexpr int kParts = 3, kSums = 2;
     static __device__ inline void x8(const words<8> &v, frag (&f)[kParts]) {
         u32x4 part[3];
 #pragma unroll
@@ -174,7 +178,7 @@ struct x_i8 {
     using elem = uint8_t;
     using frag = long;
     using acc = i32x4;
-    static constexpr int kParts = 1;
+    static constexpr int kParts = 1, kSums = 1;
     static constexpr bool kScaled = true;
     // The columns in the order of the codes' bytes below: 0 4 1 5, 2 6 3 7.
     static __device__ inline void x8(const words<2> &w, frag (&f)[kParts]) {
@@ -207,18 +211,20 @@ struct x_step {
 
 // The scales and zeros of a group, of this lane's four result rows per tile,
 // as they are stored, and the scales of its rows of x.
-template <int RT, int MT>
+template <int RT, int MT, int SUMS>
 struct scales {
     words<2> w[RT];
     words<1> zero[RT];
-    float x[MT], x1[MT];   // a packed x's scale, and its sum over the group
+    float x[MT], x1[SUMS][MT];   // a packed x's scale, and its sums over the group
 };
 
 // PACKED: x and its sums are what q4_pack_kernel wrote.  STREAM: the codes pass
 // the caches once (8192 x 28672: 26.2 us, 27.5 with plain loads); a small
 // matrix, or one that several rows of blocks read, is better left in them.
+// (Two waves a SIMD at least: left free, the packed kernel with two sums takes
+// 268 registers with SUBS = 2, one wave a SIMD, and 220 so, without a spill.)
 template <typename X, bool PACKED, bool AHEAD, bool STREAM, int SUBS, int RT, int MT, int J>
-__global__ __launch_bounds__(PACKED || RT > 2 ? 256 : 512) void q4_product_kernel(args a) {
+__global__ __launch_bounds__(PACKED || RT > 2 ? 256 : 512, PACKED && X::kSums == 2 ? 2 : 1) void q4_product_kernel(args a) {
     using x_t = x_step<X, PACKED, MT, J>;
     extern __shared__ float red[];   // [waves][RT * MT][64][4]
     using frag = typename X::frag;
@@ -269,7 +275,7 @@ __global__ __launch_bounds__(PACKED || RT > 2 ? 256 : 512) void q4_product_kerne
                 }
             }
     };
-    const auto load_scales = [&](int kb, int s, scales<RT, MT> &c) {
+    const auto load_scales = [&](int kb, int s, scales<RT, MT, X::kSums> &c) {
 #pragma unroll
         for (int r = 0; r < RT; ++r) {
             const int64_t at = ((tile[r] + kb) * subs_w + s * subs_w / SUBS) * 16 + 4 * quad;
@@ -281,23 +287,29 @@ __global__ __launch_bounds__(PACKED || RT > 2 ? 256 : 512) void q4_product_kerne
         for (int t = 0; t < MT; ++t)
         {
             c.x[t] = X::kScaled && a.x_group ? xs[t][min(kb * 128 + s * (128 / SUBS), a.K - 1) / a.x_group] : 1.0f;
-            if (PACKED) c.x1[t] = a.x_sum[((static_cast<int64_t>(m0 / 16 + t) * a.kblocks + kb) * SUBS + s) * 16 + col];
+            if (PACKED) {
+                const int64_t at = ((static_cast<int64_t>(m0 / 16 + t) * a.kblocks + kb) * SUBS + s) * X::kSums;
+#pragma unroll
+                for (int i = 0; i < X::kSums; ++i) c.x1[i][t] = a.x_sum[(at + i) * 16 + col];
+            }
         }
     };
 
     f32x4 sum[RT][MT];
-    acc_t acc[RT][MT], all[MT];   // a group's sums of the codes' products, and of x
+    acc_t acc[X::kSums][RT][MT], all[X::kSums][MT];   // a group's sums of the codes' products, and of x
 #pragma unroll
     for (int r = 0; r < RT; ++r)
 #pragma unroll
         for (int t = 0; t < MT; ++t) sum[r][t] = f32x4{0, 0, 0, 0};
     const auto open = [&] {
 #pragma unroll
-        for (int t = 0; t < MT; ++t) {
-            all[t] = acc_t{0, 0, 0, 0};
+        for (int i = 0; i < X::kSums; ++i)
 #pragma unroll
-            for (int r = 0; r < RT; ++r) acc[r][t] = acc_t{0, 0, 0, 0};
-        }
+            for (int t = 0; t < MT; ++t) {
+                all[i][t] = acc_t{0, 0, 0, 0};
+#pragma unroll
+                for (int r = 0; r < RT; ++r) acc[i][r][t] = acc_t{0, 0, 0, 0};
+            }
     };
     const auto add32 = [&](const words<4> (&w)[RT], int at, const x_t &x, int j) {
         frag q[RT];
@@ -314,13 +326,15 @@ __global__ __launch_bounds__(PACKED || RT > 2 ? 256 : 512) void q4_product_kerne
             }
 #pragma unroll
             for (int p = 0; p < X::kParts; ++p) {
-                if (!PACKED) all[t] = X::mma(X::ones(), b[p], all[t]);
+                constexpr int kLast = X::kSums - 1;
+                const int to = p < kLast ? p : kLast;
+                if (!PACKED) all[to][t] = X::mma(X::ones(), b[p], all[to][t]);
 #pragma unroll
-                for (int r = 0; r < RT; ++r) acc[r][t] = X::mma(q[r], b[p], acc[r][t]);
+                for (int r = 0; r < RT; ++r) acc[to][r][t] = X::mma(q[r], b[p], acc[to][r][t]);
             }
         }
     };
-    const auto close = [&](const scales<RT, MT> &c) {
+    const auto close = [&](const scales<RT, MT, X::kSums> &c) {
 #pragma unroll
         for (int r = 0; r < RT; ++r)
 #pragma unroll
@@ -328,18 +342,22 @@ __global__ __launch_bounds__(PACKED || RT > 2 ? 256 : 512) void q4_product_kerne
                 const float ws = aq_types::f16::load(static_cast<uint16_t>(c.w[r][i / 2] >> (i % 2 * 16)));
                 const float less = -X::kBias - static_cast<float>((c.zero[r].v >> (8 * i)) & 255u);
 #pragma unroll
-                for (int t = 0; t < MT; ++t)
-                    sum[r][t][i] = __fmaf_rn(X::kScaled ? ws * c.x[t] : ws,
-                                             __fmaf_rn(less, PACKED ? c.x1[t] : static_cast<float>(all[t][0]),
-                                                       static_cast<float>(acc[r][t][i])),
-                                             sum[r][t][i]);
+                for (int t = 0; t < MT; ++t) {
+                    float v[X::kSums];
+#pragma unroll
+                    for (int p = 0; p < X::kSums; ++p)
+                        v[p] = __fmaf_rn(less, PACKED ? c.x1[p][t] : static_cast<float>(all[p][t][0]),
+                                         static_cast<float>(acc[p][r][t][i]));
+                    if (X::kSums == 2) v[0] += v[X::kSums - 1];
+                    sum[r][t][i] = __fmaf_rn(X::kScaled ? ws * c.x[t] : ws, v[0], sum[r][t][i]);
+                }
             }
     };
 
     const int whole = PACKED ? a.kblocks : a.K / 128;   // k-blocks without columns past the end
     constexpr int kSets = AHEAD ? 2 : 1;
     words<4> w[kSets][RT];
-    scales<RT, MT> c[kSets][SUBS];
+    scales<RT, MT, X::kSums> c[kSets][SUBS];
     x_t x[2];
     const auto load_block = [&](int kb, int d) {
         load_codes(kb, w[d]);
@@ -452,10 +470,10 @@ __global__ __launch_bounds__(PACKED || RT > 2 ? 256 : 512) void q4_product_kerne
 // arithmetic, was what the product waited for (64 rows, 4096 x 16384: 39 us,
 // and 19 with the packing).
 // With them the sums of x over each of a k-block's `subs` parts, [16 rows]
-// [k-block][subs][16], as the products' groups need them.
+// [k-block][subs][kSums][16], as the products' groups need them.
 template <typename X>
 __global__ __launch_bounds__(256) void q4_pack_kernel(args a, void *to, float *sums, int subs) {
-    __shared__ float part[4][16];
+    __shared__ float part[4][X::kSums][16];
     using elem = typename X::elem;
     using frag = typename X::frag;
     const int lane = threadIdx.x & 63, j = threadIdx.x >> 6;
@@ -481,16 +499,28 @@ __global__ __launch_bounds__(256) void q4_pack_kernel(args a, void *to, float *s
     const int64_t at = (static_cast<int64_t>(blockIdx.y) * a.kblocks + kb) * 4 + j;
 #pragma unroll
     for (int p = 0; p < X::kParts; ++p) static_cast<frag *>(to)[(at * X::kParts + p) * 64 + lane] = f[p];
-    typename X::acc all{0, 0, 0, 0};
+    typename X::acc all[X::kSums];
 #pragma unroll
-    for (int p = 0; p < X::kParts; ++p) all = X::mma(X::ones(), f[p], all);   // each lane: its row's 32 columns
-    if (lane < 16) part[j][lane] = static_cast<float>(all[0]);
+    for (int i = 0; i < X::kSums; ++i) all[i] = typename X::acc{0, 0, 0, 0};
+#pragma unroll
+    for (int p = 0; p < X::kParts; ++p) {   // each lane: its row's 32 columns
+        constexpr int kLast = X::kSums - 1;
+        const int to_sum = p < kLast ? p : kLast;
+        all[to_sum] = X::mma(X::ones(), f[p], all[to_sum]);
+    }
+    if (lane < 16) {
+#pragma unroll
+        for (int i = 0; i < X::kSums; ++i) part[j][i][lane] = static_cast<float>(all[i][0]);
+    }
     __syncthreads();
-    const int per = 4 / subs;
-    if (threadIdx.x < 16 * subs) {
-        float sum = 0.0f;
-        for (int i = 0; i < per; ++i) sum += part[threadIdx.x / 16 * per + i][lane & 15];
-        sums[((static_cast<int64_t>(blockIdx.y) * a.kblocks + kb) * subs + threadIdx.x / 16) * 16 + (lane & 15)] = sum;
+    const int per = 4 / subs, s = threadIdx.x / 16;
+    if (s < subs) {
+#pragma unroll
+        for (int i = 0; i < X::kSums; ++i) {
+            float sum = 0.0f;
+            for (int k32 = 0; k32 < per; ++k32) sum += part[s * per + k32][i][lane & 15];
+            sums[(((static_cast<int64_t>(blockIdx.y) * a.kblocks + kb) * subs + s) * X::kSums + i) * 16 + (lane & 15)] = sum;
+        }
     }
 }
 
@@ -521,17 +551,19 @@ aq_status launch_subs(aq_ctx *ctx, const args &a) {
     // and at K = 8192, 1792 tiles: two 30.3 and 47.2, 33.3 and 43.0, four 28.4
     // and 31.8, 36.3 and 34.5.  With 32 columns a scale four tiles' scales do
     // not fit the registers; there one row (bf16, 1792 tiles) takes 49 us with
-    // one tile, 67 with two, 16 rows 74 and 70.
+    // one tile, 67 with two, 16 rows 74 and 70, fp32 96 and 96, 129 and 109.
     if (a.M <= 16) {
         const bool few = a.M <= 4;
         // A wave has one k-block: no loads ahead, less code to fetch (1000 x
         // 4099, five fp32 rows: 6.0 us, 8.2 with them).
         if (a.kblocks <= 8) return launch_shape<X, false, false, false, SUBS, 1, 1, 4>(ctx, a, 8);
         if (a.tiles < 512) return launch_shape<X, false, true, false, SUBS, 1, 1, 4>(ctx, a, 8);
-        if (a.tiles < (few ? 1536 : 1024)) return launch_shape<X, false, true, true, SUBS, 2, 1, 4>(ctx, a, 8);
+        // Two tiles' sums of an fp32 x leave registers for half a k-block of it.
+        constexpr int kJ = SUBS == 4 && X::kSums == 2 ? 2 : 4;
+        if (a.tiles < (few ? 1536 : 1024)) return launch_shape<X, false, true, true, SUBS, 2, 1, kJ>(ctx, a, 8);
         if constexpr (SUBS < 4) return launch_shape<X, false, true, true, SUBS, 4, 1, 4>(ctx, a, 4);
         else if (few) return launch_shape<X, false, true, true, SUBS, 1, 1, 4>(ctx, a, 4);
-        else return launch_shape<X, false, true, true, SUBS, 2, 1, 4>(ctx, a, 4);
+        else return launch_shape<X, false, true, true, SUBS, 2, 1, kJ>(ctx, a, 4);
     }
     // Packed batches of rows, at most 64 MB of them (but 64 rows).
     const int64_t row_bytes = static_cast<int64_t>(a.kblocks) * 16 * sizeof(typename X::frag) * X::kParts;
@@ -540,7 +572,7 @@ aq_status launch_subs(aq_ctx *ctx, const args &a) {
     if (rows > (a.M + 63) / 64 * 64) rows = (a.M + 63) / 64 * 64;
     char *packed = nullptr;
     const size_t bytes = static_cast<size_t>(rows * row_bytes);
-    aq_status st = aq_ctx_scratch(ctx, 8, bytes + static_cast<size_t>(rows) * a.kblocks * SUBS * 4,
+    aq_status st = aq_ctx_scratch(ctx, 8, bytes + static_cast<size_t>(rows) * a.kblocks * SUBS * X::kSums * 4,
                                   reinterpret_cast<void **>(&packed));
     if (st != AQ_OK) return st;
     float *sums = reinterpret_cast<float *>(packed + bytes);
@@ -557,10 +589,15 @@ aq_status launch_subs(aq_ctx *ctx, const args &a) {
         // 64 rows of x at once where the registers hold their sums and that
         // leaves two blocks a compute unit, else 32: 64 rows, K = 4096, bf16:
         // 14.2 and 10.7 us for 4096 columns, 19.5 and 20.2 for 16384.
+        // With 32 columns a scale the two sums of an fp32 x leave registers
+        // for one tile and 16 rows: in us for 4096 and 16384 columns, 64 rows
+        // 30 and 93, 30 and 102 as the others have it, 256 rows 88 and 327, 105
+        // and 384.
         constexpr bool kWide = SUBS != 4 && X::kParts == 1;
+        constexpr int kTiles = SUBS == 4 && X::kSums == 2 ? 1 : 2;
         const int64_t blocks = static_cast<int64_t>((a.tiles + 1) / 2) * ((b.M + 63) / 64);
-        if (kWide && blocks >= 512 && b.M > 32) st = launch_shape<X, true, true, false, SUBS, 2, kWide ? 4 : 2, 1>(ctx, b, 4);
-        else st = launch_shape<X, true, true, false, SUBS, 2, 2, X::kParts == 1 ? 2 : 1>(ctx, b, 4);
+        if (kWide && blocks >= 512 && b.M > 32) st = launch_shape<X, true, true, false, SUBS, kTiles, kWide ? 4 : kTiles, 1>(ctx, b, 4);
+        else st = launch_shape<X, true, true, false, SUBS, kTiles, kTiles, X::kParts == 1 ? 2 : 1>(ctx, b, 4);
         if (st != AQ_OK) return st;
     }
     return AQ_OK;
