@@ -26,12 +26,15 @@ struct aq_ctx {
     // 8: rows of x in operand order).
     static constexpr int kScratchSlots = 9;
     // Slots from here on (tens of MB at most, but for rows of millions of
-    // columns) at least double when they grow, and leave the buffers that they
-    // outgrow allocated until the context ends: a captured graph of a call
-    // goes on using its own.
+    // columns) at least double when they grow, where the memory is there, and
+    // leave the buffers that they outgrow allocated until the context ends: a
+    // captured graph of a call goes on using its own.
     static constexpr int kFirstKept = 7;
-    void *outgrown[(kScratchSlots - kFirstKept) * 64] = {};   // a size doubles fewer than 64 times
-    int outgrown_count = 0;
+    struct kept_buffer {
+        void *p;
+        kept_buffer *next;
+    };
+    kept_buffer *outgrown = nullptr;
     // Per-stage counters of the last Euclidean encode on this context (in
     // slot 1, or in the no-allocation scratch).
     int32_t *euclid_counts = nullptr;

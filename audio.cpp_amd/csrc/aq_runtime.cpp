@@ -2,6 +2,7 @@
 #include "aq_internal.hpp"
 
 #include <mutex>
+#include <new>
 #include <unordered_map>
 
 size_t aq_static_lds(const void *fn) {
@@ -21,12 +22,21 @@ aq_status aq_ctx_scratch(aq_ctx *ctx, int slot, size_t bytes, void **out) {
     if (bytes > ctx->scratch_bytes[slot]) {
         aq_device_guard g(ctx->device);
         if (slot >= aq_ctx::kFirstKept) {
+            aq_ctx::kept_buffer *old = nullptr;
+            if (ctx->scratch[slot] && !(old = new (std::nothrow) aq_ctx::kept_buffer{ctx->scratch[slot], ctx->outgrown}))
+                return aq_fail(ctx, AQ_E_NOMEM, "host allocation failed");
             void *grown = nullptr;
-            if (bytes < 2 * ctx->scratch_bytes[slot]) bytes = 2 * ctx->scratch_bytes[slot];
-            if (hipMalloc(&grown, bytes) != hipSuccess)
+            const size_t twice = 2 * ctx->scratch_bytes[slot];
+            size_t size = bytes < twice ? twice : bytes;
+            hipError_t e = hipMalloc(&grown, size);
+            if (e != hipSuccess && size > bytes) e = hipMalloc(&grown, size = bytes);
+            (void)hipGetLastError();   // what was not to be had is no error of the launches that follow
+            if (e != hipSuccess) {
+                delete old;
                 return aq_fail(ctx, AQ_E_NOMEM, "work buffer of %zu bytes could not be allocated", bytes);
-            if (ctx->scratch[slot]) ctx->outgrown[ctx->outgrown_count++] = ctx->scratch[slot];
-            ctx->scratch_bytes[slot] = bytes;
+            }
+            if (old) ctx->outgrown = old;
+            ctx->scratch_bytes[slot] = size;
             *out = ctx->scratch[slot] = grown;
             return AQ_OK;
         }
@@ -133,7 +143,12 @@ aq_status aq_ctx_destroy(aq_ctx *ctx) {
         if (ctx->d_flags) (void)hipFree(ctx->d_flags);
         for (int i = 0; i < aq_ctx::kScratchSlots; ++i)
             if (ctx->scratch[i]) (void)hipFree(ctx->scratch[i]);
-        for (int i = 0; i < ctx->outgrown_count; ++i) (void)hipFree(ctx->outgrown[i]);
+        while (ctx->outgrown) {
+            aq_ctx::kept_buffer *const b = ctx->outgrown;
+            ctx->outgrown = b->next;
+            (void)hipFree(b->p);
+            delete b;
+        }
         for (hipEvent_t e : ctx->ev_start) (void)hipEventDestroy(e);
         for (hipEvent_t e : ctx->ev_stop) (void)hipEventDestroy(e);
     }
