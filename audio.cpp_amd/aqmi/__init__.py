@@ -156,7 +156,11 @@ def _rows(t, rows: int, cols: int, dtype: int | None = None):
 
 
 class Context:
-    """aq_ctx on one device, bound to torch's current stream of that device."""
+    """aq_ctx on one device, bound to torch's current stream of that device.
+
+    Calls on one context share its scratch.  A call on another stream than
+    the last one's waits on the device for that one; what is captured into a
+    graph neither waits nor is waited for (its replay is the caller's to order)."""
 
     def __init__(self, device: int = 0, lib: C.CDLL | None = None):
         import torch
@@ -175,13 +179,35 @@ class Context:
         if st != AQ_OK:
             raise AqError(st, "aq_ctx_create failed")
         self.h = h
+        self._last = torch.cuda.current_stream(device)   # of the last call that was not captured
+        self._last_raw = stream
 
     def check(self, st: int):
         if st != AQ_OK:
             raise AqError(st, self.lib.aq_last_error(self.h).decode())
 
     def use_current_stream(self):
-        self.check(self.lib.aq_ctx_set_stream(self.h, self._raw_stream(self.device)))
+        raw = self._raw_stream(self.device)
+        if raw != self._last_raw:
+            self._follow(raw)
+        self.check(self.lib.aq_ctx_set_stream(self.h, raw))
+
+    def _follow(self, raw: int):
+        """The current stream waits for the last call's, unless one of them is being captured."""
+        cuda = self.torch.cuda
+        now, last = cuda.current_stream(self.device), self._last
+        if self._capturing(now):
+            return
+        try:
+            if not self._last_raw or not self._capturing(last):
+                now.wait_stream(last)
+        except RuntimeError:   # an external stream that is no more
+            cuda.synchronize(self.device)
+        self._last, self._last_raw = now, raw
+
+    def _capturing(self, stream) -> bool:
+        with self.torch.cuda.stream(stream):
+            return self.torch.cuda.is_current_stream_capturing()
 
     def synchronize(self):
         self.check(self.lib.aq_ctx_synchronize(self.h))
