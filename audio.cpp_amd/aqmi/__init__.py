@@ -576,17 +576,22 @@ def q4_quantize(w: np.ndarray, group: int, zeros: bool = False):
     """A float32 matrix [out, in] as (codes, scale, zero) of aq_q4_upload, on
     the host: per row and group of columns a float16 scale (the largest
     magnitude over 7, or the range over 15 with `zeros`) and each weight's
-    nearest code."""
+    nearest code.  ValueError where a scale is not a finite float16: a weight
+    that is not finite, or magnitudes above some 458000 (a range above 982000)."""
     N, K = w.shape
     groups = -(-K // group)
     g = np.zeros((N, groups * group), np.float32)
     g[:, :K] = w
     g = g.reshape(N, groups, group)
-    if zeros:
-        lo, hi = np.minimum(g.min(2), 0), np.maximum(g.max(2), 0)
-        scale = ((hi - lo) / 15).astype(np.float16)
-    else:
-        scale = (np.abs(g).max(2) / 7).astype(np.float16)
+    with np.errstate(over="ignore", invalid="ignore"):
+        if zeros:
+            lo, hi = np.minimum(g.min(2), 0), np.maximum(g.max(2), 0)
+            scale = ((hi - lo) / 15).astype(np.float16)
+        else:
+            scale = (np.abs(g).max(2) / 7).astype(np.float16)
+    if not np.isfinite(scale).all():
+        n, at = np.argwhere(~np.isfinite(scale))[0]
+        raise ValueError(f"row {n}, columns from {at * group}: the weights' range has no finite float16 scale")
     inv = np.divide(1, scale, out=np.zeros(scale.shape, np.float32), where=scale > 0, dtype=np.float32)
     zero = np.clip(np.rint(-lo * inv), 0, 15).astype(np.uint8) if zeros else None
     codes = np.clip(np.rint(g * inv[:, :, None]) + (zero[:, :, None] if zeros else 8), 0, 15).astype(np.uint8)
