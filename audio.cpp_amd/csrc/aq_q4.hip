@@ -118,6 +118,7 @@ aq_status aq_q4_upload(aq_ctx *ctx, int64_t out_features, int64_t in_features, i
         if (p) (void)hipFree(p);
     if (e != hipSuccess) {
         free_all(w);
+        (void)hipGetLastError();   // reported below, and no error of the caller's next launch
         return aq_fail(ctx, e == hipErrorOutOfMemory ? AQ_E_NOMEM : AQ_E_DEVICE, "aq_q4_upload: %s", hipGetErrorString(e));
     }
     *out = w;

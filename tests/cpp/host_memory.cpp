@@ -113,11 +113,39 @@ aq_status sampled(aq_ctx *ctx, int64_t rows) {
                      nullptr);
 }
 
+// An upload that runs out of memory at each of its allocations in turn.
+void refused_uploads(aq_ctx *ctx) {
+    const uint8_t codes[32 * 32] = {}, zero[32 * 2] = {};
+    const uint16_t scale[32 * 2] = {};
+    const float bias[32] = {};
+    const size_t before = used;
+    aq_q4 *w = nullptr;
+    limit = SIZE_MAX;
+    expect(aq_q4_upload(ctx, 32, 64, 32, codes, scale, zero, bias, &w) == AQ_OK, "an upload");
+    const size_t held = used - before;
+    expect(aq_q4_release(w) == AQ_OK && used == before, "and its release");
+    bool refused = true, clean = true, freed = true;
+    int refusals = 0;
+    for (limit = before; limit < before + held; limit += 64) {
+        const aq_status st = aq_q4_upload(ctx, 32, 64, 32, codes, scale, zero, bias, &w);
+        refused &= st == AQ_E_NOMEM && !w;
+        clean &= last == hipSuccess;
+        freed &= used == before;
+        last = hipSuccess;
+        ++refusals;
+    }
+    expect(refusals > 5 && refused, "uploads without room are refused");
+    expect(freed, "and hold nothing");
+    expect(clean, "and leave no error behind");
+    limit = SIZE_MAX;
+}
+
 }  // namespace
 
 int main() {
     aq_ctx *ctx = nullptr;
     expect(aq_ctx_create(0, nullptr, &ctx) == AQ_OK, "context");
+    refused_uploads(ctx);
     const size_t before = used;
     expect(sampled(ctx, 8) == AQ_OK, "first call");
     const size_t eight = used - before;
