@@ -88,10 +88,19 @@ __device__ inline void store_q8(void *q, int64_t row, int64_t D, int64_t at, uin
     }
 }
 
+// 1 / sqrt(m), root = sqrt(m) rounded: the reciprocal's error comes from what
+// is left of 1 - m r^2, so the result is within little more than half a unit,
+// where the two roundings alone give up to one and a half.
+__device__ inline float inverse_root(float m, float root) {
+    const float r = 1.0f / root, t = m * r;
+    const float left = __fmaf_rn(-__fmaf_rn(m, r, -t), r, __fmaf_rn(-t, r, 1.0f));
+    return left == left ? __fmaf_rn(0.5f * r, left, r) : r;   // not for m = 0 or infinity
+}
+
 // max |y| / L from max |p| and the root: by the product of root and L, two
 // roundings, where 1 / root, max |y| and its quotient would be three.
-__device__ inline float scale_of(float pmax, float root, bool e4m3) {
-    if (!(pmax * (1.0f / root) < INFINITY)) return NAN;   // y is not finite
+__device__ inline float scale_of(float pmax, float root, float r, bool e4m3) {
+    if (!(pmax * r < INFINITY)) return NAN;   // y is not finite
     return pmax < kLeastMax ? 0.0f : pmax / (root * (e4m3 ? 448.0f : 127.0f));
 }
 
@@ -166,11 +175,11 @@ __global__ __launch_bounds__(WAVES == 1 ? 256 : 64 * WAVES) void add_rmsnorm_ker
             rowmax = mag_max(rowmax, part[1][w]);
         }
     }
-    const float root = aq_math::sqrt_rn(ss / static_cast<float>(a.D) + a.eps), r = 1.0f / root;
+    const float mean = ss / static_cast<float>(a.D) + a.eps, root = aq_math::sqrt_rn(mean), r = inverse_root(mean, root);
 
     const bool e4m3 = a.q_type == AQ_T_E4M3;
     const int64_t groups = a.group ? (a.D + a.group - 1) / a.group : 1;
-    if (a.q && !a.group && tid == 0) a.scale[row] = scale_of(rowmax, root, e4m3);
+    if (a.q && !a.group && tid == 0) a.scale[row] = scale_of(rowmax, root, r, e4m3);
 #pragma unroll
     for (int v = 0; v < VPT; ++v) {
         const int64_t at = static_cast<int64_t>(v * kThreads + tid) * 8;
@@ -189,7 +198,7 @@ __global__ __launch_bounds__(WAVES == 1 ? 256 : 64 * WAVES) void add_rmsnorm_ker
         }
         if (a.q) {
             store_q8(a.q, row, a.D, at, quantize8(p[v], inverse_of(m, e4m3), e4m3));
-            if (a.group && at % a.group == 0) a.scale[row * groups + at / a.group] = scale_of(m, root, e4m3);
+            if (a.group && at % a.group == 0) a.scale[row * groups + at / a.group] = scale_of(m, root, r, e4m3);
         }
     }
 }
@@ -253,11 +262,11 @@ __global__ __launch_bounds__(1024) void add_rmsnorm_long_kernel(norm_args a) {
         ss += part[0][w];
         rowmax = mag_max(rowmax, part[1][w]);
     }
-    const float root = aq_math::sqrt_rn(ss / static_cast<float>(a.D) + a.eps), r = 1.0f / root;
+    const float mean = ss / static_cast<float>(a.D) + a.eps, root = aq_math::sqrt_rn(mean), r = inverse_root(mean, root);
 
     const bool e4m3 = a.q_type == AQ_T_E4M3;
     const int64_t groups = a.group ? (a.D + a.group - 1) / a.group : 1;
-    if (a.q && !a.group && threadIdx.x == 0) a.scale[row] = scale_of(rowmax, root, e4m3);
+    if (a.q && !a.group && threadIdx.x == 0) a.scale[row] = scale_of(rowmax, root, r, e4m3);
     for (int64_t base = 0; base < a.D; base += 8192) {
         const int64_t at = base + threadIdx.x * 8;
         float p[8] = {};
@@ -284,7 +293,7 @@ __global__ __launch_bounds__(1024) void add_rmsnorm_long_kernel(norm_args a) {
             }
             if (a.q) {
                 store_q8(a.q, row, a.D, at, quantize8(p, inverse_of(m, e4m3), e4m3));
-                if (a.group && at % a.group == 0) a.scale[row * groups + at / a.group] = scale_of(m, root, e4m3);
+                if (a.group && at % a.group == 0) a.scale[row * groups + at / a.group] = scale_of(m, root, r, e4m3);
             }
         }
     }

@@ -40,3 +40,19 @@ def test_rounded_once(ctx, t, dt, most, group, D):
     scale = torch.empty((len(TRIPLES), D // group if group else 1), device="cuda")
     aqmi.add_rmsnorm(ctx, x, None, 0.0, q=q, scale=scale, group=group)
     assert np.array_equal(scale.cpu().numpy(), np.array(want, np.float32))
+
+
+@pytest.mark.parametrize("D", [64, 1024, 8192, 65536])
+def test_root_within_half_a_unit(ctx, D):
+    """Rows of one power of two: with an eps that is a multiple of 2^-10 the
+    mean is exact, and y is 1 / root times that power.  The root's reciprocal
+    is 2^-24 of itself off at most, and little more than half a unit means a
+    hundredth beyond that."""
+    h = torch.tensor([0.5, 1.0, 8.0], device="cuda")
+    x = h[:, None].expand(3, D).contiguous()
+    y = torch.empty_like(x)
+    for k in range(1, 200):
+        aqmi.add_rmsnorm(ctx, x, None, k * 2.0 ** -10, y=y)
+        ref = h.double() / (h.double().square() + k * 2.0 ** -10).sqrt()
+        assert bool((y == y[:, :1]).all())
+        assert bool(((y[:, 0].double() / ref - 1).abs() <= 1.01 * 2.0 ** -24).all()), k
