@@ -596,8 +596,12 @@ aq_status launch_subs(aq_ctx *ctx, const args &a) {
         constexpr bool kWide = SUBS != 4 && X::kParts == 1;
         constexpr int kTiles = SUBS == 4 && X::kSums == 2 ? 1 : 2;
         const int64_t blocks = static_cast<int64_t>((a.tiles + 1) / 2) * ((b.M + 63) / 64);
-        if (kWide && blocks >= 512 && b.M > 32) st = launch_shape<X, true, true, false, SUBS, kTiles, kWide ? 4 : kTiles, 1>(ctx, b, 4);
-        else st = launch_shape<X, true, true, false, SUBS, kTiles, kTiles, X::kParts == 1 ? 2 : 1>(ctx, b, 4);
+        bool wide = false;
+        if constexpr (kWide) {
+            wide = blocks >= 512 && b.M > 32;
+            if (wide) st = launch_shape<X, true, true, false, SUBS, 2, 4, 1>(ctx, b, 4);
+        }
+        if (!wide) st = launch_shape<X, true, true, false, SUBS, kTiles, kTiles, X::kParts == 1 ? 2 : 1>(ctx, b, 4);
         if (st != AQ_OK) return st;
     }
     return AQ_OK;
