@@ -12,9 +12,14 @@
 // 32, 64 or 128 columns and its maximum is a butterfly within them.
 //
 // Bound by memory: 16384 bf16 rows of 8192 with every output (1.2 GB) take
-// 219 us, 5.5 TB/s, 6000 f16 rows of 4096 without y (172 MB) 35.5 us, 4.8
-// TB/s; a copy of 2 GB runs at 4.8 TB/s on the same card.  A single row is
-// latency: 3.2 us for 1024 columns, the launch, a load, a reduction.
+// 218 us, 5.5 TB/s, 6000 f16 rows of 4096 without y (172 MB) 35.5 us, 4.8
+// TB/s; a copy of 2 GB runs at 4.8 TB/s on the same card.  Few rows are bound
+// by latency: a thread waits for its vector of x, then of residual, then of
+// weight (a test of the row's end in each lane and the store of the sum lie
+// between the loads), and for the next vector only after those (fp32: x and
+// residual together).  One row of 1024 takes 3.0 us, the launch, three such
+// waits and the reduction; 1499 fp32 rows of 1001, 1.5 waves a SIMD that wait
+// four times each, 10 us, where the bytes need 5.3.
 #include "aq_device_math.hpp"
 #include "aq_internal.hpp"
 #include "aq_types.hpp"

@@ -25,9 +25,13 @@
 // What bounds it.  Up to 16 rows of x, the codes' way from memory: 8192 x
 // 28672, one int8 row, 121 MB in 26 us, 4.7 TB/s, where a copy of 2 GB runs
 // at 4.8.  Small matrices, latency: 1024 x 12288, one bf16 row, 5.6 us.  Many
-// rows, the waits of few waves with many registers: 64 rows of f16 by 4096 x
-// 16384 18.7 us with 3 us of packing, 37.7 MB and 8.6 GFLOP, of which the
-// matrix instructions take 37 % of the time and the codes' conversion as much.
+// rows, x from the caches and few waves to wait for it: for 64 rows of f16 by
+// 4096 x 16384 each of 512 blocks of two tiles reads all of the packed x, 268
+// MB beside 38 MB from memory, with two waves a SIMD (196 registers): 19 us
+// with 3 us of packing, the matrix instructions 37 % of it and the codes'
+// conversion as much.  Groups of 64 and 32 columns hold more scales: their
+// packed kernels have 280 to 320 registers there, one wave a SIMD, and take 36
+// to 42 and 67 to 73 us.
 #pragma once
 #include "aq_internal.hpp"
 #include "aq_q4.hpp"
@@ -549,7 +553,8 @@ aq_status launch_subs(aq_ctx *ctx, const args &a) {
     //   1024 tiles, two    10.7  15.4    11.3  14.5
     //               four   11.4  12.4    14.4  14.7
     // and at K = 8192, 1792 tiles: two 30.3 and 47.2, 33.3 and 43.0, four 28.4
-    // and 31.8, 36.3 and 34.5.  With 32 columns a scale four tiles' scales do
+    // and 31.8, 36.3 and 34.5: the bound for few rows follows int8, and a
+    // floating row is 3 us slower there with four tiles than with two.  With 32 columns a scale four tiles' scales do
     // not fit the registers; there one row (bf16, 1792 tiles) takes 49 us with
     // one tile, 67 with two, 16 rows 74 and 70, fp32 96 and 96, 129 and 109.
     if (a.M <= 16) {
@@ -586,9 +591,10 @@ aq_status launch_subs(aq_ctx *ctx, const args &a) {
         aq_launch_timed(ctx, false, q4_pack_kernel<X>, grid, dim3(256), 0u, b, static_cast<void *>(packed), sums, SUBS);
         b.x = packed;
         b.x_sum = sums;
-        // 64 rows of x at once where the registers hold their sums and that
-        // leaves two blocks a compute unit, else 32: 64 rows, K = 4096, bf16:
-        // 14.2 and 10.7 us for 4096 columns, 19.5 and 20.2 for 16384.
+        // 64 rows of x at once where the registers hold their sums and the
+        // grid has two blocks a compute unit, else 32: 64 rows, K = 4096, bf16:
+        // 14.2 and 10.7 us for 4096 columns, 19.5 and 20.2 for 16384.  (With
+        // 64 columns a scale only one of the two fits a compute unit at a time.)
         // With 32 columns a scale the two sums of an fp32 x leave registers
         // for one tile and 16 rows: in us for 4096 and 16384 columns, 64 rows
         // 30 and 93, 30 and 102 as the others have it, 256 rows 88 and 327, 105

@@ -670,7 +670,13 @@ __global__ __launch_bounds__(64 * WAVES) void sample_short_kernel(sample_args a)
 // 17 us at a copy's rate): the first reads at 6 TB/s; the second's time is
 // vector instructions, some 20 an element; the third's and fourth's the
 // latency of one block's steps, the fourth's with the row read again.  One row
-// of 131071: 2.5, 6, 9 and 1.
+// of 131071: 2.5, 6, 9 and 1.  In the first two and in the draw a thread's
+// four loads wait for each other (each tests the row's end in its lanes),
+// which many blocks a compute unit hide and one row does not.
+// Without filters, or with min-p alone, 43 and 13 us.  A row that is streamed
+// is read five times or more by its one block: 320 and 147 us where min-p
+// ends in a wide nucleus, 428 and 224 where its quarter has more than 8192
+// elements, 703 and 384 with top-k too.
 constexpr int kChunk = 8192;          // 256 threads, 32 elements each
 constexpr int kSlots = 2048;          // candidates of a row: 256 threads, 8 each
 constexpr int kWideWaves = 8;         // of a block in the fourth launch: with twice as many its registers spill
