@@ -35,6 +35,7 @@ EXPORTED = [
     "aq_dac_encode_ex", "aq_dac_decode_ex", "aq_euclid_upload_device", "aq_weight_norm_fold",
     "aq_linear_upload", "aq_linear_forward", "aq_linear_release",
     "aq_add_rmsnorm", "aq_q4_upload", "aq_q4_forward", "aq_q4_release", "aq_sample",
+    "aq_i8_upload", "aq_i8_forward", "aq_i8_release",
 ]
 
 # aq_euclid_recipe / aq_codebook_type
@@ -92,6 +93,9 @@ def load_library(path: str | pathlib.Path | None = None) -> C.CDLL:
     lib.aq_q4_upload.argtypes = [vp, i64, i64, i64, vp, vp, vp, vp, C.POINTER(vp)]
     lib.aq_q4_forward.argtypes = [vp, vp, C.c_int, vp, i64, vp, i64, i64, C.c_int, vp, i64]
     lib.aq_q4_release.argtypes = [vp]
+    lib.aq_i8_upload.argtypes = [vp, i64, i64, vp, vp, vp, C.POINTER(vp)]
+    lib.aq_i8_forward.argtypes = [vp, vp, C.c_int, vp, i64, vp, i64, C.c_int, vp, i64]
+    lib.aq_i8_release.argtypes = [vp]
     lib.aq_sample.argtypes = [vp, C.c_int, vp, i64, i64, i64, vp, vp, vp, vp, vp, vp, vp]
     lib.aq_euclid_decode.argtypes = [vp, vp, vp, i64, vp]
     lib.aq_euclid_encode_noalloc.argtypes = [vp, vp, vp, i64, vp, vp, vp, C.c_int, vp, vp, vp]
@@ -646,6 +650,66 @@ class Q4Linear:
     def close(self):
         if getattr(self, "h", None):
             self.ctx.lib.aq_q4_release(self.h)
+            self.h = None
+
+    def __del__(self):
+        try:
+            self.close()
+        except Exception:
+            pass
+
+
+def i8_quantize(w: np.ndarray):
+    """A float32 matrix [out, in] as (codes, scale) of aq_i8_upload, on the
+    host: per row the largest magnitude over 127 and each weight's nearest whole
+    number.  ValueError where a weight is not finite."""
+    most = np.abs(w).max(1).astype(np.float64)
+    if not np.isfinite(most).all():
+        raise ValueError(f"row {np.argwhere(~np.isfinite(most))[0, 0]} has a weight that is not finite")
+    inv = np.divide(127.0, most, out=np.zeros(most.shape), where=most > 0)
+    return np.rint(w * inv[:, None]).astype(np.int8), (most / 127).astype(np.float32)
+
+
+class I8Linear:
+    """aq_i8: a matrix [out, in] with 8-bit whole-number weights.
+
+    Host arrays: codes int8 [out, in], scale float32 [out], bias float32 [out]
+    or None."""
+
+    def __init__(self, ctx: Context, codes, scale, bias=None):
+        if codes.dtype != np.int8 or codes.ndim != 2:
+            raise ValueError("codes must be int8 [out, in]")
+        self.ctx, (self.out_features, self.in_features) = ctx, codes.shape
+        if scale.dtype != np.float32 or scale.shape != (self.out_features,):
+            raise ValueError(f"scale must be float32 ({self.out_features},)")
+        if bias is not None and bias.shape != (self.out_features,):
+            raise ValueError(f"bias must be float32 ({self.out_features},)")
+        codes, scale = np.ascontiguousarray(codes), np.ascontiguousarray(scale)
+        bias = None if bias is None else np.ascontiguousarray(bias, np.float32)
+        ptr = [None if a is None else a.ctypes.data_as(C.c_void_p) for a in (codes, scale, bias)]
+        h = C.c_void_p()
+        ctx.use_current_stream()
+        ctx.check(ctx.lib.aq_i8_upload(ctx.h, self.out_features, self.in_features, *ptr, C.byref(h)))
+        self.h = h
+
+    def forward(self, x, out, scale=None):
+        """out [M, out_features] = x [M, in_features] W^T (+ bias); both device
+        matrices, rows may be strided.  x is int8 with a float32 scale [M], or
+        of a floating type, which is brought to 8 bits row by row; out is of any
+        floating type."""
+        M, t = x.shape[0], _dtype(x)
+        if t == T_I8:
+            if scale is None or scale.numel() != M or _dtype(scale) != T_F32:
+                raise ValueError(f"an int8 x needs a float32 scale of ({M},)")
+        elif scale is not None:
+            raise ValueError("scale belongs to an int8 x")
+        self.ctx.use_current_stream()
+        self.ctx.check(self.ctx.lib.aq_i8_forward(self.ctx.h, self.h, t, *_rows(x, M, self.in_features), _dptr(scale), M,
+                                                  _dtype(out), *_rows(out, M, self.out_features)))
+
+    def close(self):
+        if getattr(self, "h", None):
+            self.ctx.lib.aq_i8_release(self.h)
             self.h = None
 
     def __del__(self):

@@ -556,6 +556,37 @@ aq_status aq_q4_forward(aq_ctx *ctx, const aq_q4 *w, int x_type, const void *x, 
                         int64_t x_group, int64_t M, int y_type, void *y, int64_t y_ld);
 aq_status aq_q4_release(aq_q4 *w);
 
+/* Products with 8-bit whole-number weights, a scale for each row of W and each
+ * row of x:
+ *   y[m, n] = (sum_k xq[m, k] * w[n, k]) * scale[n] * x_scale[m]  (+ bias[n])
+ * x is an 8-bit row with its scale (what aq_add_rmsnorm writes with group 0),
+ * or of a floating type; then the call brings each row to 8 bits first:
+ *   x_scale[m] = max |x[m]| / 127,  xq = the whole number nearest to
+ *   x * 127 / max |x[m]|, ties to even (exactly, not by a rounded quotient) */
+typedef struct aq_i8 aq_i8;
+
+/* Upload a matrix from host memory (once; it is laid out for the kernels on
+ * the device).  The call waits for the layout to be done.
+ *   w      [out_features, in_features], -128 to 127
+ *   scale  [out_features] F32
+ *   bias   [out_features] F32 or NULL
+ * out_features up to 2^24, in_features up to 2^17 - 1 (the sums are held in 32
+ * bits), 2^34 weights. */
+aq_status aq_i8_upload(aq_ctx *ctx, int64_t out_features, int64_t in_features, const int8_t *w, const float *scale,
+                       const float *bias, aq_i8 **out);
+
+/*   x        device [M, in_features], row stride x_ld (elements), x_type I8,
+ *            F32, F16 or BF16
+ *   x_scale  device [M] for I8; NULL for the others
+ *   y        device [M, out_features], row stride y_ld, y_type F32, F16 or BF16
+ * The sums are exact; the conversion to fp32, the scaling and the bias round.
+ * A floating row of zeros has scale 0; one with a value that is not finite
+ * gives a row of NaN.  A floating x, or one of more than 16 rows, is laid out
+ * in the context's scratch first. */
+aq_status aq_i8_forward(aq_ctx *ctx, const aq_i8 *w, int x_type, const void *x, int64_t x_ld, const float *x_scale,
+                        int64_t M, int y_type, void *y, int64_t y_ld);
+aq_status aq_i8_release(aq_i8 *w);
+
 /* One index per row of logits, drawn with a given random number:
  *   z[i] = (l[i] - max l) * log2(e) / temperature,  e[i] = 2^z[i]   (fp32)
  *   w[i] = floor(e[i] * 2^31): whole numbers, so no sum depends on an order

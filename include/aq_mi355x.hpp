@@ -319,6 +319,33 @@ private:
     aq_q4 *w_ = nullptr;
 };
 
+// A matrix with 8-bit whole-number weights and a scale a row (aq_i8).
+class I8Linear {
+public:
+    // Host pointers, see aq_i8_upload; bias may be null.
+    I8Linear(Context &ctx, int64_t out_features, int64_t in_features, const int8_t *w, const float *scale,
+             const float *bias = nullptr)
+        : ctx_(&ctx) {
+        ctx.check(aq_i8_upload(ctx.get(), out_features, in_features, w, scale, bias, &w_));
+    }
+    I8Linear(const I8Linear &) = delete;
+    I8Linear &operator=(const I8Linear &) = delete;
+    I8Linear(I8Linear &&o) noexcept : ctx_(o.ctx_), w_(std::exchange(o.w_, nullptr)) {}
+    ~I8Linear() {
+        if (w_) aq_i8_release(w_);
+    }
+
+    // Device pointers: y [M, out] = x [M, in] W^T + bias; x_scale [M] with an I8 x.
+    void forward(aq_dtype x_type, const void *x, int64_t x_ld, int64_t M, aq_dtype y_type, void *y, int64_t y_ld,
+                 const float *x_scale = nullptr) const {
+        ctx_->check(aq_i8_forward(ctx_->get(), w_, x_type, x, x_ld, x_scale, M, y_type, y, y_ld));
+    }
+
+private:
+    Context *ctx_;
+    aq_i8 *w_ = nullptr;
+};
+
 // What aq_sample draws with, per row (device pointers; null: off).
 struct SampleFilters {
     const float *temperature = nullptr;
