@@ -36,7 +36,16 @@ EXPORTED = [
     "aq_linear_upload", "aq_linear_forward", "aq_linear_release",
     "aq_add_rmsnorm", "aq_q4_upload", "aq_q4_forward", "aq_q4_release", "aq_sample",
     "aq_i8_upload", "aq_i8_forward", "aq_i8_release",
+    "aq_cross_attention", "aq_prefix_attention",
 ]
+
+
+
+class Heads(C.Structure):
+    """aq_heads"""
+
+    _fields_ = [("data", C.c_void_p), ("batch_ld", C.c_int64), ("row_ld", C.c_int64), ("head_ld", C.c_int64)]
+
 
 # aq_euclid_recipe / aq_codebook_type
 OMNIVOICE, HIGGS, DIRECT = 0, 1, 2
@@ -96,6 +105,8 @@ def load_library(path: str | pathlib.Path | None = None) -> C.CDLL:
     lib.aq_i8_upload.argtypes = [vp, i64, i64, vp, vp, vp, C.POINTER(vp)]
     lib.aq_i8_forward.argtypes = [vp, vp, C.c_int, vp, i64, vp, i64, C.c_int, vp, i64]
     lib.aq_i8_release.argtypes = [vp]
+    lib.aq_cross_attention.argtypes = [vp, C.c_int, *[i64] * 6, Heads, Heads, Heads, vp, vp, vp, i64, C.c_float, Heads]
+    lib.aq_prefix_attention.argtypes = [vp, C.c_int, *[i64] * 7, *[Heads] * 5, vp, vp, C.c_float, Heads]
     lib.aq_sample.argtypes = [vp, C.c_int, vp, i64, i64, i64, vp, vp, vp, vp, vp, vp, vp]
     lib.aq_euclid_decode.argtypes = [vp, vp, vp, i64, vp]
     lib.aq_euclid_encode_noalloc.argtypes = [vp, vp, vp, i64, vp, vp, vp, C.c_int, vp, vp, vp]
@@ -717,6 +728,55 @@ class I8Linear:
             self.close()
         except Exception:
             pass
+
+
+def _heads(t, shape, dtype: int) -> Heads:
+    """aq_heads of a device tensor [.., heads, D] whose last axis is adjacent."""
+    if not t.is_cuda or tuple(t.shape) != shape or (t.stride(-1) != 1 and shape[-1] > 1):
+        raise ValueError(f"expected a device tensor {shape} with adjacent elements, got {tuple(t.shape)} strides {t.stride()}")
+    if _dtype(t) != dtype:
+        raise TypeError(f"expected element type {dtype}, got {t.dtype}")
+    *batch, row, head = t.stride()[:-1]
+    return Heads(t.data_ptr(), batch[0] if batch else 0, row, head)
+
+
+def _lengths(t, B: int):
+    """Pointer of int32 lengths [B], or None."""
+    if t is not None and (str(t.dtype) != "torch.int32" or t.numel() != B):
+        raise ValueError(f"expected {B} int32 lengths, got {tuple(t.shape)} of {t.dtype}")
+    return _dptr(t)
+
+
+def cross_attention(ctx: Context, q, k, v, out, kv_len=None, q_len=None, mask=None, scale: float | None = None):
+    """aq_cross_attention on device tensors of one floating type: q, out [B, T,
+    heads, D], k, v [B, S, kv_heads, D] (any strides but the last axis's);
+    kv_len, q_len int32 [B]; mask bool or uint8 [B, S]; scale None: D ** -0.5."""
+    B, T, H, D = q.shape
+    S, Hkv = k.shape[1:3]
+    t = _dtype(q)
+    if mask is not None and (tuple(mask.shape) != (B, S) or mask.element_size() != 1 or not mask.is_cuda
+                             or (mask.stride(1) != 1 and S > 1)):
+        raise ValueError(f"mask must be bool or uint8 ({B}, {S}) with adjacent elements")
+    ctx.use_current_stream()
+    ctx.check(ctx.lib.aq_cross_attention(
+        ctx.h, t, B, T, S, H, Hkv, D, _heads(q, (B, T, H, D), t), _heads(k, (B, S, Hkv, D), t), _heads(v, (B, S, Hkv, D), t),
+        _lengths(q_len, B), _lengths(kv_len, B), None if mask is None else mask.data_ptr(),
+        0 if mask is None or B == 1 else mask.stride(0), D ** -0.5 if scale is None else scale, _heads(out, (B, T, H, D), t)))
+
+
+def prefix_attention(ctx: Context, q, prefix_k, prefix_v, k, v, out, kv_len=None, q_len=None, scale: float | None = None):
+    """aq_prefix_attention on device tensors of one floating type: q, out [B, T,
+    heads, D], prefix_k, prefix_v [P, kv_heads, D], k, v [B, S, kv_heads, D];
+    kv_len, q_len int32 [B]; scale None: D ** -0.5."""
+    B, T, H, D = q.shape
+    S, Hkv = k.shape[1:3]
+    P = prefix_k.shape[0]
+    t = _dtype(q)
+    ctx.use_current_stream()
+    ctx.check(ctx.lib.aq_prefix_attention(
+        ctx.h, t, B, T, P, S, H, Hkv, D, _heads(q, (B, T, H, D), t), _heads(prefix_k, (P, Hkv, D), t),
+        _heads(prefix_v, (P, Hkv, D), t), _heads(k, (B, S, Hkv, D), t), _heads(v, (B, S, Hkv, D), t), _lengths(q_len, B),
+        _lengths(kv_len, B), D ** -0.5 if scale is None else scale, _heads(out, (B, T, H, D), t)))
 
 
 def sample(ctx: Context, logits, u, token, temperature=None, top_k=None, top_p=None, min_p=None, logp=None):

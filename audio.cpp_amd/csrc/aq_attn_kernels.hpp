@@ -1,0 +1,585 @@
+// Attention to an encoder's states and over a shared prefix (aq_cross_attention,
+// aq_prefix_attention).
+//
+// A row r of a head's group of G query heads is (token, head of the group).
+// One pass over the keys with each row's running maximum m and weight l:
+//   s = q . k,  m' = max(m, c max s),  p = 2^(c s - m'),
+//   o = o 2^(m - m') + sum p v,  l = l 2^(m - m') + sum p,   out = o / l
+// with c = scale log2(e).
+//
+// Both products have the keys' side as the first operand, so that every lane
+// works for one row: S^T = K Q^T has a row per column, the lane's own, with 16
+// of a tile's 32 keys in its registers and the other 16 in lane ^ 32, and O^T =
+// V^T P^T takes p from those registers as they are: the order of the keys in
+// the second product is the one that the first leaves, and V is read from LDS
+// in that order, by the loads that transpose (16-bit types) or one value a
+// lane (fp32).  A row's m, l and rescaling are plain registers; one exchange
+// per tile joins the two halves' maxima.
+//
+// Scores, m, l and o are fp32.  p is rounded to the 16-bit type of v (half a
+// step of 2^-9, 2^-12 for f16, with errors of either sign that the sum over
+// the keys averages); an f16 p is 2^14 times the weight, so that small weights
+// are not lost below its range.  fp32 inputs keep fp32 products throughout.
+//
+// A key that a row does not see is never multiplied into it: its score is
+// -infinity whatever the product gave, keys that no row of the tile sees are
+// zeros in LDS, and where a causal tile holds values that are not finite, those
+// are added apart to the rows that see them (0 * infinity would be NaN).
+#pragma once
+#include "aq_attn.hpp"
+#include "aq_types.hpp"
+
+namespace aq_attn_impl {
+
+using namespace aq_types;
+
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef float f32x16 __attribute__((ext_vector_type(16)));
+typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef short s16x4 __attribute__((ext_vector_type(4)));
+typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+
+// A tile of KT keys by DP columns in LDS, rows of 16-byte pieces.  A piece's
+// place in its row is XORed with a number of the row's, so that the lanes that
+// read together meet different banks.
+template <typename T, int DP>
+struct shape {
+    static constexpr bool kF32 = sizeof(typename T::raw) == 4;
+    static constexpr int kPer = 16 / sizeof(typename T::raw);   // elements of a piece
+    static constexpr int kPieces = DP / kPer;                   // of a row
+    static constexpr int kRow = kPieces * 16;                   // bytes of a row
+    static __device__ inline int swz_k(int key) { return kRow >= 256 ? key & 15 : (key >> 1) & 7; }
+    static __device__ inline int swz_v(int key) {
+        if (kF32) return kRow >= 256 ? ((key >> 2) & 1) * 8 : 0;
+        return kRow >= 256 ? (key & 3) * 4 : ((key >> 1) & 1) * 4;
+    }
+};
+
+__device__ inline f32x16 mma(f16, u32x4 a, u32x4 b, f32x16 c) {
+    return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
+}
+__device__ inline f32x16 mma(bf16, u32x4 a, u32x4 b, f32x16 c) {
+    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+}
+__device__ inline f32x16 mma(f32, float a, float b, f32x16 c) { return __builtin_amdgcn_mfma_f32_32x32x2f32(a, b, c, 0, 0, 0); }
+
+__device__ inline bool odd_bits(f16, uint32_t v) { return (v & 0x7C00u) == 0x7C00u || (v & 0x7C000000u) == 0x7C000000u; }
+__device__ inline bool odd_bits(bf16, uint32_t v) { return (v & 0x7F80u) == 0x7F80u || (v & 0x7F800000u) == 0x7F800000u; }
+__device__ inline bool odd_bits(f32, uint32_t v) { return (v & 0x7F800000u) == 0x7F800000u; }
+// Each element of a word that is not finite replaced by zero.
+__device__ inline uint32_t finite_bits(f16, uint32_t v) {
+    return ((v & 0x7C00u) == 0x7C00u ? 0u : v & 0xFFFFu) | ((v & 0x7C000000u) == 0x7C000000u ? 0u : v & 0xFFFF0000u);
+}
+__device__ inline uint32_t finite_bits(bf16, uint32_t v) {
+    return ((v & 0x7F80u) == 0x7F80u ? 0u : v & 0xFFFFu) | ((v & 0x7F800000u) == 0x7F800000u ? 0u : v & 0xFFFF0000u);
+}
+__device__ inline uint32_t finite_bits(f32, uint32_t v) { return odd_bits(f32(), v) ? 0u : v; }
+
+// A piece of a row, elements at.. of D; zeros from D on, and where !use.
+template <typename T>
+__device__ inline u32x4 load_piece(const typename T::raw *row, int at, int D, bool use) {
+    typedef u32x4 any __attribute__((aligned(1)));
+    constexpr int kPer = 16 / sizeof(typename T::raw);
+    u32x4 r = {0, 0, 0, 0};
+    if (!use || at >= D) return r;
+    if (at + kPer <= D) return *reinterpret_cast<const any *>(row + at);
+#pragma unroll
+    for (int i = 0; i < kPer; ++i)
+        if (at + i < D) {
+            if (sizeof(typename T::raw) == 4) r[i] = bits_of(row[at + i]);
+            else r[i / 2] |= bits_of(row[at + i]) << (16 * (i % 2));
+        }
+    return r;
+}
+
+// The rows of one wave's 32 columns and what they have gathered.
+template <typename T, int DP>
+struct row_state {
+    using S = shape<T, DP>;
+    static constexpr int kQ = S::kF32 ? DP / 8 : DP / 16;   // pieces of q in a lane
+    u32x4 q[kQ];
+    f32x16 o[DP / 32];
+    float m, l;        // the row's; l holds the half's keys
+    int b, t, h;       // the lane's row
+    bool used;         // it exists
+    int see;           // own keys that it sees
+};
+
+template <typename T, int DP>
+__device__ inline void open_rows(const args &a, int b0, int r, int hk, row_state<T, DP> &w) {
+    using S = shape<T, DP>;
+    const int half = (threadIdx.x & 63) >> 5;
+    const int tok = r / a.G;
+    w.b = b0 + tok / a.T;
+    w.t = tok % a.T;
+    w.h = hk * a.G + r % a.G;
+    // (for a stream's own walk b0 is the stream, and rows past its T tokens are no rows)
+    w.used = w.b < a.B && (a.walk == kPrefix || tok < a.T);
+    int rows = a.T, keys = a.S;
+    if (w.used) {
+        if (a.q_len) rows = max(0, min(a.q_len[w.b], a.T));
+        if (a.kv_len) keys = max(0, min(a.kv_len[w.b], a.S));
+    }
+    w.used = w.used && w.t < rows;
+    w.see = !w.used ? 0 : a.causal ? max(0, keys - rows + w.t + 1) : keys;
+    const typename T::raw *row = static_cast<const typename T::raw *>(a.q);
+    if (w.used) row += w.b * a.sq.batch + w.t * a.sq.row + w.h * a.sq.head;
+#pragma unroll
+    for (int i = 0; i < row_state<T, DP>::kQ; ++i) w.q[i] = load_piece<T>(row, (2 * i + half) * S::kPer, a.D, w.used);
+#pragma unroll
+    for (int d = 0; d < DP / 32; ++d)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) w.o[d][i] = 0.0f;
+    w.m = -INFINITY;
+    w.l = 0.0f;
+}
+
+// One tile of 32 NT keys from LDS.  vis: bit j is set where this lane's row
+// sees key j of each 32; all: every lane sees every key.  odd: V may hold
+// values that are not finite in keys that some rows do not see.
+template <typename T, int DP, int NT>
+__device__ inline void add_tile(const unsigned char *lk, const unsigned char *lv, const uint32_t (&vis)[NT], bool all,
+                                bool odd, float c, row_state<T, DP> &w) {
+    using S = shape<T, DP>;
+    constexpr int kShift = std::is_same<T, f16>::value ? 14 : 0;   // p is 2^kShift times the weight
+    const int lane = threadIdx.x & 63, half = lane >> 5, col = lane & 31;
+    f32x16 s[NT];
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+#pragma unroll
+        for (int i = 0; i < 16; ++i) s[n][i] = 0.0f;
+        const int key = 32 * n + col;
+#pragma unroll
+        for (int i = 0; i < row_state<T, DP>::kQ; ++i) {
+            const u32x4 k = *reinterpret_cast<const u32x4 *>(lk + key * S::kRow + (((2 * i + half) ^ S::swz_k(key)) << 4));
+            if constexpr (S::kF32) {
+#pragma unroll
+                for (int j = 0; j < 4; ++j) s[n] = mma(f32(), __uint_as_float(k[j]), __uint_as_float(w.q[i][j]), s[n]);
+            } else {
+                s[n] = mma(T(), k, w.q[i], s[n]);
+            }
+        }
+    }
+    if (!all) {
+#pragma unroll
+        for (int n = 0; n < NT; ++n) {
+            const uint32_t v = vis[n] >> (4 * half);
+#pragma unroll
+            for (int i = 0; i < 16; ++i) s[n][i] = v >> (8 * (i >> 2) + (i & 3)) & 1u ? s[n][i] : -INFINITY;
+        }
+    }
+    float top = -INFINITY;
+#pragma unroll
+    for (int n = 0; n < NT; ++n)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) top = fmaxf(top, s[n][i]);
+    top = fmaxf(top, __shfl_xor(top, 32));
+    const float m = fmaxf(w.m, top * c);
+    const float from = (m == -INFINITY ? 0.0f : m) - kShift;
+    const float keep = __builtin_amdgcn_exp2f(w.m - (from + kShift));
+    w.m = m;
+    float sum = 0.0f;
+#pragma unroll
+    for (int n = 0; n < NT; ++n)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+            s[n][i] = __builtin_amdgcn_exp2f(__fmaf_rn(s[n][i], c, -from));
+            sum += s[n][i];
+        }
+    w.l = __fmaf_rn(w.l, keep, sum);
+#pragma unroll
+    for (int d = 0; d < DP / 32; ++d) w.o[d] *= keep;
+
+    if constexpr (S::kF32) {
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+                const int key = 32 * n + 8 * (i >> 2) + (i & 3) + 4 * half;
+#pragma unroll
+                for (int d = 0; d < DP / 32; ++d) {
+                    const int at = 32 * d + col;
+                    uint32_t v = *reinterpret_cast<const uint32_t *>(lv + key * S::kRow + (((at >> 2) ^ S::swz_v(key)) << 4) +
+                                                                     (at & 3) * 4);
+                    if (odd) v = finite_bits(T(), v);
+                    w.o[d] = mma(f32(), __uint_as_float(v), s[n][i], w.o[d]);
+                }
+            }
+    } else {
+        const int sub = (lane >> 2) & 3;   // of the four keys that 16 lanes load for each other
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+            for (int g = 0; g < 2; ++g) {
+                typename T::raw p[8];
+#pragma unroll
+                for (int i = 0; i < 8; i += 2) T::store2(p + i, s[n][8 * g + i], s[n][8 * g + i + 1]);
+                u32x4 pf;
+                std::memcpy(&pf, p, 16);
+                const int key = 32 * n + 16 * g + 4 * half + sub;
+#pragma unroll
+                for (int d = 0; d < DP / 32; ++d) {
+                    const int piece = 4 * d + 2 * ((lane >> 4) & 1) + ((lane >> 1) & 1);
+                    const unsigned char *at = lv + key * S::kRow + ((piece ^ S::swz_v(key)) << 4) + (lane & 1) * 8;
+                    typedef __attribute__((address_space(3))) s16x4 *lds4;
+                    const u32x2 lo = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4)at));
+                    const u32x2 hi = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4)(at + 8 * S::kRow)));
+                    u32x4 v = {lo[0], lo[1], hi[0], hi[1]};
+                    if (odd) {
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) v[i] = finite_bits(T(), v[i]);
+                    }
+                    w.o[d] = mma(T(), v, pf, w.o[d]);
+                }
+            }
+    }
+    if (odd) {   // the values left out, key by key
+#pragma unroll 1
+        for (int key = 0; key < 32 * NT; ++key) {
+            float p = 0.0f;
+            uint32_t sees = 0;
+#pragma unroll
+            for (int n = 0; n < NT; ++n) {
+                if (key >> 5 == n) sees = all ? 1u : vis[n] >> (key & 31) & 1u;
+#pragma unroll
+                for (int i = 0; i < 16; ++i)
+                    if (32 * n + 8 * (i >> 2) + (i & 3) + 4 * half == key) p = s[n][i];
+            }
+            p += __shfl_xor(p, 32);   // (the other half's is 0, or this one's)
+#pragma unroll
+            for (int d = 0; d < DP / 32; ++d)
+#pragma unroll
+                for (int i = 0; i < 16; ++i) {
+                    const int at = 32 * d + 8 * (i >> 2) + 4 * half + (i & 3);
+                    const auto v = *reinterpret_cast<const typename T::raw *>(
+                        lv + key * S::kRow + ((at / S::kPer ^ S::swz_v(key)) << 4) + at % S::kPer * sizeof(typename T::raw));
+                    if (sees && odd_bits(T(), bits_of(v))) w.o[d][i] = __fmaf_rn(p, T::load(v), w.o[d][i]);
+                }
+        }
+    }
+}
+
+// The keys that a walk meets one after the other: the prefix's tiles, then the
+// stream's own.  Everything here is the same for all lanes that share a tile.
+template <typename T>
+struct key_walk {
+    const typename T::raw *pk, *pv, *k, *v;
+    const uint8_t *mask;
+    int prefix_tiles, P, keys, own;   // keys: of the stream (for the staging); own: that the rows can see
+    int64_t pk_row, pv_row, k_row, v_row;
+};
+
+template <typename T, int KT>
+__device__ inline int open_walk(const args &a, int b, int hk, int most, key_walk<T> &w) {
+    using E = typename T::raw;
+    w.P = a.walk & kPrefix ? a.P : 0;
+    w.prefix_tiles = (w.P + KT - 1) / KT;
+    w.own = a.walk & kOwn ? most : 0;
+    w.pk = static_cast<const E *>(a.pk) + hk * a.spk.head;
+    w.pv = static_cast<const E *>(a.pv) + hk * a.spv.head;
+    w.k = static_cast<const E *>(a.k) + b * a.sk.batch + hk * a.sk.head;
+    w.v = static_cast<const E *>(a.v) + b * a.sv.batch + hk * a.sv.head;
+    w.pk_row = a.spk.row;
+    w.pv_row = a.spv.row;
+    w.k_row = a.sk.row;
+    w.v_row = a.sv.row;
+    w.mask = a.mask ? a.mask + b * a.mask_ld : nullptr;
+    return w.prefix_tiles + (w.own + KT - 1) / KT;
+}
+
+// Sixteen bytes of zeros, for the pieces past D and the keys that no row sees.
+static __device__ const u32x4 kZeros = {0, 0, 0, 0};
+
+// Brings a tile's K and V to LDS.  DIRECT (rows that start and end at 16
+// bytes): straight from memory, still on their way when load() returns; each
+// wave's 64 pieces land next to each other, so the piece of a place is the one
+// that the swizzle puts there.  Otherwise through registers.
+template <typename T, int DP, int KT, int THREADS, bool DIRECT>
+struct stager {
+    using S = shape<T, DP>;
+    using E = typename T::raw;
+    static constexpr int kEach = KT * S::kPieces / THREADS;
+
+    static __device__ inline void piece(const E *from, unsigned char *to) {
+        __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void *)from,
+                                         (__attribute__((address_space(3))) void *)to, 16, 0, 0);
+    }
+
+    // The keys of the tile that any row may see come back as bits.
+    static __device__ inline uint64_t load(const args &a, const key_walk<T> &w, int tile, unsigned char *lk, unsigned char *lv,
+                                           int thread) {
+        const bool pre = tile < w.prefix_tiles;
+        const int j0 = (pre ? tile : tile - w.prefix_tiles) * KT, n = (pre ? w.P : w.own) - j0;
+        uint64_t bits = n >= 64 ? ~uint64_t{0} : (uint64_t{1} << n) - 1;
+        const int lane = threadIdx.x & 63;
+        if (!pre && w.mask) bits &= __ballot(lane < n && w.mask[j0 + min(lane, n - 1)] != 0);
+        const int64_t kr = pre ? w.pk_row : w.k_row, vr = pre ? w.pv_row : w.v_row;
+        const E *kp = (pre ? w.pk : w.k) + j0 * kr, *vp = (pre ? w.pv : w.v) + j0 * vr;
+        if constexpr (DIRECT) {
+            unsigned char *const k0 = lk + (thread - lane) * 16, *const v0 = lv + (thread - lane) * 16;
+            constexpr uint64_t kAll = KT == 64 ? ~uint64_t{0} : (uint64_t{1} << (KT % 64)) - 1;
+            const bool whole = (bits & kAll) == kAll && a.D == DP;
+#pragma unroll
+            for (int i = 0; i < kEach; ++i) {
+                const int at = i * THREADS + thread, key = at / S::kPieces, place = at % S::kPieces;
+                const int pk = (place ^ S::swz_k(key)) * S::kPer, pv = (place ^ S::swz_v(key)) * S::kPer;
+                const E *kg = kp + key * kr + pk, *vg = vp + key * vr + pv;
+                if (!whole) {
+                    const E *const none = reinterpret_cast<const E *>(&kZeros);
+                    if (!(bits >> key & 1) || pk >= a.D) kg = none;
+                    if (!(bits >> key & 1) || pv >= a.D) vg = none;
+                }
+                piece(kg, k0 + i * THREADS * 16);
+                piece(vg, v0 + i * THREADS * 16);
+            }
+        } else {
+#pragma unroll 4
+            for (int i = 0; i < kEach; ++i) {
+                const int at = i * THREADS + thread, key = at / S::kPieces, piece = at % S::kPieces;
+                const bool use = bits >> key & 1;
+                const u32x4 k = load_piece<T>(kp + key * kr, piece * S::kPer, a.D, use);
+                const u32x4 v = load_piece<T>(vp + key * vr, piece * S::kPer, a.D, use);
+                *reinterpret_cast<u32x4 *>(lk + key * S::kRow + ((piece ^ S::swz_k(key)) << 4)) = k;
+                *reinterpret_cast<u32x4 *>(lv + key * S::kRow + ((piece ^ S::swz_v(key)) << 4)) = v;
+            }
+        }
+        return bits;
+    }
+};
+
+// What this wave sent to LDS has landed, and what it read from there has come.
+__device__ inline void landed() { __builtin_amdgcn_s_waitcnt(0x0070); }   // vmcnt(0) lgkmcnt(0)
+
+// Whether V's tile holds a value that is not finite, for the wave.
+template <typename T, int DP, int KT>
+__device__ inline bool any_odd(const unsigned char *lv) {
+    using S = shape<T, DP>;
+    bool odd = false;
+    for (int i = threadIdx.x & 63; i < KT * S::kPieces; i += 64) {
+        const u32x4 v = reinterpret_cast<const u32x4 *>(lv)[i];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) odd = odd || odd_bits(T(), v[j]);
+    }
+    return __ballot(odd) != 0;
+}
+
+// A staged tile for this wave's rows.
+template <typename T, int DP, int NT>
+__device__ inline void take_tile(const args &a, const key_walk<T> &walk, int tile, uint64_t bits, const unsigned char *lk,
+                                 const unsigned char *lv, row_state<T, DP> &w) {
+    constexpr int KT = 32 * NT;
+    const bool pre = tile < walk.prefix_tiles;
+    uint32_t vis[NT];
+    bool mine = true;
+    // Keys of the tile that the row sees, masks apart.  (A column without a row may see any.)
+    const int n = pre || !w.used ? KT : w.see - (tile - walk.prefix_tiles) * KT;
+#pragma unroll
+    for (int i = 0; i < NT; ++i) {
+        const int c = min(max(n - 32 * i, 0), 32);
+        vis[i] = (c == 32 ? ~0u : (1u << c) - 1u) & static_cast<uint32_t>(bits >> (32 * i));
+        mine = mine && vis[i] == ~0u;
+    }
+    const bool all = __ballot(mine) == ~uint64_t{0};
+    // Causal rows share a tile that not all of them see: V needs a look.
+    bool odd = false;
+    if (!all && a.causal && !pre) odd = any_odd<T, DP, KT>(lv);
+    add_tile<T, DP, NT>(lk, lv, vis, all, odd, a.c, w);
+}
+
+// The row's result, or its part of one.  l is whole here.
+template <typename T, int DP>
+__device__ inline void close_rows(const args &a, int part, const row_state<T, DP> &w) {
+    if (!w.used) return;
+    const int half = (threadIdx.x & 63) >> 5;
+    if (a.sums) {
+        const int64_t row = (static_cast<int64_t>(part) * a.rows) + (static_cast<int64_t>(w.b) * a.T + w.t) * a.H + w.h;
+        float *to = a.sums + row * a.D;
+#pragma unroll
+        for (int d = 0; d < DP / 32; ++d)
+#pragma unroll
+            for (int g = 0; g < 4; ++g) {
+                const int at = 32 * d + 8 * g + 4 * half;
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+                    if (at + i < a.D) to[at + i] = w.o[d][4 * g + i];
+            }
+        if (half == 0) {
+            a.ml[row * 2] = w.m;
+            a.ml[row * 2 + 1] = w.l;
+        }
+        return;
+    }
+    const float by = w.l == 0.0f ? 0.0f : 1.0f / w.l;   // no key at all: 0
+    typename T::raw *to = static_cast<typename T::raw *>(a.out) + w.b * a.so.batch + w.t * a.so.row + w.h * a.so.head;
+#pragma unroll
+    for (int d = 0; d < DP / 32; ++d)
+#pragma unroll
+        for (int g = 0; g < 4; ++g) {
+            const int at = 32 * d + 8 * g + 4 * half;
+            typename T::raw r[4];
+#pragma unroll
+            for (int i = 0; i < 4; i += 2) T::store2(r + i, w.o[d][4 * g + i] * by, w.o[d][4 * g + i + 1] * by);
+            if (at + 4 <= a.D) std::memcpy(to + at, r, sizeof(r));
+            else
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+                    if (at + i < a.D) to[at + i] = r[i];
+        }
+}
+
+// The most own keys that any row of the block (or wave) sees.
+__device__ inline int most_of(int see) {
+#pragma unroll
+    for (int d = 32; d; d >>= 1) see = max(see, __shfl_xor(see, d));
+    return see;
+}
+
+// Many rows: 32 a wave, 128 a block, which brings each tile to LDS once, into
+// one of two places while the other is used.
+template <typename T, int DP, int NT, bool DIRECT>
+__global__ __launch_bounds__(256) void attn_rows_kernel(args a) {
+    using S = shape<T, DP>;
+    constexpr int KT = 32 * NT, kTile = KT * S::kRow;
+    using stage = stager<T, DP, KT, 256, DIRECT>;
+    extern __shared__ __align__(16) unsigned char lds[];   // [2][K, V]
+    __shared__ int see[4];
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
+    int at = blockIdx.x;
+    const int split = at % a.splits;
+    at /= a.splits;
+    const int rt = at % a.tiles;
+    at /= a.tiles;
+    const int hk = at % a.Hkv, b = at / a.Hkv;   // b: 0 for the prefix alone
+    row_state<T, DP> w;
+    open_rows(a, b, rt * 128 + wave * 32 + (lane & 31), hk, w);
+    const int mine = most_of(w.see);
+    if (lane == 0) see[wave] = mine;
+    if (__syncthreads_or(w.used) == 0) return;
+    key_walk<T> walk;
+    const int most = __builtin_amdgcn_readfirstlane(max(max(see[0], see[1]), max(see[2], see[3])));
+    const int tiles = open_walk<T, KT>(a, b, hk, most, walk);
+    const int per = (tiles + a.splits - 1) / a.splits, first = split * per, end = min(tiles, first + per);
+    uint64_t bits = 0;
+    if (first < end) bits = stage::load(a, walk, first, lds, lds + kTile, threadIdx.x);
+#pragma unroll 1
+    for (int tile = first; tile < end; ++tile) {
+        unsigned char *const now = lds + ((tile - first) & 1) * 2 * kTile, *const then = lds + ((tile - first + 1) & 1) * 2 * kTile;
+        landed();
+        __syncthreads();   // the tile is there, and all waves are done with the one before
+        const uint64_t use = bits;
+        if (tile + 1 < end) bits = stage::load(a, walk, tile + 1, then, then + kTile, threadIdx.x);
+        take_tile<T, DP, NT>(a, walk, tile, use, now, now + kTile, w);
+    }
+    w.l += __shfl_xor(w.l, 32);
+    close_rows(a, a.part + split, w);
+}
+
+// Few rows: 32 a block; each of its waves takes every WAVES-th tile, with LDS
+// of its own, and the waves' sums are joined in LDS, in the waves' order.
+template <typename T, int DP, int WAVES, bool DIRECT>
+__global__ __launch_bounds__(64 * WAVES) void attn_keys_kernel(args a) {
+    using S = shape<T, DP>;
+    constexpr int KT = 32, kTile = KT * S::kRow;
+    using stage = stager<T, DP, KT, 64, DIRECT>;
+    extern __shared__ __align__(16) unsigned char lds[];   // [waves][2][K, V]
+    __shared__ float ml[WAVES][2][32];
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
+    unsigned char *const own = lds + wave * 4 * kTile;
+    int at = blockIdx.x;
+    const int split = at % a.splits;
+    at /= a.splits;
+    const int rt = at % a.tiles;
+    at /= a.tiles;
+    const int hk = at % a.Hkv, b = at / a.Hkv;
+    row_state<T, DP> w;
+    open_rows(a, b, rt * 32 + (lane & 31), hk, w);
+    if (__ballot(w.used) == 0) return;   // the same for all waves
+    key_walk<T> walk;
+    const int tiles = open_walk<T, KT>(a, b, hk, __builtin_amdgcn_readfirstlane(most_of(w.see)), walk);
+    const int per = (tiles + a.splits - 1) / a.splits, first = split * per, end = min(tiles, first + per);
+    uint64_t bits = 0;
+    if (first + wave < end) bits = stage::load(a, walk, first + wave, own, own + kTile, lane);
+    int turn = 0;
+#pragma unroll 1
+    for (int tile = first + wave; tile < end; tile += WAVES, turn ^= 1) {
+        unsigned char *const now = own + turn * 2 * kTile, *const then = own + (turn ^ 1) * 2 * kTile;
+        landed();
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        const uint64_t use = bits;
+        if (tile + WAVES < end) bits = stage::load(a, walk, tile + WAVES, then, then + kTile, lane);
+        take_tile<T, DP, 1>(a, walk, tile, use, now, now + kTile, w);
+    }
+    w.l += __shfl_xor(w.l, 32);
+    if constexpr (WAVES > 1) {
+        if (lane < 32) {
+            ml[wave][0][lane] = w.m;
+            ml[wave][1][lane] = w.l;
+        }
+        __syncthreads();   // (the tiles are not used any more either)
+        float m = -INFINITY, l = 0.0f;
+#pragma unroll
+        for (int i = 0; i < WAVES; ++i) m = fmaxf(m, ml[i][0][lane & 31]);
+        const float from = m == -INFINITY ? 0.0f : m;
+#pragma unroll
+        for (int i = 0; i < WAVES; ++i) l = __fmaf_rn(ml[i][1][lane & 31], __builtin_amdgcn_exp2f(ml[i][0][lane & 31] - from), l);
+        const float keep = __builtin_amdgcn_exp2f(w.m - from);
+        f32x16 *const red = reinterpret_cast<f32x16 *>(lds);   // [WAVES][DP / 32][64]
+#pragma unroll
+        for (int d = 0; d < DP / 32; ++d) red[(wave * (DP / 32) + d) * 64 + lane] = w.o[d] * keep;
+        __syncthreads();
+        if (wave != 0) return;
+#pragma unroll
+        for (int d = 0; d < DP / 32; ++d) {
+            w.o[d] = red[d * 64 + lane];
+#pragma unroll
+            for (int i = 1; i < WAVES; ++i) w.o[d] += red[(i * (DP / 32) + d) * 64 + lane];
+        }
+        w.m = m;
+        w.l = l;
+    }
+    close_rows(a, a.part + split, w);
+}
+
+template <typename K>
+aq_status run(aq_ctx *ctx, const args &a, K kernel, int threads, uint32_t lds) {
+    aq_status st = aq_launch_lds(ctx, reinterpret_cast<const void *>(kernel), lds, "attention");
+    if (st != AQ_OK) return st;
+    const int64_t grid = static_cast<int64_t>(a.walk == kPrefix ? 1 : a.B) * a.Hkv * a.tiles * a.splits;
+    aq_launch_timed(ctx, true, kernel, dim3(static_cast<uint32_t>(grid)), dim3(static_cast<uint32_t>(threads)), lds, a);
+    AQ_HIP(ctx, hipGetLastError());
+    return AQ_OK;
+}
+
+template <typename T, int DP, int NT>
+aq_status run_rows(aq_ctx *ctx, const args &a) {
+    constexpr uint32_t kLds = 4 * 32 * NT * shape<T, DP>::kRow;
+    if (a.direct) return run(ctx, a, attn_rows_kernel<T, DP, NT, true>, 256, kLds);
+    return run(ctx, a, attn_rows_kernel<T, DP, NT, false>, 256, kLds);
+}
+
+template <typename T, int DP, int WAVES>
+aq_status run_keys(aq_ctx *ctx, const args &a) {
+    constexpr uint32_t kLds = WAVES * 4 * 32 * shape<T, DP>::kRow;   // the waves' sums, 32 rows of DP floats each, fit
+    if (a.direct) return run(ctx, a, attn_keys_kernel<T, DP, WAVES, true>, 64 * WAVES, kLds);
+    return run(ctx, a, attn_keys_kernel<T, DP, WAVES, false>, 64 * WAVES, kLds);
+}
+
+template <typename T>
+aq_status launch_rows(aq_ctx *ctx, const args &a) {
+    constexpr int kNT = sizeof(typename T::raw) == 4 ? 1 : 2;
+    if (a.D <= 64) return run_rows<T, 64, kNT>(ctx, a);
+    if (a.D <= 128) return run_rows<T, 128, kNT>(ctx, a);
+    return run_rows<T, 256, 1>(ctx, a);
+}
+
+template <typename T>
+aq_status launch_keys(aq_ctx *ctx, const args &a) {
+    constexpr int kWide = sizeof(typename T::raw) == 4 ? 2 : 1;
+    if (a.D <= 64) return run_keys<T, 64, 4>(ctx, a);
+    if (a.D <= 128) return run_keys<T, 128, 4 / kWide>(ctx, a);
+    return run_keys<T, 256, 2 / kWide>(ctx, a);
+}
+
+}  // namespace aq_attn_impl

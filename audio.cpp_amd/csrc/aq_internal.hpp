@@ -23,10 +23,10 @@ struct aq_ctx {
     // 3: refine-pass keys, 4: sweep keys and frame norms, 5: gathered
     // strided input rows of a DAC encode, 6: exact values of the frames an
     // exact scan takes, 7: largest logits and candidates of sampled rows,
-    // 8: rows of x in operand order).
-    static constexpr int kScratchSlots = 9;
-    // Slots from here on (tens of MB at most, but for rows of millions of
-    // columns) at least double when they grow, where the memory is there, and
+    // 8: rows of x in operand order, 9: an attention's parts).
+    static constexpr int kScratchSlots = 10;
+    // Slots from here on (tens of MB, for an attention's parts up to 256, and
+    // more for rows of millions of columns) at least double when they grow, where the memory is there, and
     // leave the buffers that they outgrow allocated until the context ends: a
     // captured graph of a call goes on using its own.
     static constexpr int kFirstKept = 7;

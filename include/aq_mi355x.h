@@ -587,6 +587,54 @@ aq_status aq_i8_forward(aq_ctx *ctx, const aq_i8 *w, int x_type, const void *x, 
                         int64_t M, int y_type, void *y, int64_t y_ld);
 aq_status aq_i8_release(aq_i8 *w);
 
+/* Rows of D adjacent elements by stream, token and head: that of (b, t, h)
+ * starts at data + b * batch_ld + t * row_ld + h * head_ld (elements, none
+ * negative; an input's may be 0).  No alignment beyond the type's is needed;
+ * rows of keys and values that start and end at 16 bytes are read faster. */
+typedef struct aq_heads {
+    void *data;
+    int64_t batch_ld, row_ld, head_ld;
+} aq_heads;
+
+/* Attention of B streams' rows to the states of an encoder:
+ *   out[b, t, h] = sum_j p[j] v[b, j, g] / sum_j p[j],  p[j] = exp(scale * q[b, t, h] . k[b, j, g]),
+ * over the keys j < kv_len[b] with mask[b, j] != 0, where g = h / (heads /
+ * kv_heads).  What lies in keys that are left out does not matter, NaN
+ * included.  A row without a key (or whose scores are all -infinity) is 0.
+ *   type     F32, F16 or BF16: q, k, v and out
+ *   q, out   device, [B, T, heads, D]; rows of out must not overlap.  out may
+ *            be q with the same strides, and else none of the inputs.
+ *   k, v     device, [B, S, kv_heads, D] (a batch_ld of 0: one encoder's
+ *            states for all streams); heads is a multiple of kv_heads
+ *   q_len    device [B] or NULL (T): rows of a stream; those from q_len on are
+ *            not written
+ *   kv_len   device [B] or NULL (S); lengths outside 0 to T and S count as the
+ *            nearest inside
+ *   mask     device, [B, S] bytes with row stride mask_ld (0: one for all
+ *            streams), or NULL
+ *   scale    above 0
+ * D from 1 to 256, S up to 2^30, B * T * heads up to 2^30.  Scores, sums and
+ * weights are fp32; with 16-bit types each p is rounded to the type before it
+ * meets v, an F32 call is fp32 throughout.  The order of a row's sum depends
+ * on the sizes alone, not on timing.  Calls of few rows use the context's
+ * scratch. */
+aq_status aq_cross_attention(aq_ctx *ctx, int type, int64_t B, int64_t T, int64_t S, int64_t heads, int64_t kv_heads, int64_t D,
+                             aq_heads q, aq_heads k, aq_heads v, const int32_t *q_len, const int32_t *kv_len,
+                             const uint8_t *mask, int64_t mask_ld, float scale, aq_heads out);
+
+/* Causal attention of B streams that share a prefix of P keys (the same
+ * formula): row t of stream b, with n = q_len[b] rows and m = kv_len[b] own
+ * keys, sees all of the prefix and its own keys j <= m - n + t; the last n own
+ * keys are the rows' own.  The prefix is read for all streams together.
+ *   prefix_k, prefix_v  device, [P, kv_heads, D] (batch_ld is not looked at)
+ *   k, v                device, [B, S, kv_heads, D]: the streams' own keys, of
+ *                       which kv_len[b] are in use (NULL: S)
+ * The rest, and the limits, are as above; P up to 2^30.  P = 0 is causal
+ * attention with a cache. */
+aq_status aq_prefix_attention(aq_ctx *ctx, int type, int64_t B, int64_t T, int64_t P, int64_t S, int64_t heads, int64_t kv_heads,
+                              int64_t D, aq_heads q, aq_heads prefix_k, aq_heads prefix_v, aq_heads k, aq_heads v,
+                              const int32_t *q_len, const int32_t *kv_len, float scale, aq_heads out);
+
 /* One index per row of logits, drawn with a given random number:
  *   z[i] = (l[i] - max l) * log2(e) / temperature,  e[i] = 2^z[i]   (fp32)
  *   w[i] = floor(e[i] * 2^31): whole numbers, so no sum depends on an order

@@ -346,6 +346,34 @@ private:
     aq_i8 *w_ = nullptr;
 };
 
+// Sizes of an attention: streams, rows of each, keys of each, heads and their width.
+struct AttentionShape {
+    int64_t B = 1, T = 1, S = 0, heads = 1, kv_heads = 1, D = 64;
+};
+
+// Which rows and keys count (device pointers; null: all).
+struct AttentionLengths {
+    const int32_t *q_len = nullptr;
+    const int32_t *kv_len = nullptr;
+    const uint8_t *mask = nullptr;   // of cross_attention, [B, S] with row stride mask_ld
+    int64_t mask_ld = 0;
+};
+
+// Rows of streams over an encoder's states, see aq_cross_attention.
+inline void cross_attention(Context &ctx, aq_dtype type, const AttentionShape &s, aq_heads q, aq_heads k, aq_heads v,
+                            aq_heads out, float scale, const AttentionLengths &n = {}) {
+    ctx.check(aq_cross_attention(ctx.get(), type, s.B, s.T, s.S, s.heads, s.kv_heads, s.D, q, k, v, n.q_len, n.kv_len, n.mask,
+                                 n.mask_ld, scale, out));
+}
+
+// Rows of streams over P keys that they share and their own, see aq_prefix_attention.
+inline void prefix_attention(Context &ctx, aq_dtype type, const AttentionShape &s, int64_t P, aq_heads q, aq_heads prefix_k,
+                             aq_heads prefix_v, aq_heads k, aq_heads v, aq_heads out, float scale,
+                             const AttentionLengths &n = {}) {
+    ctx.check(aq_prefix_attention(ctx.get(), type, s.B, s.T, P, s.S, s.heads, s.kv_heads, s.D, q, prefix_k, prefix_v, k, v,
+                                  n.q_len, n.kv_len, scale, out));
+}
+
 // What aq_sample draws with, per row (device pointers; null: off).
 struct SampleFilters {
     const float *temperature = nullptr;
