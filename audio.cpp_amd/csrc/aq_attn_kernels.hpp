@@ -5,7 +5,8 @@
 // One pass over the keys with each row's running maximum m and weight l:
 //   s = q . k,  m' = max(m, c max s),  p = 2^(c s - m'),
 //   o = o 2^(m - m') + sum p v,  l = l 2^(m - m') + sum p,   out = o / l
-// with c = scale log2(e).
+// with c = scale log2(e).  m' stays m while it would grow by no more than 5:
+// a p of up to 32 is as good as one of up to 1, and most tiles rescale nothing.
 //
 // Both products have the keys' side as the first operand, so that every lane
 // works for one row: S^T = K Q^T has a row per column, the lane's own, with 16
@@ -18,16 +19,20 @@
 //
 // Scores, m, l and o are fp32.  p is rounded to the 16-bit type of v (half a
 // step of 2^-9, 2^-12 for f16, with errors of either sign that the sum over
-// the keys averages); an f16 p is 2^14 times the weight, so that small weights
+// the keys averages); an f16 p is 2^10 times the weight, so that small weights
 // are not lost below its range.  fp32 inputs keep fp32 products throughout.
 //
 // A key that a row does not see is never multiplied into it: its score is
 // -infinity whatever the product gave, keys that no row of the tile sees are
-// zeros in LDS, and where a causal tile holds values that are not finite, those
-// are added apart to the rows that see them (0 * infinity would be NaN).
+// zeros in LDS, and where a causal tile that some rows see in part holds values
+// that are not finite, those are kept out of the products (0 * infinity is
+// NaN) and reach the rows that see them at the end.
 #pragma once
 #include "aq_attn.hpp"
 #include "aq_types.hpp"
+
+#include <climits>
+#include <type_traits>
 
 namespace aq_attn_impl {
 
@@ -65,17 +70,13 @@ __device__ inline f32x16 mma(bf16, u32x4 a, u32x4 b, f32x16 c) {
 }
 __device__ inline f32x16 mma(f32, float a, float b, f32x16 c) { return __builtin_amdgcn_mfma_f32_32x32x2f32(a, b, c, 0, 0, 0); }
 
-__device__ inline bool odd_bits(f16, uint32_t v) { return (v & 0x7C00u) == 0x7C00u || (v & 0x7C000000u) == 0x7C000000u; }
-__device__ inline bool odd_bits(bf16, uint32_t v) { return (v & 0x7F80u) == 0x7F80u || (v & 0x7F800000u) == 0x7F800000u; }
-__device__ inline bool odd_bits(f32, uint32_t v) { return (v & 0x7F800000u) == 0x7F800000u; }
 // Each element of a word that is not finite replaced by zero.
-__device__ inline uint32_t finite_bits(f16, uint32_t v) {
-    return ((v & 0x7C00u) == 0x7C00u ? 0u : v & 0xFFFFu) | ((v & 0x7C000000u) == 0x7C000000u ? 0u : v & 0xFFFF0000u);
+template <typename T>
+__device__ inline uint32_t finite_bits(uint32_t v) {
+    if (std::is_same<T, f32>::value) return (v & 0x7F800000u) == 0x7F800000u ? 0u : v;
+    constexpr uint32_t kLow = std::is_same<T, f16>::value ? 0x7C00u : 0x7F80u, kHigh = kLow << 16;
+    return ((v & kLow) == kLow ? 0u : v & 0xFFFFu) | ((v & kHigh) == kHigh ? 0u : v & 0xFFFF0000u);
 }
-__device__ inline uint32_t finite_bits(bf16, uint32_t v) {
-    return ((v & 0x7F80u) == 0x7F80u ? 0u : v & 0xFFFFu) | ((v & 0x7F800000u) == 0x7F800000u ? 0u : v & 0xFFFF0000u);
-}
-__device__ inline uint32_t finite_bits(f32, uint32_t v) { return odd_bits(f32(), v) ? 0u : v; }
 
 // A piece of a row, elements at.. of D; zeros from D on, and where !use.
 template <typename T>
@@ -93,6 +94,9 @@ __device__ inline u32x4 load_piece(const typename T::raw *row, int at, int D, bo
         }
     return r;
 }
+
+// Sixteen bytes of zeros, for the pieces past D and the keys that no row sees.
+static __device__ const u32x4 kZeros = {0, 0, 0, 0};
 
 // The rows of one wave's 32 columns and what they have gathered.
 template <typename T, int DP>
@@ -126,8 +130,19 @@ __device__ inline void open_rows(const args &a, int b0, int r, int hk, row_state
     w.see = !w.used ? 0 : a.causal ? max(0, keys - rows + w.t + 1) : keys;
     const typename T::raw *row = static_cast<const typename T::raw *>(a.q);
     if (w.used) row += w.b * a.sq.batch + w.t * a.sq.row + w.h * a.sq.head;
+    if (a.D % S::kPer == 0) {   // whole pieces: one load each, and all on their way together
 #pragma unroll
-    for (int i = 0; i < row_state<T, DP>::kQ; ++i) w.q[i] = load_piece<T>(row, (2 * i + half) * S::kPer, a.D, w.used);
+        for (int i = 0; i < row_state<T, DP>::kQ; ++i) {
+            typedef u32x4 any __attribute__((aligned(1)));
+            const int at = (2 * i + half) * S::kPer;
+            const bool use = w.used && at < a.D;
+            const u32x4 v = *reinterpret_cast<const any *>(use ? row + at : reinterpret_cast<const typename T::raw *>(&kZeros));
+            w.q[i] = v;
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < row_state<T, DP>::kQ; ++i) w.q[i] = load_piece<T>(row, (2 * i + half) * S::kPer, a.D, w.used);
+    }
 #pragma unroll
     for (int d = 0; d < DP / 32; ++d)
 #pragma unroll
@@ -136,14 +151,59 @@ __device__ inline void open_rows(const args &a, int b0, int r, int hk, row_state
     w.l = 0.0f;
 }
 
+// o += P V for a tile, p in s.
+template <typename T, int DP, int NT>
+__device__ inline void add_values(const unsigned char *lv, const f32x16 (&s)[NT], row_state<T, DP> &w) {
+    using S = shape<T, DP>;
+    const int lane = threadIdx.x & 63, half = lane >> 5, col = lane & 31;
+    if constexpr (S::kF32) {
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+                const int key = 32 * n + 8 * (i >> 2) + (i & 3) + 4 * half;   // this half's
+#pragma unroll
+                for (int d = 0; d < DP / 32; ++d) {
+                    const int at = 32 * d + col;
+                    const uint32_t v = *reinterpret_cast<const uint32_t *>(lv + key * S::kRow + (((at >> 2) ^ S::swz_v(key)) << 4) +
+                                                                           (at & 3) * 4);
+                    w.o[d] = mma(f32(), __uint_as_float(v), s[n][i], w.o[d]);
+                }
+            }
+    } else {
+        const int sub = (lane >> 2) & 3;   // of the four keys that 16 lanes load for each other
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+            for (int g = 0; g < 2; ++g) {
+                typename T::raw p[8];
+#pragma unroll
+                for (int i = 0; i < 8; i += 2) T::store2(p + i, s[n][8 * g + i], s[n][8 * g + i + 1]);
+                u32x4 pf;
+                std::memcpy(&pf, p, 16);
+                const int key = 32 * n + 16 * g + 4 * half + sub;
+#pragma unroll
+                for (int d = 0; d < DP / 32; ++d) {
+                    const int piece = 4 * d + 2 * ((lane >> 4) & 1) + ((lane >> 1) & 1);
+                    const unsigned char *at = lv + key * S::kRow + ((piece ^ S::swz_v(key)) << 4) + (lane & 1) * 8;
+                    typedef __attribute__((address_space(3))) s16x4 *lds4;
+                    const u32x2 lo = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4)at));
+                    const u32x2 hi = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4)(at + 8 * S::kRow)));
+                    const u32x4 v = {lo[0], lo[1], hi[0], hi[1]};   // keys 16 g + 4 half + 0..3, and 8 on
+                    w.o[d] = mma(T(), v, pf, w.o[d]);
+                }
+            }
+    }
+}
+
 // One tile of 32 NT keys from LDS.  vis: bit j is set where this lane's row
-// sees key j of each 32; all: every lane sees every key.  odd: V may hold
-// values that are not finite in keys that some rows do not see.
+// sees key j of each 32; all: every lane sees every key.
 template <typename T, int DP, int NT>
 __device__ inline void add_tile(const unsigned char *lk, const unsigned char *lv, const uint32_t (&vis)[NT], bool all,
-                                bool odd, float c, row_state<T, DP> &w) {
+                                float c, row_state<T, DP> &w) {
     using S = shape<T, DP>;
-    constexpr int kShift = std::is_same<T, f16>::value ? 14 : 0;   // p is 2^kShift times the weight
+    constexpr int kShift = std::is_same<T, f16>::value ? 10 : 0;   // p is 2^kShift times the weight
+    constexpr float kSlack = 5.0f;
     const int lane = threadIdx.x & 63, half = lane >> 5, col = lane & 31;
     f32x16 s[NT];
 #pragma unroll
@@ -176,10 +236,18 @@ __device__ inline void add_tile(const unsigned char *lk, const unsigned char *lv
 #pragma unroll
         for (int i = 0; i < 16; ++i) top = fmaxf(top, s[n][i]);
     top = fmaxf(top, __shfl_xor(top, 32));
-    const float m = fmaxf(w.m, top * c);
-    const float from = (m == -INFINITY ? 0.0f : m) - kShift;
-    const float keep = __builtin_amdgcn_exp2f(w.m - (from + kShift));
-    w.m = m;
+    // The sums' reference moves only when a row's maximum has outgrown it by
+    // 2^kSlack: until then the weights are that much above 1 at most.
+    // (Row by row: a row's result does not depend on its neighbours'.)
+    const bool grown = top * c > w.m + kSlack;
+    if (__ballot(grown) != 0) {
+        const float keep = grown ? __builtin_amdgcn_exp2f(w.m - top * c) : 1.0f;
+        w.m = grown ? top * c : w.m;
+        w.l *= keep;
+#pragma unroll
+        for (int d = 0; d < DP / 32; ++d) w.o[d] *= keep;
+    }
+    const float from = (w.m == -INFINITY ? 0.0f : w.m) - kShift;
     float sum = 0.0f;
 #pragma unroll
     for (int n = 0; n < NT; ++n)
@@ -188,77 +256,8 @@ __device__ inline void add_tile(const unsigned char *lk, const unsigned char *lv
             s[n][i] = __builtin_amdgcn_exp2f(__fmaf_rn(s[n][i], c, -from));
             sum += s[n][i];
         }
-    w.l = __fmaf_rn(w.l, keep, sum);
-#pragma unroll
-    for (int d = 0; d < DP / 32; ++d) w.o[d] *= keep;
-
-    if constexpr (S::kF32) {
-#pragma unroll
-        for (int n = 0; n < NT; ++n)
-#pragma unroll
-            for (int i = 0; i < 16; ++i) {
-                const int key = 32 * n + 8 * (i >> 2) + (i & 3) + 4 * half;
-#pragma unroll
-                for (int d = 0; d < DP / 32; ++d) {
-                    const int at = 32 * d + col;
-                    uint32_t v = *reinterpret_cast<const uint32_t *>(lv + key * S::kRow + (((at >> 2) ^ S::swz_v(key)) << 4) +
-                                                                     (at & 3) * 4);
-                    if (odd) v = finite_bits(T(), v);
-                    w.o[d] = mma(f32(), __uint_as_float(v), s[n][i], w.o[d]);
-                }
-            }
-    } else {
-        const int sub = (lane >> 2) & 3;   // of the four keys that 16 lanes load for each other
-#pragma unroll
-        for (int n = 0; n < NT; ++n)
-#pragma unroll
-            for (int g = 0; g < 2; ++g) {
-                typename T::raw p[8];
-#pragma unroll
-                for (int i = 0; i < 8; i += 2) T::store2(p + i, s[n][8 * g + i], s[n][8 * g + i + 1]);
-                u32x4 pf;
-                std::memcpy(&pf, p, 16);
-                const int key = 32 * n + 16 * g + 4 * half + sub;
-#pragma unroll
-                for (int d = 0; d < DP / 32; ++d) {
-                    const int piece = 4 * d + 2 * ((lane >> 4) & 1) + ((lane >> 1) & 1);
-                    const unsigned char *at = lv + key * S::kRow + ((piece ^ S::swz_v(key)) << 4) + (lane & 1) * 8;
-                    typedef __attribute__((address_space(3))) s16x4 *lds4;
-                    const u32x2 lo = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4)at));
-                    const u32x2 hi = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4)(at + 8 * S::kRow)));
-                    u32x4 v = {lo[0], lo[1], hi[0], hi[1]};
-                    if (odd) {
-#pragma unroll
-                        for (int i = 0; i < 4; ++i) v[i] = finite_bits(T(), v[i]);
-                    }
-                    w.o[d] = mma(T(), v, pf, w.o[d]);
-                }
-            }
-    }
-    if (odd) {   // the values left out, key by key
-#pragma unroll 1
-        for (int key = 0; key < 32 * NT; ++key) {
-            float p = 0.0f;
-            uint32_t sees = 0;
-#pragma unroll
-            for (int n = 0; n < NT; ++n) {
-                if (key >> 5 == n) sees = all ? 1u : vis[n] >> (key & 31) & 1u;
-#pragma unroll
-                for (int i = 0; i < 16; ++i)
-                    if (32 * n + 8 * (i >> 2) + (i & 3) + 4 * half == key) p = s[n][i];
-            }
-            p += __shfl_xor(p, 32);   // (the other half's is 0, or this one's)
-#pragma unroll
-            for (int d = 0; d < DP / 32; ++d)
-#pragma unroll
-                for (int i = 0; i < 16; ++i) {
-                    const int at = 32 * d + 8 * (i >> 2) + 4 * half + (i & 3);
-                    const auto v = *reinterpret_cast<const typename T::raw *>(
-                        lv + key * S::kRow + ((at / S::kPer ^ S::swz_v(key)) << 4) + at % S::kPer * sizeof(typename T::raw));
-                    if (sees && odd_bits(T(), bits_of(v))) w.o[d][i] = __fmaf_rn(p, T::load(v), w.o[d][i]);
-                }
-        }
-    }
+    w.l += sum;
+    add_values<T, DP, NT>(lv, s, w);
 }
 
 // The keys that a walk meets one after the other: the prefix's tiles, then the
@@ -288,9 +287,6 @@ __device__ inline int open_walk(const args &a, int b, int hk, int most, key_walk
     w.mask = a.mask ? a.mask + b * a.mask_ld : nullptr;
     return w.prefix_tiles + (w.own + KT - 1) / KT;
 }
-
-// Sixteen bytes of zeros, for the pieces past D and the keys that no row sees.
-static __device__ const u32x4 kZeros = {0, 0, 0, 0};
 
 // Brings a tile's K and V to LDS.  DIRECT (rows that start and end at 16
 // bytes): straight from memory, still on their way when load() returns; each
@@ -352,17 +348,47 @@ struct stager {
 // What this wave sent to LDS has landed, and what it read from there has come.
 __device__ inline void landed() { __builtin_amdgcn_s_waitcnt(0x0070); }   // vmcnt(0) lgkmcnt(0)
 
-// Whether V's tile holds a value that is not finite, for the wave.
+// A causal tile that not all rows of the block see, its V in LDS: values that
+// are not finite become zeros there, so that they do not reach the rows that
+// do not see them (0 * infinity is NaN); add_odd() gives them to the others.
+// Each of `threads` threads looks at its part; whether any was found there.
 template <typename T, int DP, int KT>
-__device__ inline bool any_odd(const unsigned char *lv) {
+__device__ inline bool hide_odd(unsigned char *lv, int thread, int threads) {
     using S = shape<T, DP>;
     bool odd = false;
-    for (int i = threadIdx.x & 63; i < KT * S::kPieces; i += 64) {
-        const u32x4 v = reinterpret_cast<const u32x4 *>(lv)[i];
+    for (int i = thread; i < KT * S::kPieces; i += threads) {
+        u32x4 v = reinterpret_cast<const u32x4 *>(lv)[i];
+        bool any = false;
 #pragma unroll
-        for (int j = 0; j < 4; ++j) odd = odd || odd_bits(T(), v[j]);
+        for (int j = 0; j < 4; ++j) {
+            const uint32_t f = finite_bits<T>(v[j]);
+            any = any || f != v[j];
+            v[j] = f;
+        }
+        if (any) reinterpret_cast<u32x4 *>(lv)[i] = v;
+        odd = odd || any;
     }
-    return __ballot(odd) != 0;
+    return odd;
+}
+
+// The values that hide_odd() took out of own keys first to end, to the rows
+// that see them.  A weight is above 0 and its product with such a value is
+// that value again, which no finite sum changes: it is added as it is.
+template <typename T, int DP>
+__device__ inline void add_odd(const args &a, const typename T::raw *v, int64_t v_row, int first, int end, row_state<T, DP> &w) {
+    const int half = (threadIdx.x & 63) >> 5;
+    for (int key = first; key < end; ++key) {
+        if (key >= w.see) continue;
+#pragma unroll
+        for (int d = 0; d < DP / 32; ++d)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+                const int at = 32 * d + 8 * (i >> 2) + 4 * half + (i & 3);
+                if (at >= a.D) continue;
+                const float value = T::load(v[key * v_row + at]);
+                if (!__builtin_isfinite(value)) w.o[d][i] += value;
+            }
+    }
 }
 
 // A staged tile for this wave's rows.
@@ -381,11 +407,7 @@ __device__ inline void take_tile(const args &a, const key_walk<T> &walk, int til
         vis[i] = (c == 32 ? ~0u : (1u << c) - 1u) & static_cast<uint32_t>(bits >> (32 * i));
         mine = mine && vis[i] == ~0u;
     }
-    const bool all = __ballot(mine) == ~uint64_t{0};
-    // Causal rows share a tile that not all of them see: V needs a look.
-    bool odd = false;
-    if (!all && a.causal && !pre) odd = any_odd<T, DP, KT>(lv);
-    add_tile<T, DP, NT>(lk, lv, vis, all, odd, a.c, w);
+    add_tile<T, DP, NT>(lk, lv, vis, __ballot(mine) == ~uint64_t{0}, a.c, w);
 }
 
 // The row's result, or its part of one.  l is whole here.
@@ -436,15 +458,22 @@ __device__ inline int most_of(int see) {
     return see;
 }
 
+// The fewest own keys that any of the rows sees.
+__device__ inline int least_of(int see) {
+#pragma unroll
+    for (int d = 32; d; d >>= 1) see = min(see, __shfl_xor(see, d));
+    return see;
+}
+
 // Many rows: 32 a wave, 128 a block, which brings each tile to LDS once, into
 // one of two places while the other is used.
 template <typename T, int DP, int NT, bool DIRECT>
-__global__ __launch_bounds__(256) void attn_rows_kernel(args a) {
+__global__ __launch_bounds__(256, sizeof(typename T::raw) == 2 && DP <= 128 ? 2 : 1) void attn_rows_kernel(args a) {
     using S = shape<T, DP>;
     constexpr int KT = 32 * NT, kTile = KT * S::kRow;
     using stage = stager<T, DP, KT, 256, DIRECT>;
     extern __shared__ __align__(16) unsigned char lds[];   // [2][K, V]
-    __shared__ int see[4];
+    __shared__ int see[2][4];
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
     int at = blockIdx.x;
     const int split = at % a.splits;
@@ -454,14 +483,20 @@ __global__ __launch_bounds__(256) void attn_rows_kernel(args a) {
     const int hk = at % a.Hkv, b = at / a.Hkv;   // b: 0 for the prefix alone
     row_state<T, DP> w;
     open_rows(a, b, rt * 128 + wave * 32 + (lane & 31), hk, w);
-    const int mine = most_of(w.see);
-    if (lane == 0) see[wave] = mine;
+    const int high = most_of(w.see), low = least_of(w.used ? w.see : INT_MAX);
+    if (lane == 0) {
+        see[0][wave] = high;
+        see[1][wave] = low;
+    }
     if (__syncthreads_or(w.used) == 0) return;
     key_walk<T> walk;
-    const int most = __builtin_amdgcn_readfirstlane(max(max(see[0], see[1]), max(see[2], see[3])));
+    const int most = __builtin_amdgcn_readfirstlane(max(max(see[0][0], see[0][1]), max(see[0][2], see[0][3])));
+    const int least = __builtin_amdgcn_readfirstlane(min(min(see[1][0], see[1][1]), min(see[1][2], see[1][3])));
     const int tiles = open_walk<T, KT>(a, b, hk, most, walk);
+    const int mixed = least < most ? walk.prefix_tiles + least / KT : INT_MAX;   // from here on tiles that not all rows see
     const int per = (tiles + a.splits - 1) / a.splits, first = split * per, end = min(tiles, first + per);
     uint64_t bits = 0;
+    bool odd = false;
     if (first < end) bits = stage::load(a, walk, first, lds, lds + kTile, threadIdx.x);
 #pragma unroll 1
     for (int tile = first; tile < end; ++tile) {
@@ -470,8 +505,10 @@ __global__ __launch_bounds__(256) void attn_rows_kernel(args a) {
         __syncthreads();   // the tile is there, and all waves are done with the one before
         const uint64_t use = bits;
         if (tile + 1 < end) bits = stage::load(a, walk, tile + 1, then, then + kTile, threadIdx.x);
+        if (tile >= mixed) odd |= __syncthreads_or(hide_odd<T, DP, KT>(now + kTile, threadIdx.x, 256)) != 0;
         take_tile<T, DP, NT>(a, walk, tile, use, now, now + kTile, w);
     }
+    if (odd) add_odd(a, walk.v, walk.v_row, max(max(first, mixed) - walk.prefix_tiles, 0) * KT, (end - walk.prefix_tiles) * KT, w);
     w.l += __shfl_xor(w.l, 32);
     close_rows(a, a.part + split, w);
 }
@@ -497,20 +534,31 @@ __global__ __launch_bounds__(64 * WAVES) void attn_keys_kernel(args a) {
     open_rows(a, b, rt * 32 + (lane & 31), hk, w);
     if (__ballot(w.used) == 0) return;   // the same for all waves
     key_walk<T> walk;
-    const int tiles = open_walk<T, KT>(a, b, hk, __builtin_amdgcn_readfirstlane(most_of(w.see)), walk);
+    const int most = __builtin_amdgcn_readfirstlane(most_of(w.see));
+    const int least = __builtin_amdgcn_readfirstlane(least_of(w.used ? w.see : INT_MAX));
+    const int tiles = open_walk<T, KT>(a, b, hk, most, walk);
+    const int mixed = least < most ? walk.prefix_tiles + least / KT : INT_MAX;
+    bool odd = false;
     const int per = (tiles + a.splits - 1) / a.splits, first = split * per, end = min(tiles, first + per);
     uint64_t bits = 0;
     if (first + wave < end) bits = stage::load(a, walk, first + wave, own, own + kTile, lane);
-    int turn = 0;
+    int turn = 0, tile;
 #pragma unroll 1
-    for (int tile = first + wave; tile < end; tile += WAVES, turn ^= 1) {
+    for (tile = first + wave; tile < end; tile += WAVES, turn ^= 1) {
         unsigned char *const now = own + turn * 2 * kTile, *const then = own + (turn ^ 1) * 2 * kTile;
         landed();
         __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
         const uint64_t use = bits;
         if (tile + WAVES < end) bits = stage::load(a, walk, tile + WAVES, then, then + kTile, lane);
+        if (tile >= mixed && __ballot(hide_odd<T, DP, KT>(now + kTile, lane, 64)) != 0) {
+            odd = true;
+            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        }
         take_tile<T, DP, 1>(a, walk, tile, use, now, now + kTile, w);
     }
+    if (odd)   // of this wave's tiles
+        for (tile = first + wave; tile < end; tile += WAVES)
+            if (tile >= mixed) add_odd(a, walk.v, walk.v_row, (tile - walk.prefix_tiles) * KT, (tile - walk.prefix_tiles + 1) * KT, w);
     w.l += __shfl_xor(w.l, 32);
     if constexpr (WAVES > 1) {
         if (lane < 32) {
