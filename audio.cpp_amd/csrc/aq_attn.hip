@@ -20,10 +20,12 @@ struct join_args {
 };
 
 // One wave a row: out = sum over parts of 2^(m_part - m) sums_part, over the
-// same sum of the weights.  In the parts' order.
-template <typename T>
+// same sum of the weights.  Four columns a lane; where that leaves lanes, 64 /
+// LANES parts are taken at once, in an order that the sizes alone decide.
+template <typename T, int LANES>
 __global__ __launch_bounds__(256) void attn_join_kernel(join_args a) {
-    const int lane = threadIdx.x & 63;
+    constexpr int kAt = 64 / LANES;
+    const int lane = threadIdx.x & 63, at = (lane % LANES) * 4, set = lane / LANES;
     const int64_t r = static_cast<int64_t>(blockIdx.x) * 4 + (threadIdx.x >> 6);
     if (r >= a.rows) return;
     const int h = static_cast<int>(r % a.H);
@@ -35,20 +37,46 @@ __global__ __launch_bounds__(256) void attn_join_kernel(join_args a) {
     for (int d = 32; d; d >>= 1) m = fmaxf(m, __shfl_xor(m, d));
     const float from = m == -INFINITY ? 0.0f : m;
     float l = 0.0f, o[4] = {};
-    for (int p = 0; p < a.parts; ++p) {
-        const int64_t at = p * a.rows + r;
-        const float by = __builtin_amdgcn_exp2f(a.ml[at * 2] - from);
-        l = __fmaf_rn(a.ml[at * 2 + 1], by, l);
-        if (by == 0.0f) continue;   // (a part without a key for this row holds zeros)
+#pragma unroll 4
+    for (int p = set; p < a.parts; p += kAt) {
+        const int64_t row = p * a.rows + r;
+        const float by = __builtin_amdgcn_exp2f(a.ml[row * 2] - from);
+        l = __fmaf_rn(a.ml[row * 2 + 1], by, l);
+        float v[4] = {};
+        const float *sums = a.sums + row * a.D + at;
+        if (at + 4 <= a.D) std::memcpy(v, sums, 16);
+        else
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+                if (at + i < a.D) v[i] = sums[i];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) o[i] = __fmaf_rn(v[i], by, o[i]);
+    }
+#pragma unroll
+    for (int d = LANES; d < 64; d <<= 1) {
+        l += __shfl_xor(l, d);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) o[i] += __shfl_xor(o[i], d);
+    }
+    if (set != 0) return;
+    const float by = l == 0.0f ? 0.0f : 1.0f / l;
+    typename T::raw *to = static_cast<typename T::raw *>(a.out) + b * a.batch + t * a.row + h * a.head + at;
+    typename T::raw y[4];
+#pragma unroll
+    for (int i = 0; i < 4; i += 2) T::store2(y + i, o[i] * by, o[i + 1] * by);
+    if (at + 4 <= a.D) std::memcpy(to, y, sizeof(y));
+    else
 #pragma unroll
         for (int i = 0; i < 4; ++i)
-            if (lane + 64 * i < a.D) o[i] = __fmaf_rn(a.sums[at * a.D + lane + 64 * i], by, o[i]);
-    }
-    const float by = l == 0.0f ? 0.0f : 1.0f / l;
-    typename T::raw *to = static_cast<typename T::raw *>(a.out) + b * a.batch + t * a.row + h * a.head;
-#pragma unroll
-    for (int i = 0; i < 4; ++i)
-        if (lane + 64 * i < a.D) to[lane + 64 * i] = T::store(o[i] * by);
+            if (at + i < a.D) to[i] = y[i];
+}
+
+template <typename T>
+void launch_join(aq_ctx *ctx, const join_args &j) {
+    const dim3 grid(static_cast<uint32_t>((j.rows + 3) / 4));
+    if (j.D <= 64) aq_launch_timed(ctx, false, attn_join_kernel<T, 16>, grid, dim3(256), 0u, j);
+    else if (j.D <= 128) aq_launch_timed(ctx, false, attn_join_kernel<T, 32>, grid, dim3(256), 0u, j);
+    else aq_launch_timed(ctx, false, attn_join_kernel<T, 64>, grid, dim3(256), 0u, j);
 }
 
 // Scratch of the parts, at most.
@@ -56,49 +84,43 @@ constexpr int64_t kPartBytes = int64_t{256} << 20;
 
 int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
 
-struct plan {
-    bool rows;      // which kernel
-    int tiles, splits;
-};
-
-// A launch over `rows` rows (of each of `groups` groups) and `keys` keys: the
-// kernel, and in how many parts the keys are taken so that the card is full.
-plan plan_of(const aq_ctx *ctx, int64_t groups, int64_t rows, int64_t keys, int64_t most_parts) {
-    plan p;
-    p.rows = rows > 32;
-    p.tiles = static_cast<int>(ceil_div(rows, p.rows ? 128 : 32));
-    const int64_t blocks = groups * p.tiles, want = 2 * ctx->num_cus;
-    // at least 256 keys a part
-    const int64_t most = std::min(most_parts, ceil_div(keys, 256));
-    p.splits = static_cast<int>(std::max<int64_t>(1, std::min(most, want / std::max<int64_t>(blocks, 1))));
-    return p;
-}
-
-aq_status launch(aq_ctx *ctx, int type, const args &a, bool rows) {
-    switch (type) {
-    case AQ_T_F32: return rows ? aq_attn_impl::launch_rows_f32(ctx, a) : aq_attn_impl::launch_keys_f32(ctx, a);
-    case AQ_T_F16: return rows ? aq_attn_impl::launch_rows_f16(ctx, a) : aq_attn_impl::launch_keys_f16(ctx, a);
-    default: return rows ? aq_attn_impl::launch_rows_bf16(ctx, a) : aq_attn_impl::launch_keys_bf16(ctx, a);
-    }
+// A job over `rows` rows (of each of `groups` groups) and `keys` keys: in how
+// many parts the keys are taken so that the card is full.
+aq_attn_impl::job job_of(const aq_ctx *ctx, int walk, int type, int64_t groups, int64_t rows, int64_t keys, int64_t most_parts) {
+    aq_attn_impl::job j{};
+    j.walk = walk;
+    j.many = rows > 32;
+    j.tiles = static_cast<int>(ceil_div(rows, j.many ? 128 : 32));
+    const int64_t blocks = groups * j.tiles, want = 2 * ctx->num_cus;
+    // At least this many keys a part: fp32 products are slow enough for few.
+    const int64_t least = type == AQ_T_F32 ? 64 : 256;
+    const int64_t most = std::min(most_parts, ceil_div(keys, least));
+    j.splits = static_cast<int>(std::max<int64_t>(1, std::min(most, want / std::max<int64_t>(blocks, 1))));
+    j.blocks = static_cast<int>(blocks * j.splits);
+    return j;
 }
 
 aq_status attend(aq_ctx *ctx, int type, args a) {
     const int64_t per_stream = static_cast<int64_t>(a.T) * a.G;   // rows of a stream and key head
+    const int64_t heads = static_cast<int64_t>(a.B) * a.Hkv;
     a.rows = static_cast<int64_t>(a.B) * a.T * a.H;
     const int64_t part_bytes = a.rows * (a.D + 2) * 4, most_parts = std::max<int64_t>(kPartBytes / part_bytes, 1);
     // The streams' rows go over the prefix together where a stream alone would
     // not fill a tile of rows; then its own keys are a part of their own.
     const bool apart = a.P > 0 && a.B > 1 && per_stream < 64 && most_parts >= 2;
-    plan first, second{};
     int parts;
     if (apart) {
-        first = plan_of(ctx, a.Hkv, per_stream * a.B, a.P, most_parts / 2);
-        second = plan_of(ctx, static_cast<int64_t>(a.B) * a.Hkv, per_stream, a.S, most_parts / 2);
-        parts = first.splits + second.splits;
+        a.jobs[0] = job_of(ctx, aq_attn_impl::kPrefix, type, a.Hkv, per_stream * a.B, a.P, most_parts / 2);
+        a.jobs[1] = job_of(ctx, aq_attn_impl::kOwn, type, heads, per_stream, a.S, most_parts / 2);
+        a.jobs[1].part = a.jobs[0].splits;
+        parts = a.jobs[0].splits + a.jobs[1].splits;
     } else {
-        first = plan_of(ctx, static_cast<int64_t>(a.B) * a.Hkv, per_stream, static_cast<int64_t>(a.P) + a.S, most_parts);
-        parts = first.splits;
+        a.jobs[0] = job_of(ctx, aq_attn_impl::kBoth, type, heads, per_stream, static_cast<int64_t>(a.P) + a.S, most_parts);
+        parts = a.jobs[0].splits;
     }
+    if (int64_t{a.jobs[0].blocks} + a.jobs[1].blocks >= int64_t{1} << 24)
+        return aq_fail(ctx, AQ_E_SHAPE, "attention: %lld streams' heads of %lld rows each need more than 2^24 blocks",
+                       (long long)heads, (long long)per_stream);
     if (parts > 1) {
         void *p = nullptr;
         aq_status st = aq_ctx_scratch(ctx, 9, static_cast<size_t>(parts) * static_cast<size_t>(part_bytes), &p);
@@ -106,23 +128,14 @@ aq_status attend(aq_ctx *ctx, int type, args a) {
         a.sums = static_cast<float *>(p);
         a.ml = a.sums + static_cast<int64_t>(parts) * a.rows * a.D;
     }
-    a.walk = apart ? aq_attn_impl::kPrefix : aq_attn_impl::kBoth;
-    a.tiles = first.tiles;
-    a.splits = first.splits;
-    aq_status st = launch(ctx, type, a, first.rows);
-    if (st == AQ_OK && apart) {
-        a.walk = aq_attn_impl::kOwn;
-        a.tiles = second.tiles;
-        a.splits = second.splits;
-        a.part = first.splits;
-        st = launch(ctx, type, a, second.rows);
-    }
+    aq_status st = type == AQ_T_F32   ? aq_attn_impl::launch_f32(ctx, a)
+                   : type == AQ_T_F16 ? aq_attn_impl::launch_f16(ctx, a)
+                                      : aq_attn_impl::launch_bf16(ctx, a);
     if (st != AQ_OK || parts == 1) return st;
     const join_args j{a.sums, a.ml, a.out, a.q_len, a.rows, a.so.batch, a.so.row, a.so.head, a.T, a.H, a.D, parts};
-    const dim3 grid(static_cast<uint32_t>(ceil_div(a.rows, 4)));
-    if (type == AQ_T_F32) aq_launch_timed(ctx, false, attn_join_kernel<aq_types::f32>, grid, dim3(256), 0u, j);
-    else if (type == AQ_T_F16) aq_launch_timed(ctx, false, attn_join_kernel<aq_types::f16>, grid, dim3(256), 0u, j);
-    else aq_launch_timed(ctx, false, attn_join_kernel<aq_types::bf16>, grid, dim3(256), 0u, j);
+    if (type == AQ_T_F32) launch_join<aq_types::f32>(ctx, j);
+    else if (type == AQ_T_F16) launch_join<aq_types::f16>(ctx, j);
+    else launch_join<aq_types::bf16>(ctx, j);
     AQ_HIP(ctx, hipGetLastError());
     return AQ_OK;
 }

@@ -12,6 +12,17 @@ struct strides {
     int64_t batch, row, head;   // elements
 };
 
+// A set of blocks: rows of all streams over the prefix, or of each stream over
+// its own keys, or over both.
+struct job {
+    int walk;
+    int many;      // 128 rows a block, whose waves share the keys; or 32, whose waves split them
+    int tiles;     // row tiles: of a stream, or of all streams' rows for the prefix alone
+    int splits;    // parts of the keys, by blocks
+    int part;      // the first of them in `sums`
+    int blocks;
+};
+
 struct args {
     const void *q, *pk, *pv, *k, *v;   // pk, pv: the shared prefix (no batch)
     void *out;
@@ -23,25 +34,16 @@ struct args {
     int B, T, S, P, H, Hkv, G, D;
     int causal;    // own keys up to the row's own
     int direct;    // rows of keys and values start and end at 16 bytes
-    // Work of a launch.
-    int walk;
-    int splits;    // parts of the keys, by blocks
-    int tiles;     // row tiles: of a stream, or of all streams' rows for the prefix alone
+    job jobs[2];   // of the launch; the second may be empty
     // Parts that another launch joins (null: the launch writes `out`): sums
-    // [part][row][D] and their largest scores and weights [part][row][2], row
-    // = (b T + t) H + h; this launch's parts start at `part`.
+    // [part][row][D] and their references and weights [part][row][2], row =
+    // (b T + t) H + h.
     float *sums, *ml;
-    int part;
     int64_t rows;   // B T H
 };
 
-// The launches: many rows (128 a block, its waves share the keys) and few
-// rows (32 a block, its waves share the rows and split the keys).
-aq_status launch_rows_f32(aq_ctx *ctx, const args &a);
-aq_status launch_rows_f16(aq_ctx *ctx, const args &a);
-aq_status launch_rows_bf16(aq_ctx *ctx, const args &a);
-aq_status launch_keys_f32(aq_ctx *ctx, const args &a);
-aq_status launch_keys_f16(aq_ctx *ctx, const args &a);
-aq_status launch_keys_bf16(aq_ctx *ctx, const args &a);
+aq_status launch_f32(aq_ctx *ctx, const args &a);
+aq_status launch_f16(aq_ctx *ctx, const args &a);
+aq_status launch_bf16(aq_ctx *ctx, const args &a);
 
 }  // namespace aq_attn_impl

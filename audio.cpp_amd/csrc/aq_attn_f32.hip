@@ -2,6 +2,5 @@
 #include "aq_attn_kernels.hpp"
 
 namespace aq_attn_impl {
-aq_status launch_rows_f32(aq_ctx *ctx, const args &a) { return launch_rows<aq_types::f32>(ctx, a); }
-aq_status launch_keys_f32(aq_ctx *ctx, const args &a) { return launch_keys<aq_types::f32>(ctx, a); }
+aq_status launch_f32(aq_ctx *ctx, const args &a) { return launch<aq_types::f32>(ctx, a); }
 }  // namespace aq_attn_impl

@@ -112,7 +112,7 @@ struct row_state {
 };
 
 template <typename T, int DP>
-__device__ inline void open_rows(const args &a, int b0, int r, int hk, row_state<T, DP> &w) {
+__device__ inline void open_rows(const args &a, int walk, int b0, int r, int hk, row_state<T, DP> &w) {
     using S = shape<T, DP>;
     const int half = (threadIdx.x & 63) >> 5;
     const int tok = r / a.G;
@@ -120,7 +120,7 @@ __device__ inline void open_rows(const args &a, int b0, int r, int hk, row_state
     w.t = tok % a.T;
     w.h = hk * a.G + r % a.G;
     // (for a stream's own walk b0 is the stream, and rows past its T tokens are no rows)
-    w.used = w.b < a.B && (a.walk == kPrefix || tok < a.T);
+    w.used = w.b < a.B && (walk == kPrefix || tok < a.T);
     int rows = a.T, keys = a.S;
     if (w.used) {
         if (a.q_len) rows = max(0, min(a.q_len[w.b], a.T));
@@ -169,6 +169,7 @@ __device__ inline void add_values(const unsigned char *lv, const f32x16 (&s)[NT]
                                                                            (at & 3) * 4);
                     w.o[d] = mma(f32(), __uint_as_float(v), s[n][i], w.o[d]);
                 }
+                if (DP > 128) __builtin_amdgcn_sched_barrier(0);
             }
     } else {
         const int sub = (lane >> 2) & 3;   // of the four keys that 16 lanes load for each other
@@ -217,6 +218,7 @@ __device__ inline void add_tile(const unsigned char *lk, const unsigned char *lv
             if constexpr (S::kF32) {
 #pragma unroll
                 for (int j = 0; j < 4; ++j) s[n] = mma(f32(), __uint_as_float(k[j]), __uint_as_float(w.q[i][j]), s[n]);
+                if (DP > 128 && i % 4 == 3) __builtin_amdgcn_sched_barrier(0);   // (or loads run so far ahead that registers spill)
             } else {
                 s[n] = mma(T(), k, w.q[i], s[n]);
             }
@@ -271,11 +273,11 @@ struct key_walk {
 };
 
 template <typename T, int KT>
-__device__ inline int open_walk(const args &a, int b, int hk, int most, key_walk<T> &w) {
+__device__ inline int open_walk(const args &a, int walk, int b, int hk, int most, key_walk<T> &w) {
     using E = typename T::raw;
-    w.P = a.walk & kPrefix ? a.P : 0;
+    w.P = walk & kPrefix ? a.P : 0;
     w.prefix_tiles = (w.P + KT - 1) / KT;
-    w.own = a.walk & kOwn ? most : 0;
+    w.own = walk & kOwn ? most : 0;
     w.pk = static_cast<const E *>(a.pk) + hk * a.spk.head;
     w.pv = static_cast<const E *>(a.pv) + hk * a.spv.head;
     w.k = static_cast<const E *>(a.k) + b * a.sk.batch + hk * a.sk.head;
@@ -351,12 +353,14 @@ __device__ inline void landed() { __builtin_amdgcn_s_waitcnt(0x0070); }   // vmc
 // A causal tile that not all rows of the block see, its V in LDS: values that
 // are not finite become zeros there, so that they do not reach the rows that
 // do not see them (0 * infinity is NaN); add_odd() gives them to the others.
-// Each of `threads` threads looks at its part; whether any was found there.
-template <typename T, int DP, int KT>
-__device__ inline bool hide_odd(unsigned char *lv, int thread, int threads) {
+// Each of THREADS threads looks at its part; whether any was found there.
+template <typename T, int DP, int KT, int THREADS>
+__device__ inline bool hide_odd(unsigned char *lv, int thread) {
     using S = shape<T, DP>;
     bool odd = false;
-    for (int i = thread; i < KT * S::kPieces; i += threads) {
+#pragma unroll 1
+    for (int n = 0; n < KT * S::kPieces / THREADS; ++n) {
+        const int i = n * THREADS + thread;
         u32x4 v = reinterpret_cast<const u32x4 *>(lv)[i];
         bool any = false;
 #pragma unroll
@@ -377,17 +381,21 @@ __device__ inline bool hide_odd(unsigned char *lv, int thread, int threads) {
 template <typename T, int DP>
 __device__ inline void add_odd(const args &a, const typename T::raw *v, int64_t v_row, int first, int end, row_state<T, DP> &w) {
     const int half = (threadIdx.x & 63) >> 5;
+#pragma unroll 1
     for (int key = first; key < end; ++key) {
-        if (key >= w.see) continue;
+        int D = key < w.see ? a.D : 0;
+        asm("" : "+v"(D));   // (compared anew for each key: 16 DP / 32 comparisons kept over the loop fill the scalar registers)
+        const typename T::raw *row = v + key * v_row;
 #pragma unroll
-        for (int d = 0; d < DP / 32; ++d)
+        for (int d = 0; d < DP / 32; ++d) {
 #pragma unroll
             for (int i = 0; i < 16; ++i) {
                 const int at = 32 * d + 8 * (i >> 2) + 4 * half + (i & 3);
-                if (at >= a.D) continue;
-                const float value = T::load(v[key * v_row + at]);
-                if (!__builtin_isfinite(value)) w.o[d][i] += value;
+                const float value = T::load(row[max(min(at, D - 1), 0)]);
+                w.o[d][i] += at < D && !(__builtin_fabsf(value) < INFINITY) ? value : 0.0f;
             }
+            __builtin_amdgcn_sched_barrier(0);
+        }
     }
 }
 
@@ -465,24 +473,35 @@ __device__ inline int least_of(int see) {
     return see;
 }
 
+// Where a block stands in its job.  The key head is outermost, so that blocks
+// near each other share a prefix; the streams' order comes next.
+struct place {
+    int hk, b, tile, split;   // b: 0 for the prefix alone
+};
+
+__device__ inline place place_of(const args &a, const job &j, int at) {
+    place p;
+    p.split = at % j.splits;
+    at /= j.splits;
+    p.tile = at % j.tiles;
+    at /= j.tiles;
+    const int streams = j.walk == kPrefix ? 1 : a.B;
+    p.b = at % streams;
+    p.hk = at / streams;
+    return p;
+}
+
 // Many rows: 32 a wave, 128 a block, which brings each tile to LDS once, into
 // one of two places while the other is used.
 template <typename T, int DP, int NT, bool DIRECT>
-__global__ __launch_bounds__(256, sizeof(typename T::raw) == 2 && DP <= 128 ? 2 : 1) void attn_rows_kernel(args a) {
+__device__ inline void rows_body(const args &a, const job &j, const place &at, unsigned char *lds) {
     using S = shape<T, DP>;
     constexpr int KT = 32 * NT, kTile = KT * S::kRow;
     using stage = stager<T, DP, KT, 256, DIRECT>;
-    extern __shared__ __align__(16) unsigned char lds[];   // [2][K, V]
     __shared__ int see[2][4];
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
-    int at = blockIdx.x;
-    const int split = at % a.splits;
-    at /= a.splits;
-    const int rt = at % a.tiles;
-    at /= a.tiles;
-    const int hk = at % a.Hkv, b = at / a.Hkv;   // b: 0 for the prefix alone
     row_state<T, DP> w;
-    open_rows(a, b, rt * 128 + wave * 32 + (lane & 31), hk, w);
+    open_rows(a, j.walk, at.b, at.tile * 128 + wave * 32 + (lane & 31), at.hk, w);
     const int high = most_of(w.see), low = least_of(w.used ? w.see : INT_MAX);
     if (lane == 0) {
         see[0][wave] = high;
@@ -492,9 +511,9 @@ __global__ __launch_bounds__(256, sizeof(typename T::raw) == 2 && DP <= 128 ? 2 
     key_walk<T> walk;
     const int most = __builtin_amdgcn_readfirstlane(max(max(see[0][0], see[0][1]), max(see[0][2], see[0][3])));
     const int least = __builtin_amdgcn_readfirstlane(min(min(see[1][0], see[1][1]), min(see[1][2], see[1][3])));
-    const int tiles = open_walk<T, KT>(a, b, hk, most, walk);
+    const int tiles = open_walk<T, KT>(a, j.walk, at.b, at.hk, most, walk);
     const int mixed = least < most ? walk.prefix_tiles + least / KT : INT_MAX;   // from here on tiles that not all rows see
-    const int per = (tiles + a.splits - 1) / a.splits, first = split * per, end = min(tiles, first + per);
+    const int per = (tiles + j.splits - 1) / j.splits, first = at.split * per, end = min(tiles, first + per);
     uint64_t bits = 0;
     bool odd = false;
     if (first < end) bits = stage::load(a, walk, first, lds, lds + kTile, threadIdx.x);
@@ -505,129 +524,128 @@ __global__ __launch_bounds__(256, sizeof(typename T::raw) == 2 && DP <= 128 ? 2 
         __syncthreads();   // the tile is there, and all waves are done with the one before
         const uint64_t use = bits;
         if (tile + 1 < end) bits = stage::load(a, walk, tile + 1, then, then + kTile, threadIdx.x);
-        if (tile >= mixed) odd |= __syncthreads_or(hide_odd<T, DP, KT>(now + kTile, threadIdx.x, 256)) != 0;
+        if (tile >= mixed) odd |= __syncthreads_or(hide_odd<T, DP, KT, 256>(now + kTile, threadIdx.x)) != 0;
         take_tile<T, DP, NT>(a, walk, tile, use, now, now + kTile, w);
     }
     if (odd) add_odd(a, walk.v, walk.v_row, max(max(first, mixed) - walk.prefix_tiles, 0) * KT, (end - walk.prefix_tiles) * KT, w);
     w.l += __shfl_xor(w.l, 32);
-    close_rows(a, a.part + split, w);
+    close_rows(a, j.part + at.split, w);
 }
 
-// Few rows: 32 a block; each of its waves takes every WAVES-th tile, with LDS
-// of its own, and the waves' sums are joined in LDS, in the waves' order.
+// Few rows: 32 a block; each of its first WAVES waves takes every WAVES-th
+// tile, with LDS of its own, and the waves' sums are joined in LDS, in the
+// waves' order.  A wave waits for its tile; what overlaps are the eight waves
+// of a compute unit.
 template <typename T, int DP, int WAVES, bool DIRECT>
-__global__ __launch_bounds__(64 * WAVES) void attn_keys_kernel(args a) {
+__device__ inline void keys_body(const args &a, const job &j, const place &at, unsigned char *lds) {
     using S = shape<T, DP>;
     constexpr int KT = 32, kTile = KT * S::kRow;
     using stage = stager<T, DP, KT, 64, DIRECT>;
-    extern __shared__ __align__(16) unsigned char lds[];   // [waves][2][K, V]
     __shared__ float ml[WAVES][2][32];
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
-    unsigned char *const own = lds + wave * 4 * kTile;
-    int at = blockIdx.x;
-    const int split = at % a.splits;
-    at /= a.splits;
-    const int rt = at % a.tiles;
-    at /= a.tiles;
-    const int hk = at % a.Hkv, b = at / a.Hkv;
+    unsigned char *const own = lds + wave * 2 * kTile;
     row_state<T, DP> w;
-    open_rows(a, b, rt * 32 + (lane & 31), hk, w);
+    open_rows(a, j.walk, at.b, at.tile * 32 + (lane & 31), at.hk, w);
     if (__ballot(w.used) == 0) return;   // the same for all waves
     key_walk<T> walk;
     const int most = __builtin_amdgcn_readfirstlane(most_of(w.see));
     const int least = __builtin_amdgcn_readfirstlane(least_of(w.used ? w.see : INT_MAX));
-    const int tiles = open_walk<T, KT>(a, b, hk, most, walk);
+    const int tiles = open_walk<T, KT>(a, j.walk, at.b, at.hk, most, walk);
     const int mixed = least < most ? walk.prefix_tiles + least / KT : INT_MAX;
     bool odd = false;
-    const int per = (tiles + a.splits - 1) / a.splits, first = split * per, end = min(tiles, first + per);
-    uint64_t bits = 0;
-    if (first + wave < end) bits = stage::load(a, walk, first + wave, own, own + kTile, lane);
-    int turn = 0, tile;
+    const int per = (tiles + j.splits - 1) / j.splits, first = at.split * per;
+    const int end = wave < WAVES ? min(tiles, first + per) : 0;
+    int tile;
 #pragma unroll 1
-    for (tile = first + wave; tile < end; tile += WAVES, turn ^= 1) {
-        unsigned char *const now = own + turn * 2 * kTile, *const then = own + (turn ^ 1) * 2 * kTile;
+    for (tile = first + wave; tile < end; tile += WAVES) {
+        const uint64_t bits = stage::load(a, walk, tile, own, own + kTile, lane);
         landed();
         __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-        const uint64_t use = bits;
-        if (tile + WAVES < end) bits = stage::load(a, walk, tile + WAVES, then, then + kTile, lane);
-        if (tile >= mixed && __ballot(hide_odd<T, DP, KT>(now + kTile, lane, 64)) != 0) {
+        if (tile >= mixed && __ballot(hide_odd<T, DP, KT, 64>(own + kTile, lane)) != 0) {
             odd = true;
             __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
         }
-        take_tile<T, DP, 1>(a, walk, tile, use, now, now + kTile, w);
+        take_tile<T, DP, 1>(a, walk, tile, bits, own, own + kTile, w);
+        landed();   // its last reads, before the next tile takes the place
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
     }
     if (odd)   // of this wave's tiles
         for (tile = first + wave; tile < end; tile += WAVES)
             if (tile >= mixed) add_odd(a, walk.v, walk.v_row, (tile - walk.prefix_tiles) * KT, (tile - walk.prefix_tiles + 1) * KT, w);
     w.l += __shfl_xor(w.l, 32);
-    if constexpr (WAVES > 1) {
-        if (lane < 32) {
-            ml[wave][0][lane] = w.m;
-            ml[wave][1][lane] = w.l;
-        }
-        __syncthreads();   // (the tiles are not used any more either)
-        float m = -INFINITY, l = 0.0f;
+    if (wave < WAVES && lane < 32) {
+        ml[wave][0][lane] = w.m;
+        ml[wave][1][lane] = w.l;
+    }
+    __syncthreads();   // (the tiles are not used any more either)
+    float m = -INFINITY, l = 0.0f;
 #pragma unroll
-        for (int i = 0; i < WAVES; ++i) m = fmaxf(m, ml[i][0][lane & 31]);
-        const float from = m == -INFINITY ? 0.0f : m;
+    for (int i = 0; i < WAVES; ++i) m = fmaxf(m, ml[i][0][lane & 31]);
+    const float from = m == -INFINITY ? 0.0f : m;
 #pragma unroll
-        for (int i = 0; i < WAVES; ++i) l = __fmaf_rn(ml[i][1][lane & 31], __builtin_amdgcn_exp2f(ml[i][0][lane & 31] - from), l);
-        const float keep = __builtin_amdgcn_exp2f(w.m - from);
-        f32x16 *const red = reinterpret_cast<f32x16 *>(lds);   // [WAVES][DP / 32][64]
+    for (int i = 0; i < WAVES; ++i) l = __fmaf_rn(ml[i][1][lane & 31], __builtin_amdgcn_exp2f(ml[i][0][lane & 31] - from), l);
+    const float keep = __builtin_amdgcn_exp2f(w.m - from);
+    f32x16 *const red = reinterpret_cast<f32x16 *>(lds);   // [WAVES][DP / 32][64]
+    if (wave < WAVES) {
 #pragma unroll
         for (int d = 0; d < DP / 32; ++d) red[(wave * (DP / 32) + d) * 64 + lane] = w.o[d] * keep;
-        __syncthreads();
-        if (wave != 0) return;
-#pragma unroll
-        for (int d = 0; d < DP / 32; ++d) {
-            w.o[d] = red[d * 64 + lane];
-#pragma unroll
-            for (int i = 1; i < WAVES; ++i) w.o[d] += red[(i * (DP / 32) + d) * 64 + lane];
-        }
-        w.m = m;
-        w.l = l;
     }
-    close_rows(a, a.part + split, w);
+    __syncthreads();
+    if (wave != 0) return;
+#pragma unroll
+    for (int d = 0; d < DP / 32; ++d) {
+        w.o[d] = red[d * 64 + lane];
+#pragma unroll
+        for (int i = 1; i < WAVES; ++i) w.o[d] += red[(i * (DP / 32) + d) * 64 + lane];
+    }
+    w.m = m;
+    w.l = l;
+    close_rows(a, j.part + at.split, w);
 }
 
-template <typename K>
-aq_status run(aq_ctx *ctx, const args &a, K kernel, int threads, uint32_t lds) {
+// The blocks of one job, or of two at once, evenly mixed: a prefix's products
+// and the streams' own keys, which wait for memory, share the compute units.
+template <typename T, int DP, int NT, int WAVES, bool DIRECT>
+__global__ __launch_bounds__(256, sizeof(typename T::raw) == 2 && DP <= 128 ? 2 : 1) void attn_kernel(args a) {
+    extern __shared__ __align__(16) unsigned char lds[];
+    // Blocks are dealt to the eight dies in turn; each die gets a run of
+    // neighbours, which share keys, and so its cache serves them.
+    const int total = gridDim.x, die = blockIdx.x % 8;
+    const int at = die * (total / 8) + min(die, total % 8) + blockIdx.x / 8;
+    const int64_t n0 = a.jobs[0].blocks;
+    const int before = static_cast<int>(at * n0 / total), after = static_cast<int>((at + 1) * n0 / total);
+    const job &j = after > before ? a.jobs[0] : a.jobs[1];
+    const place p = place_of(a, j, after > before ? before : at - before);
+    if (j.many) rows_body<T, DP, NT, DIRECT>(a, j, p, lds);
+    else keys_body<T, DP, WAVES, DIRECT>(a, j, p, lds);
+}
+
+template <typename T, int DP, int NT, int WAVES>
+aq_status run(aq_ctx *ctx, const args &a) {
+    constexpr uint32_t kRows = 4 * 32 * NT * shape<T, DP>::kRow, kKeys = WAVES * 2 * 32 * shape<T, DP>::kRow;
+    static_assert(kKeys >= WAVES * 32 * DP * 4, "the waves' sums fit where the tiles were");
+    uint32_t lds = 0;
+    int64_t blocks = 0;
+    for (const job &j : a.jobs) {
+        if (!j.blocks) continue;
+        const uint32_t need = j.many ? kRows : kKeys;
+        if (need > lds) lds = need;
+        blocks += j.blocks;
+    }
+    auto kernel = a.direct ? attn_kernel<T, DP, NT, WAVES, true> : attn_kernel<T, DP, NT, WAVES, false>;
     aq_status st = aq_launch_lds(ctx, reinterpret_cast<const void *>(kernel), lds, "attention");
     if (st != AQ_OK) return st;
-    const int64_t grid = static_cast<int64_t>(a.walk == kPrefix ? 1 : a.B) * a.Hkv * a.tiles * a.splits;
-    aq_launch_timed(ctx, true, kernel, dim3(static_cast<uint32_t>(grid)), dim3(static_cast<uint32_t>(threads)), lds, a);
+    aq_launch_timed(ctx, true, kernel, dim3(static_cast<uint32_t>(blocks)), dim3(256), lds, a);
     AQ_HIP(ctx, hipGetLastError());
     return AQ_OK;
 }
 
-template <typename T, int DP, int NT>
-aq_status run_rows(aq_ctx *ctx, const args &a) {
-    constexpr uint32_t kLds = 4 * 32 * NT * shape<T, DP>::kRow;
-    if (a.direct) return run(ctx, a, attn_rows_kernel<T, DP, NT, true>, 256, kLds);
-    return run(ctx, a, attn_rows_kernel<T, DP, NT, false>, 256, kLds);
-}
-
-template <typename T, int DP, int WAVES>
-aq_status run_keys(aq_ctx *ctx, const args &a) {
-    constexpr uint32_t kLds = WAVES * 4 * 32 * shape<T, DP>::kRow;   // the waves' sums, 32 rows of DP floats each, fit
-    if (a.direct) return run(ctx, a, attn_keys_kernel<T, DP, WAVES, true>, 64 * WAVES, kLds);
-    return run(ctx, a, attn_keys_kernel<T, DP, WAVES, false>, 64 * WAVES, kLds);
-}
-
 template <typename T>
-aq_status launch_rows(aq_ctx *ctx, const args &a) {
-    constexpr int kNT = sizeof(typename T::raw) == 4 ? 1 : 2;
-    if (a.D <= 64) return run_rows<T, 64, kNT>(ctx, a);
-    if (a.D <= 128) return run_rows<T, 128, kNT>(ctx, a);
-    return run_rows<T, 256, 1>(ctx, a);
-}
-
-template <typename T>
-aq_status launch_keys(aq_ctx *ctx, const args &a) {
-    constexpr int kWide = sizeof(typename T::raw) == 4 ? 2 : 1;
-    if (a.D <= 64) return run_keys<T, 64, 4>(ctx, a);
-    if (a.D <= 128) return run_keys<T, 128, 4 / kWide>(ctx, a);
-    return run_keys<T, 256, 2 / kWide>(ctx, a);
+aq_status launch(aq_ctx *ctx, const args &a) {
+    constexpr bool kWide = sizeof(typename T::raw) == 4;
+    if (a.D <= 64) return run<T, 64, kWide ? 1 : 2, 4>(ctx, a);
+    if (a.D <= 128) return run<T, 128, kWide ? 1 : 2, 4>(ctx, a);
+    return run<T, 256, 1, kWide ? 2 : 4>(ctx, a);
 }
 
 }  // namespace aq_attn_impl
