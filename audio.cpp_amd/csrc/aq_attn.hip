@@ -86,10 +86,10 @@ int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
 
 // A job over `rows` rows (of each of `groups` groups) and `keys` keys: in how
 // many parts the keys are taken so that the card is full.
-aq_attn_impl::job job_of(const aq_ctx *ctx, int walk, int type, int64_t groups, int64_t rows, int64_t keys, int64_t most_parts) {
+aq_attn_impl::job job_of(const aq_ctx *ctx, int walk, int type, int D, int64_t groups, int64_t rows, int64_t keys, int64_t most_parts) {
     aq_attn_impl::job j{};
     j.walk = walk;
-    j.many = rows > 32;
+    j.many = rows > 32 || (type == AQ_T_F32 && D > 128);   // (such rows have the first kind of block only)
     j.tiles = static_cast<int>(ceil_div(rows, j.many ? 128 : 32));
     const int64_t blocks = groups * j.tiles, want = 2 * ctx->num_cus;
     // At least this many keys a part: fp32 products are slow enough for few.
@@ -110,12 +110,12 @@ aq_status attend(aq_ctx *ctx, int type, args a) {
     const bool apart = a.P > 0 && a.B > 1 && per_stream < 64 && most_parts >= 2;
     int parts;
     if (apart) {
-        a.jobs[0] = job_of(ctx, aq_attn_impl::kPrefix, type, a.Hkv, per_stream * a.B, a.P, most_parts / 2);
-        a.jobs[1] = job_of(ctx, aq_attn_impl::kOwn, type, heads, per_stream, a.S, most_parts / 2);
+        a.jobs[0] = job_of(ctx, aq_attn_impl::kPrefix, type, a.D, a.Hkv, per_stream * a.B, a.P, most_parts / 2);
+        a.jobs[1] = job_of(ctx, aq_attn_impl::kOwn, type, a.D, heads, per_stream, a.S, most_parts / 2);
         a.jobs[1].part = a.jobs[0].splits;
         parts = a.jobs[0].splits + a.jobs[1].splits;
     } else {
-        a.jobs[0] = job_of(ctx, aq_attn_impl::kBoth, type, heads, per_stream, static_cast<int64_t>(a.P) + a.S, most_parts);
+        a.jobs[0] = job_of(ctx, aq_attn_impl::kBoth, type, a.D, heads, per_stream, static_cast<int64_t>(a.P) + a.S, most_parts);
         parts = a.jobs[0].splits;
     }
     if (int64_t{a.jobs[0].blocks} + a.jobs[1].blocks >= int64_t{1} << 24)

@@ -347,6 +347,48 @@ struct stager {
     }
 };
 
+// The same through registers, for a tile that one wave has to itself: the next
+// tile's pieces are on their way in registers while one is used.
+template <typename T, int DP, int KT, bool DIRECT>
+struct carrier {
+    using S = shape<T, DP>;
+    using E = typename T::raw;
+    static constexpr int kEach = KT * S::kPieces / 64;
+    u32x4 k[kEach + !kEach], v[kEach + !kEach];
+    uint64_t bits;
+
+    __device__ inline void load(const args &a, const key_walk<T> &w, int tile, int lane) {
+        const bool pre = tile < w.prefix_tiles;
+        const int j0 = (pre ? tile : tile - w.prefix_tiles) * KT, n = (pre ? w.P : w.own) - j0;
+        bits = n >= 64 ? ~uint64_t{0} : (uint64_t{1} << n) - 1;
+        if (!pre && w.mask) bits &= __ballot(lane < n && w.mask[j0 + min(lane, n - 1)] != 0);
+        const int64_t kr = pre ? w.pk_row : w.k_row, vr = pre ? w.pv_row : w.v_row;
+        const E *kp = (pre ? w.pk : w.k) + j0 * kr, *vp = (pre ? w.pv : w.v) + j0 * vr;
+#pragma unroll
+        for (int i = 0; i < kEach; ++i) {
+            const int at = i * 64 + lane, key = at / S::kPieces, piece = at % S::kPieces * S::kPer;
+            const bool use = bits >> key & 1;
+            if constexpr (DIRECT) {   // whole pieces: a load each, from zeros where there is none
+                const E *const none = reinterpret_cast<const E *>(&kZeros);
+                const bool in = use && piece < a.D;
+                k[i] = *reinterpret_cast<const u32x4 *>(in ? kp + key * kr + piece : none);
+                v[i] = *reinterpret_cast<const u32x4 *>(in ? vp + key * vr + piece : none);
+            } else {
+                k[i] = load_piece<T>(kp + key * kr, piece, a.D, use);
+                v[i] = load_piece<T>(vp + key * vr, piece, a.D, use);
+            }
+        }
+    }
+    __device__ inline void store(unsigned char *lk, unsigned char *lv, int lane) const {
+#pragma unroll
+        for (int i = 0; i < kEach; ++i) {
+            const int at = i * 64 + lane, key = at / S::kPieces, piece = at % S::kPieces;
+            *reinterpret_cast<u32x4 *>(lk + key * S::kRow + ((piece ^ S::swz_k(key)) << 4)) = k[i];
+            *reinterpret_cast<u32x4 *>(lv + key * S::kRow + ((piece ^ S::swz_v(key)) << 4)) = v[i];
+        }
+    }
+};
+
 // What this wave sent to LDS has landed, and what it read from there has come.
 __device__ inline void landed() { __builtin_amdgcn_s_waitcnt(0x0070); }   // vmcnt(0) lgkmcnt(0)
 
@@ -534,13 +576,11 @@ __device__ inline void rows_body(const args &a, const job &j, const place &at, u
 
 // Few rows: 32 a block; each of its first WAVES waves takes every WAVES-th
 // tile, with LDS of its own, and the waves' sums are joined in LDS, in the
-// waves' order.  A wave waits for its tile; what overlaps are the eight waves
-// of a compute unit.
+// waves' order.
 template <typename T, int DP, int WAVES, bool DIRECT>
 __device__ inline void keys_body(const args &a, const job &j, const place &at, unsigned char *lds) {
     using S = shape<T, DP>;
     constexpr int KT = 32, kTile = KT * S::kRow;
-    using stage = stager<T, DP, KT, 64, DIRECT>;
     __shared__ float ml[WAVES][2][32];
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
     unsigned char *const own = lds + wave * 2 * kTile;
@@ -555,18 +595,29 @@ __device__ inline void keys_body(const args &a, const job &j, const place &at, u
     bool odd = false;
     const int per = (tiles + j.splits - 1) / j.splits, first = at.split * per;
     const int end = wave < WAVES ? min(tiles, first + per) : 0;
-    int tile;
+    constexpr bool kAhead = S::kRow <= 512 && DP <= 128;   // registers hold a tile on its way
+    carrier<T, DP, kAhead ? KT : 0, DIRECT> next;
+    int tile = first + wave;
+    if (kAhead && tile < end) next.load(a, walk, tile, lane);
 #pragma unroll 1
-    for (tile = first + wave; tile < end; tile += WAVES) {
-        const uint64_t bits = stage::load(a, walk, tile, own, own + kTile, lane);
-        landed();
-        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    for (; tile < end; tile += WAVES) {
+        uint64_t bits;
+        if constexpr (kAhead) {
+            next.store(own, own + kTile, lane);
+            bits = next.bits;
+            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+            if (tile + WAVES < end) next.load(a, walk, tile + WAVES, lane);
+        } else {
+            landed();   // the last tile's reads, before this one takes the place
+            bits = stager<T, DP, KT, 64, DIRECT>::load(a, walk, tile, own, own + kTile, lane);
+            landed();
+            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        }
         if (tile >= mixed && __ballot(hide_odd<T, DP, KT, 64>(own + kTile, lane)) != 0) {
             odd = true;
             __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
         }
         take_tile<T, DP, 1>(a, walk, tile, bits, own, own + kTile, w);
-        landed();   // its last reads, before the next tile takes the place
         __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
     }
     if (odd)   // of this wave's tiles
@@ -606,7 +657,7 @@ __device__ inline void keys_body(const args &a, const job &j, const place &at, u
 // The blocks of one job, or of two at once, evenly mixed: a prefix's products
 // and the streams' own keys, which wait for memory, share the compute units.
 template <typename T, int DP, int NT, int WAVES, bool DIRECT>
-__global__ __launch_bounds__(256, sizeof(typename T::raw) == 2 && DP <= 128 ? 2 : 1) void attn_kernel(args a) {
+__global__ __launch_bounds__(256, sizeof(typename T::raw) * DP <= 256 ? 2 : 1) void attn_kernel(args a) {
     extern __shared__ __align__(16) unsigned char lds[];
     // Blocks are dealt to the eight dies in turn; each die gets a run of
     // neighbours, which share keys, and so its cache serves them.
@@ -616,8 +667,13 @@ __global__ __launch_bounds__(256, sizeof(typename T::raw) == 2 && DP <= 128 ? 2 
     const int before = static_cast<int>(at * n0 / total), after = static_cast<int>((at + 1) * n0 / total);
     const job &j = after > before ? a.jobs[0] : a.jobs[1];
     const place p = place_of(a, j, after > before ? before : at - before);
-    if (j.many) rows_body<T, DP, NT, DIRECT>(a, j, p, lds);
-    else keys_body<T, DP, WAVES, DIRECT>(a, j, p, lds);
+    if constexpr (WAVES > 0) {
+        if (!j.many) {
+            keys_body<T, DP, WAVES, DIRECT>(a, j, p, lds);
+            return;
+        }
+    }
+    rows_body<T, DP, NT, DIRECT>(a, j, p, lds);
 }
 
 template <typename T, int DP, int NT, int WAVES>
@@ -645,7 +701,7 @@ aq_status launch(aq_ctx *ctx, const args &a) {
     constexpr bool kWide = sizeof(typename T::raw) == 4;
     if (a.D <= 64) return run<T, 64, kWide ? 1 : 2, 4>(ctx, a);
     if (a.D <= 128) return run<T, 128, kWide ? 1 : 2, 4>(ctx, a);
-    return run<T, 256, 1, kWide ? 2 : 4>(ctx, a);
+    return run<T, 256, 1, kWide ? 0 : 4>(ctx, a);   // (no registers for an fp32 tile of that width on its way)
 }
 
 }  // namespace aq_attn_impl
