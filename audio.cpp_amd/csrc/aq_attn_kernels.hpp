@@ -111,7 +111,7 @@ struct row_state {
     int see;           // own keys that it sees
 };
 
-template <typename T, int DP>
+template <typename T, int DP, bool DIRECT>
 __device__ inline void open_rows(const args &a, int walk, int b0, int r, int hk, row_state<T, DP> &w) {
     using S = shape<T, DP>;
     const int half = (threadIdx.x & 63) >> 5;
@@ -130,7 +130,7 @@ __device__ inline void open_rows(const args &a, int walk, int b0, int r, int hk,
     w.see = !w.used ? 0 : a.causal ? max(0, keys - rows + w.t + 1) : keys;
     const typename T::raw *row = static_cast<const typename T::raw *>(a.q);
     if (w.used) row += w.b * a.sq.batch + w.t * a.sq.row + w.h * a.sq.head;
-    if (a.D % S::kPer == 0) {   // whole pieces: one load each, and all on their way together
+    if constexpr (DIRECT) {   // whole pieces: one load each, and all on their way together
 #pragma unroll
         for (int i = 0; i < row_state<T, DP>::kQ; ++i) {
             typedef u32x4 any __attribute__((aligned(1)));
@@ -151,50 +151,114 @@ __device__ inline void open_rows(const args &a, int walk, int b0, int r, int hk,
     w.l = 0.0f;
 }
 
-// o += P V for a tile, p in s.
+// Steps of a chain of products whose operands come from LDS: kAhead of them are
+// on their way before the first is used.  The scheduling barriers keep it so;
+// left alone, the compiler loads each next to its use, or all at once.
+// (One row tile's products next to a tile on its way leave room for two.)
+template <int NT> constexpr int kAheadSteps = NT > 1 ? 4 : 2;
+
+// S^T for a tile of 32 NT keys: s[n] += K q.
 template <typename T, int DP, int NT>
-__device__ inline void add_values(const unsigned char *lv, const f32x16 (&s)[NT], row_state<T, DP> &w) {
+__device__ inline void add_scores(const unsigned char *lk, f32x16 (&s)[NT], const row_state<T, DP> &w) {
+    using S = shape<T, DP>;
+    constexpr int kQ = row_state<T, DP>::kQ, kSteps = NT * kQ, kAhead = kAheadSteps<NT>, kRing = kAhead + 1;
+    const int lane = threadIdx.x & 63, half = lane >> 5, col = lane & 31;
+    const auto piece = [&](int e) {
+        const int key = 32 * (e % NT) + col, i = e / NT;
+        return *reinterpret_cast<const u32x4 *>(lk + key * S::kRow + (((2 * i + half) ^ S::swz_k(key)) << 4));
+    };
+#pragma unroll
+    for (int n = 0; n < NT; ++n)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) s[n][i] = 0.0f;
+    u32x4 ring[kRing];
+#pragma unroll
+    for (int e = 0; e < kAhead; ++e) ring[e] = piece(e);
+#pragma unroll
+    for (int e = 0; e < kSteps; ++e) {
+        if (e + kAhead < kSteps) ring[(e + kAhead) % kRing] = piece(e + kAhead);
+        __builtin_amdgcn_sched_barrier(0);
+        const u32x4 k = ring[e % kRing];
+        if constexpr (S::kF32) {
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+                s[e % NT] = mma(f32(), __uint_as_float(k[j]), __uint_as_float(w.q[e / NT][j]), s[e % NT]);
+        } else {
+            s[e % NT] = mma(T(), k, w.q[e / NT], s[e % NT]);
+        }
+    }
+}
+
+// o += P V, with p = 2^(c s - from): the sum of the lane's p comes back.  16-bit
+// types: the exponentials of 16 keys are taken between the products of the 16
+// before them.
+template <typename T, int DP, int NT>
+__device__ inline float add_values(const unsigned char *lv, f32x16 (&s)[NT], float c, float from, row_state<T, DP> &w) {
     using S = shape<T, DP>;
     const int lane = threadIdx.x & 63, half = lane >> 5, col = lane & 31;
+    constexpr int kD = DP / 32;
+    float sum = 0.0f;
+    const auto weigh = [&](int n, int i) {
+        s[n][i] = __builtin_amdgcn_exp2f(__fmaf_rn(s[n][i], c, -from));
+        sum += s[n][i];
+    };
     if constexpr (S::kF32) {
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) weigh(n, i);
 #pragma unroll
         for (int n = 0; n < NT; ++n)
 #pragma unroll
             for (int i = 0; i < 16; ++i) {
                 const int key = 32 * n + 8 * (i >> 2) + (i & 3) + 4 * half;   // this half's
 #pragma unroll
-                for (int d = 0; d < DP / 32; ++d) {
+                for (int d = 0; d < kD; ++d) {
                     const int at = 32 * d + col;
                     const uint32_t v = *reinterpret_cast<const uint32_t *>(lv + key * S::kRow + (((at >> 2) ^ S::swz_v(key)) << 4) +
                                                                            (at & 3) * 4);
                     w.o[d] = mma(f32(), __uint_as_float(v), s[n][i], w.o[d]);
                 }
-                if (DP > 128) __builtin_amdgcn_sched_barrier(0);
+                if (DP > 128) __builtin_amdgcn_sched_barrier(0);   // (or loads run so far ahead that registers spill)
             }
     } else {
+        constexpr int kGroups = 2 * NT, kSteps = kGroups * kD, kAhead = kAheadSteps<NT>, kRing = kAhead + 1;
         const int sub = (lane >> 2) & 3;   // of the four keys that 16 lanes load for each other
+        const auto values = [&](int e) {   // keys 16 (e / kD) + 4 half + 0..3, and 8 on, of column 32 (e % kD) + col
+            const int key = 16 * (e / kD) + 4 * half + sub, piece = 4 * (e % kD) + 2 * ((lane >> 4) & 1) + ((lane >> 1) & 1);
+            const unsigned char *at = lv + key * S::kRow + ((piece ^ S::swz_v(key)) << 4) + (lane & 1) * 8;
+            typedef __attribute__((address_space(3))) s16x4 *lds4;
+            const u32x2 lo = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4)at));
+            const u32x2 hi = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4)(at + 8 * S::kRow)));
+            return u32x4{lo[0], lo[1], hi[0], hi[1]};
+        };
+        const auto packed = [&](int g) {
+            typename T::raw p[8];
+            u32x4 r;
 #pragma unroll
-        for (int n = 0; n < NT; ++n)
+            for (int i = 0; i < 8; i += 2) T::store2(p + i, s[g / 2][8 * (g % 2) + i], s[g / 2][8 * (g % 2) + i + 1]);
+            std::memcpy(&r, p, 16);
+            return r;
+        };
 #pragma unroll
-            for (int g = 0; g < 2; ++g) {
-                typename T::raw p[8];
+        for (int i = 0; i < 8; ++i) weigh(0, i);
+        u32x4 ring[kRing], p = packed(0);
 #pragma unroll
-                for (int i = 0; i < 8; i += 2) T::store2(p + i, s[n][8 * g + i], s[n][8 * g + i + 1]);
-                u32x4 pf;
-                std::memcpy(&pf, p, 16);
-                const int key = 32 * n + 16 * g + 4 * half + sub;
+        for (int e = 0; e < kAhead; ++e) ring[e] = values(e);
 #pragma unroll
-                for (int d = 0; d < DP / 32; ++d) {
-                    const int piece = 4 * d + 2 * ((lane >> 4) & 1) + ((lane >> 1) & 1);
-                    const unsigned char *at = lv + key * S::kRow + ((piece ^ S::swz_v(key)) << 4) + (lane & 1) * 8;
-                    typedef __attribute__((address_space(3))) s16x4 *lds4;
-                    const u32x2 lo = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4)at));
-                    const u32x2 hi = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4)(at + 8 * S::kRow)));
-                    const u32x4 v = {lo[0], lo[1], hi[0], hi[1]};   // keys 16 g + 4 half + 0..3, and 8 on
-                    w.o[d] = mma(T(), v, pf, w.o[d]);
-                }
+        for (int e = 0; e < kSteps; ++e) {
+            const int g = e / kD, d = e % kD;
+            if (e + kAhead < kSteps) ring[(e + kAhead) % kRing] = values(e + kAhead);
+            __builtin_amdgcn_sched_barrier(0);
+            w.o[d] = mma(T(), ring[e % kRing], p, w.o[d]);
+            if (g + 1 < kGroups) {
+#pragma unroll
+                for (int i = 8 * d / kD; i < 8 * (d + 1) / kD; ++i) weigh((g + 1) / 2, 8 * ((g + 1) % 2) + i);
+                if (d == kD - 1) p = packed(g + 1);
             }
+        }
     }
+    return sum;
 }
 
 // One tile of 32 NT keys from LDS.  vis: bit j is set where this lane's row
@@ -202,28 +266,11 @@ __device__ inline void add_values(const unsigned char *lv, const f32x16 (&s)[NT]
 template <typename T, int DP, int NT>
 __device__ inline void add_tile(const unsigned char *lk, const unsigned char *lv, const uint32_t (&vis)[NT], bool all,
                                 float c, row_state<T, DP> &w) {
-    using S = shape<T, DP>;
     constexpr int kShift = std::is_same<T, f16>::value ? 10 : 0;   // p is 2^kShift times the weight
     constexpr float kSlack = 5.0f;
-    const int lane = threadIdx.x & 63, half = lane >> 5, col = lane & 31;
+    const int half = (threadIdx.x & 63) >> 5;
     f32x16 s[NT];
-#pragma unroll
-    for (int n = 0; n < NT; ++n) {
-#pragma unroll
-        for (int i = 0; i < 16; ++i) s[n][i] = 0.0f;
-        const int key = 32 * n + col;
-#pragma unroll
-        for (int i = 0; i < row_state<T, DP>::kQ; ++i) {
-            const u32x4 k = *reinterpret_cast<const u32x4 *>(lk + key * S::kRow + (((2 * i + half) ^ S::swz_k(key)) << 4));
-            if constexpr (S::kF32) {
-#pragma unroll
-                for (int j = 0; j < 4; ++j) s[n] = mma(f32(), __uint_as_float(k[j]), __uint_as_float(w.q[i][j]), s[n]);
-                if (DP > 128 && i % 4 == 3) __builtin_amdgcn_sched_barrier(0);   // (or loads run so far ahead that registers spill)
-            } else {
-                s[n] = mma(T(), k, w.q[i], s[n]);
-            }
-        }
-    }
+    add_scores<T, DP, NT>(lk, s, w);
     if (!all) {
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
@@ -249,17 +296,7 @@ __device__ inline void add_tile(const unsigned char *lk, const unsigned char *lv
 #pragma unroll
         for (int d = 0; d < DP / 32; ++d) w.o[d] *= keep;
     }
-    const float from = (w.m == -INFINITY ? 0.0f : w.m) - kShift;
-    float sum = 0.0f;
-#pragma unroll
-    for (int n = 0; n < NT; ++n)
-#pragma unroll
-        for (int i = 0; i < 16; ++i) {
-            s[n][i] = __builtin_amdgcn_exp2f(__fmaf_rn(s[n][i], c, -from));
-            sum += s[n][i];
-        }
-    w.l += sum;
-    add_values<T, DP, NT>(lv, s, w);
+    w.l += add_values<T, DP, NT>(lv, s, c, (w.m == -INFINITY ? 0.0f : w.m) - kShift, w);
 }
 
 // The keys that a walk meets one after the other: the prefix's tiles, then the
@@ -364,18 +401,35 @@ struct carrier {
         if (!pre && w.mask) bits &= __ballot(lane < n && w.mask[j0 + min(lane, n - 1)] != 0);
         const int64_t kr = pre ? w.pk_row : w.k_row, vr = pre ? w.pv_row : w.v_row;
         const E *kp = (pre ? w.pk : w.k) + j0 * kr, *vp = (pre ? w.pv : w.v) + j0 * vr;
+        if constexpr (DIRECT) {   // whole pieces: a load each, from zeros where there is none
+            constexpr int kStep = 64 / S::kPieces;   // keys from one of a lane's pieces to the next
+            const int key = lane / S::kPieces, piece = lane % S::kPieces * S::kPer;
+            const E *kg = kp + key * kr + piece, *vg = vp + key * vr + piece;
+            constexpr uint64_t kAll = (uint64_t{1} << (KT % 64)) - 1;
+            if ((bits & kAll) == kAll && a.D == DP) {
 #pragma unroll
-        for (int i = 0; i < kEach; ++i) {
-            const int at = i * 64 + lane, key = at / S::kPieces, piece = at % S::kPieces * S::kPer;
-            const bool use = bits >> key & 1;
-            if constexpr (DIRECT) {   // whole pieces: a load each, from zeros where there is none
-                const E *const none = reinterpret_cast<const E *>(&kZeros);
-                const bool in = use && piece < a.D;
-                k[i] = *reinterpret_cast<const u32x4 *>(in ? kp + key * kr + piece : none);
-                v[i] = *reinterpret_cast<const u32x4 *>(in ? vp + key * vr + piece : none);
+                for (int i = 0; i < kEach; ++i) {
+                    k[i] = *reinterpret_cast<const u32x4 *>(kg + i * kStep * kr);
+                    v[i] = *reinterpret_cast<const u32x4 *>(vg + i * kStep * vr);
+                }
             } else {
+                const E *const none = reinterpret_cast<const E *>(&kZeros);
+#pragma unroll
+                for (int i = 0; i < kEach; ++i) {
+                    const bool in = (bits >> (key + i * kStep) & 1) != 0 && piece < a.D;
+                    k[i] = *reinterpret_cast<const u32x4 *>(in ? kg + i * kStep * kr : none);
+                    v[i] = *reinterpret_cast<const u32x4 *>(in ? vg + i * kStep * vr : none);
+                    __builtin_amdgcn_sched_barrier(0);
+                }
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < kEach; ++i) {
+                const int at = i * 64 + lane, key = at / S::kPieces, piece = at % S::kPieces * S::kPer;
+                const bool use = bits >> key & 1;
                 k[i] = load_piece<T>(kp + key * kr, piece, a.D, use);
                 v[i] = load_piece<T>(vp + key * vr, piece, a.D, use);
+                __builtin_amdgcn_sched_barrier(0);
             }
         }
     }
@@ -460,45 +514,75 @@ __device__ inline void take_tile(const args &a, const key_walk<T> &walk, int til
     add_tile<T, DP, NT>(lk, lv, vis, __ballot(mine) == ~uint64_t{0}, a.c, w);
 }
 
-// The row's result, or its part of one.  l is whole here.
+// Where the lane's row starts, in `out` or among the parts; -1 if it has none.
 template <typename T, int DP>
-__device__ inline void close_rows(const args &a, int part, const row_state<T, DP> &w) {
-    if (!w.used) return;
-    const int half = (threadIdx.x & 63) >> 5;
+__device__ inline int64_t row_start(const args &a, int part, const row_state<T, DP> &w) {
+    if (!w.used) return -1;
+    if (!a.sums) return w.b * a.so.batch + w.t * a.so.row + w.h * a.so.head;
+    return (part * a.rows + (static_cast<int64_t>(w.b) * a.T + w.t) * a.H + w.h) * a.D;
+}
+
+// A part's reference and weight, by one lane of the row.
+__device__ inline void put_ml(const args &a, int64_t start, float m, float l) {
+    if (start < 0 || !a.sums) return;
+    a.ml[start / a.D * 2] = m;
+    a.ml[start / a.D * 2 + 1] = l;
+}
+
+// What a row's sums are multiplied by: a part's stay as they are; no key at all gives 0.
+__device__ inline float share_of(const args &a, float l) { return a.sums ? 1.0f : l == 0.0f ? 0.0f : 1.0f / l; }
+
+// Columns c..c + 3 of a row.
+template <typename T, bool DIRECT>
+__device__ inline void put4(const args &a, int64_t start, int c, f32x4 v) {
+    if (start < 0 || c >= a.D) return;
     if (a.sums) {
-        const int64_t row = (static_cast<int64_t>(part) * a.rows) + (static_cast<int64_t>(w.b) * a.T + w.t) * a.H + w.h;
-        float *to = a.sums + row * a.D;
-#pragma unroll
-        for (int d = 0; d < DP / 32; ++d)
-#pragma unroll
-            for (int g = 0; g < 4; ++g) {
-                const int at = 32 * d + 8 * g + 4 * half;
-#pragma unroll
-                for (int i = 0; i < 4; ++i)
-                    if (at + i < a.D) to[at + i] = w.o[d][4 * g + i];
-            }
-        if (half == 0) {
-            a.ml[row * 2] = w.m;
-            a.ml[row * 2 + 1] = w.l;
-        }
+        float *to = a.sums + start + c;
+        if (DIRECT || c + 4 <= a.D) std::memcpy(to, &v, 16);   // (DIRECT: D is a multiple of 4)
+        else
+            for (int j = 0; j < a.D - c; ++j) to[j] = v[j];
         return;
     }
-    const float by = w.l == 0.0f ? 0.0f : 1.0f / w.l;   // no key at all: 0
-    typename T::raw *to = static_cast<typename T::raw *>(a.out) + w.b * a.so.batch + w.t * a.so.row + w.h * a.so.head;
+    typename T::raw *to = static_cast<typename T::raw *>(a.out) + start + c, y[4];
 #pragma unroll
-    for (int d = 0; d < DP / 32; ++d)
+    for (int j = 0; j < 4; j += 2) T::store2(y + j, v[j], v[j + 1]);
+    if (DIRECT || c + 4 <= a.D) std::memcpy(to, y, sizeof(y));
+    else
+        for (int j = 0; j < a.D - c; ++j) to[j] = y[j];
+}
+
+// The wave's rows, or their part of them, to memory.  l is whole here.  A lane
+// holds a row's columns four by four; they go through LDS (`lds`, BYTES of the
+// wave's own), so that lanes next to each other write next to each other.
+template <typename T, int DP, int BYTES, bool DIRECT>
+__device__ inline void close_rows(const args &a, int part, row_state<T, DP> &w, unsigned char *lds) {
+    constexpr int kTurns = 32 * DP * 4 > BYTES ? 2 : 1, kCols = DP / kTurns, kPieces = kCols / 4;
+    static_assert(32 * kCols * 4 <= BYTES, "the columns of a turn fit");
+    const int lane = threadIdx.x & 63, half = lane >> 5, col = lane & 31;
+    const int64_t start = row_start<T, DP>(a, part, w);
+    if (half == 0) put_ml(a, start, w.m, w.l);
+    const float by = share_of(a, w.l);
 #pragma unroll
-        for (int g = 0; g < 4; ++g) {
-            const int at = 32 * d + 8 * g + 4 * half;
-            typename T::raw r[4];
+    for (int turn = 0; turn < kTurns; ++turn) {
 #pragma unroll
-            for (int i = 0; i < 4; i += 2) T::store2(r + i, w.o[d][4 * g + i] * by, w.o[d][4 * g + i + 1] * by);
-            if (at + 4 <= a.D) std::memcpy(to + at, r, sizeof(r));
-            else
+        for (int d = 0; d < kCols / 32; ++d)
 #pragma unroll
-                for (int i = 0; i < 4; ++i)
-                    if (at + i < a.D) to[at + i] = r[i];
+            for (int g = 0; g < 4; ++g) {
+                f32x4 v;
+#pragma unroll
+                for (int i = 0; i < 4; ++i) v[i] = w.o[turn * (kCols / 32) + d][4 * g + i] * by;
+                const int piece = 8 * d + 2 * g + half;
+                *reinterpret_cast<f32x4 *>(lds + (col * kPieces + (piece ^ (col & 15))) * 16) = v;
+            }
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+#pragma unroll 4
+        for (int i = 0; i < 32 * kPieces / 64; ++i) {
+            const int at = i * 64 + lane, r = at / kPieces, piece = at % kPieces;
+            const f32x4 v = *reinterpret_cast<const f32x4 *>(lds + (r * kPieces + (piece ^ (r & 15))) * 16);
+            put4<T, DIRECT>(a, __shfl(start, r), turn * kCols + piece * 4, v);
         }
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    }
 }
 
 // The most own keys that any row of the block (or wave) sees.
@@ -543,7 +627,7 @@ __device__ inline void rows_body(const args &a, const job &j, const place &at, u
     __shared__ int see[2][4];
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
     row_state<T, DP> w;
-    open_rows(a, j.walk, at.b, at.tile * 128 + wave * 32 + (lane & 31), at.hk, w);
+    open_rows<T, DP, DIRECT>(a, j.walk, at.b, at.tile * 128 + wave * 32 + (lane & 31), at.hk, w);
     const int high = most_of(w.see), low = least_of(w.used ? w.see : INT_MAX);
     if (lane == 0) {
         see[0][wave] = high;
@@ -571,7 +655,8 @@ __device__ inline void rows_body(const args &a, const job &j, const place &at, u
     }
     if (odd) add_odd(a, walk.v, walk.v_row, max(max(first, mixed) - walk.prefix_tiles, 0) * KT, (end - walk.prefix_tiles) * KT, w);
     w.l += __shfl_xor(w.l, 32);
-    close_rows(a, j.part + at.split, w);
+    __syncthreads();   // no tile is read any more
+    close_rows<T, DP, kTile, DIRECT>(a, j.part + at.split, w, lds + wave * kTile);
 }
 
 // Few rows: 32 a block; each of its first WAVES waves takes every WAVES-th
@@ -585,7 +670,7 @@ __device__ inline void keys_body(const args &a, const job &j, const place &at, u
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
     unsigned char *const own = lds + wave * 2 * kTile;
     row_state<T, DP> w;
-    open_rows(a, j.walk, at.b, at.tile * 32 + (lane & 31), at.hk, w);
+    open_rows<T, DP, DIRECT>(a, j.walk, at.b, at.tile * 32 + (lane & 31), at.hk, w);
     if (__ballot(w.used) == 0) return;   // the same for all waves
     key_walk<T> walk;
     const int most = __builtin_amdgcn_readfirstlane(most_of(w.see));
@@ -642,21 +727,25 @@ __device__ inline void keys_body(const args &a, const job &j, const place &at, u
         for (int d = 0; d < DP / 32; ++d) red[(wave * (DP / 32) + d) * 64 + lane] = w.o[d] * keep;
     }
     __syncthreads();
-    if (wave != 0) return;
+    // Each wave joins and writes a share of the columns.
+    const int64_t start = row_start<T, DP>(a, j.part + at.split, w);
+    const int half = lane >> 5;
+    if (wave == 0 && half == 0) put_ml(a, start, m, l);
+    const float by = share_of(a, l);
+#pragma unroll 1
+    for (int d = wave; d < DP / 32; d += 4) {
+        f32x16 o = red[d * 64 + lane];
 #pragma unroll
-    for (int d = 0; d < DP / 32; ++d) {
-        w.o[d] = red[d * 64 + lane];
+        for (int i = 1; i < WAVES; ++i) o += red[(i * (DP / 32) + d) * 64 + lane];
 #pragma unroll
-        for (int i = 1; i < WAVES; ++i) w.o[d] += red[(i * (DP / 32) + d) * 64 + lane];
+        for (int g = 0; g < 4; ++g)
+            put4<T, DIRECT>(a, start, 32 * d + 8 * g + 4 * half, f32x4{o[4 * g], o[4 * g + 1], o[4 * g + 2], o[4 * g + 3]} * by);
     }
-    w.m = m;
-    w.l = l;
-    close_rows(a, j.part + at.split, w);
 }
 
 // The blocks of one job, or of two at once, evenly mixed: a prefix's products
 // and the streams' own keys, which wait for memory, share the compute units.
-template <typename T, int DP, int NT, int WAVES, bool DIRECT>
+template <typename T, int DP, int NT, int WAVES, bool DIRECT, bool ROWS_ONLY>
 __global__ __launch_bounds__(256, sizeof(typename T::raw) * DP <= 256 ? 2 : 1) void attn_kernel(args a) {
     extern __shared__ __align__(16) unsigned char lds[];
     // Blocks are dealt to the eight dies in turn; each die gets a run of
@@ -667,7 +756,7 @@ __global__ __launch_bounds__(256, sizeof(typename T::raw) * DP <= 256 ? 2 : 1) v
     const int before = static_cast<int>(at * n0 / total), after = static_cast<int>((at + 1) * n0 / total);
     const job &j = after > before ? a.jobs[0] : a.jobs[1];
     const place p = place_of(a, j, after > before ? before : at - before);
-    if constexpr (WAVES > 0) {
+    if constexpr (WAVES > 0 && !ROWS_ONLY) {
         if (!j.many) {
             keys_body<T, DP, WAVES, DIRECT>(a, j, p, lds);
             return;
@@ -688,7 +777,9 @@ aq_status run(aq_ctx *ctx, const args &a) {
         if (need > lds) lds = need;
         blocks += j.blocks;
     }
-    auto kernel = a.direct ? attn_kernel<T, DP, NT, WAVES, true> : attn_kernel<T, DP, NT, WAVES, false>;
+    auto kernel = !a.direct ? attn_kernel<T, DP, NT, WAVES, false, false> : attn_kernel<T, DP, NT, WAVES, true, false>;
+    // Many rows alone have a kernel without the other kind of block, whose registers they do not need.
+    if (a.direct && a.jobs[0].many && !a.jobs[1].blocks) kernel = attn_kernel<T, DP, NT, WAVES, true, true>;
     aq_status st = aq_launch_lds(ctx, reinterpret_cast<const void *>(kernel), lds, "attention");
     if (st != AQ_OK) return st;
     aq_launch_timed(ctx, true, kernel, dim3(static_cast<uint32_t>(blocks)), dim3(256), lds, a);
