@@ -162,9 +162,10 @@ bool overlaps(const aq_heads &t, int64_t B, int64_t T, int64_t H, int64_t D) {
     return false;
 }
 
-// Rows that start and end at 16 bytes.
+// Rows that start and end at 16 bytes, with 64 of them within 2^31 bytes.
 bool pieces(const aq_heads &t, int64_t D, int64_t size) {
-    return reinterpret_cast<uintptr_t>(t.data) % 16 == 0 && D * size % 16 == 0 && t.batch_ld * size % 16 == 0 &&
+    return t.row_ld < (int64_t{1} << 25) / size &&
+           reinterpret_cast<uintptr_t>(t.data) % 16 == 0 && D * size % 16 == 0 && t.batch_ld * size % 16 == 0 &&
            t.row_ld * size % 16 == 0 && t.head_ld * size % 16 == 0;
 }
 

@@ -261,6 +261,12 @@ __device__ inline float add_values(const unsigned char *lv, f32x16 (&s)[NT], flo
     return sum;
 }
 
+// The larger of this lane's value and lane ^ 32's.
+__device__ inline float both_halves_max(float v) {
+    const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
+}
+
 // One tile of 32 NT keys from LDS.  vis: bit j is set where this lane's row
 // sees key j of each 32; all: every lane sees every key.
 template <typename T, int DP, int NT>
@@ -284,7 +290,7 @@ __device__ inline void add_tile(const unsigned char *lk, const unsigned char *lv
     for (int n = 0; n < NT; ++n)
 #pragma unroll
         for (int i = 0; i < 16; ++i) top = fmaxf(top, s[n][i]);
-    top = fmaxf(top, __shfl_xor(top, 32));
+    top = both_halves_max(top);
     // The sums' reference moves only when a row's maximum has outgrown it by
     // 2^kSlack: until then the weights are that much above 1 at most.
     // (Row by row: a row's result does not depend on its neighbours'.)
@@ -337,37 +343,46 @@ struct stager {
     using E = typename T::raw;
     static constexpr int kEach = KT * S::kPieces / THREADS;
 
-    static __device__ inline void piece(const E *from, unsigned char *to) {
+    static __device__ inline void piece(const void *from, unsigned char *to) {
         __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void *)from,
                                          (__attribute__((address_space(3))) void *)to, 16, 0, 0);
     }
 
-    // The keys of the tile that any row may see come back as bits.
+    // The keys of the tile that any row may see come back as bits.  wave: of
+    // the block's, the same for all its lanes (0 where a wave has the tile to
+    // itself).
     static __device__ inline uint64_t load(const args &a, const key_walk<T> &w, int tile, unsigned char *lk, unsigned char *lv,
-                                           int thread) {
+                                           int wave) {
         const bool pre = tile < w.prefix_tiles;
         const int j0 = (pre ? tile : tile - w.prefix_tiles) * KT, n = (pre ? w.P : w.own) - j0;
         uint64_t bits = n >= 64 ? ~uint64_t{0} : (uint64_t{1} << n) - 1;
-        const int lane = threadIdx.x & 63;
+        const int lane = threadIdx.x & 63, thread = wave * 64 + lane;
         if (!pre && w.mask) bits &= __ballot(lane < n && w.mask[j0 + min(lane, n - 1)] != 0);
         const int64_t kr = pre ? w.pk_row : w.k_row, vr = pre ? w.pv_row : w.v_row;
         const E *kp = (pre ? w.pk : w.k) + j0 * kr, *vp = (pre ? w.pv : w.v) + j0 * vr;
         if constexpr (DIRECT) {
-            unsigned char *const k0 = lk + (thread - lane) * 16, *const v0 = lv + (thread - lane) * 16;
+            unsigned char *const k0 = lk + wave * 1024, *const v0 = lv + wave * 1024;
             constexpr uint64_t kAll = KT == 64 ? ~uint64_t{0} : (uint64_t{1} << (KT % 64)) - 1;
-            const bool whole = (bits & kAll) == kAll && a.D == DP;
+            // Offsets within a tile fit 32 bits (the host saw to it), so a
+            // piece's address is one multiplication.
+            const uint32_t kb = static_cast<uint32_t>(kr * sizeof(E)), vb = static_cast<uint32_t>(vr * sizeof(E));
+            if ((bits & kAll) == kAll && a.D == DP) {
 #pragma unroll
-            for (int i = 0; i < kEach; ++i) {
-                const int at = i * THREADS + thread, key = at / S::kPieces, place = at % S::kPieces;
-                const int pk = (place ^ S::swz_k(key)) * S::kPer, pv = (place ^ S::swz_v(key)) * S::kPer;
-                const E *kg = kp + key * kr + pk, *vg = vp + key * vr + pv;
-                if (!whole) {
-                    const E *const none = reinterpret_cast<const E *>(&kZeros);
-                    if (!(bits >> key & 1) || pk >= a.D) kg = none;
-                    if (!(bits >> key & 1) || pv >= a.D) vg = none;
+                for (int i = 0; i < kEach; ++i) {
+                    const uint32_t at = i * THREADS + thread, key = at / S::kPieces, place = at % S::kPieces;
+                    piece(reinterpret_cast<const char *>(kp) + (key * kb + ((place ^ S::swz_k(key)) << 4)), k0 + i * THREADS * 16);
+                    piece(reinterpret_cast<const char *>(vp) + (key * vb + ((place ^ S::swz_v(key)) << 4)), v0 + i * THREADS * 16);
                 }
-                piece(kg, k0 + i * THREADS * 16);
-                piece(vg, v0 + i * THREADS * 16);
+            } else {
+#pragma unroll
+                for (int i = 0; i < kEach; ++i) {
+                    const uint32_t at = i * THREADS + thread, key = at / S::kPieces, place = at % S::kPieces;
+                    const uint32_t pk = place ^ S::swz_k(key), pv = place ^ S::swz_v(key), end = a.D / S::kPer;
+                    const bool use = bits >> key & 1;
+                    const void *none = &kZeros;
+                    piece(use && pk < end ? reinterpret_cast<const char *>(kp) + (key * kb + (pk << 4)) : none, k0 + i * THREADS * 16);
+                    piece(use && pv < end ? reinterpret_cast<const char *>(vp) + (key * vb + (pv << 4)) : none, v0 + i * THREADS * 16);
+                }
             }
         } else {
 #pragma unroll 4
@@ -642,14 +657,14 @@ __device__ inline void rows_body(const args &a, const job &j, const place &at, u
     const int per = (tiles + j.splits - 1) / j.splits, first = at.split * per, end = min(tiles, first + per);
     uint64_t bits = 0;
     bool odd = false;
-    if (first < end) bits = stage::load(a, walk, first, lds, lds + kTile, threadIdx.x);
+    if (first < end) bits = stage::load(a, walk, first, lds, lds + kTile, wave);
 #pragma unroll 1
     for (int tile = first; tile < end; ++tile) {
         unsigned char *const now = lds + ((tile - first) & 1) * 2 * kTile, *const then = lds + ((tile - first + 1) & 1) * 2 * kTile;
         landed();
         __syncthreads();   // the tile is there, and all waves are done with the one before
         const uint64_t use = bits;
-        if (tile + 1 < end) bits = stage::load(a, walk, tile + 1, then, then + kTile, threadIdx.x);
+        if (tile + 1 < end) bits = stage::load(a, walk, tile + 1, then, then + kTile, wave);
         if (tile >= mixed) odd |= __syncthreads_or(hide_odd<T, DP, KT, 256>(now + kTile, threadIdx.x)) != 0;
         take_tile<T, DP, NT>(a, walk, tile, use, now, now + kTile, w);
     }
@@ -694,7 +709,7 @@ __device__ inline void keys_body(const args &a, const job &j, const place &at, u
             if (tile + WAVES < end) next.load(a, walk, tile + WAVES, lane);
         } else {
             landed();   // the last tile's reads, before this one takes the place
-            bits = stager<T, DP, KT, 64, DIRECT>::load(a, walk, tile, own, own + kTile, lane);
+            bits = stager<T, DP, KT, 64, DIRECT>::load(a, walk, tile, own, own + kTile, 0);
             landed();
             __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
         }
