@@ -153,9 +153,10 @@ __device__ inline void open_rows(const args &a, int walk, int b0, int r, int hk,
 
 // Steps of a chain of products whose operands come from LDS: kAhead of them are
 // on their way before the first is used.  The scheduling barriers keep it so;
-// left alone, the compiler loads each next to its use, or all at once.
-// (One row tile's products next to a tile on its way leave room for two.)
-template <int NT> constexpr int kAheadSteps = NT > 1 ? 4 : 2;
+// left alone, the compiler loads each next to its use, or all at once.  Tiles
+// of 32 keys are left to it: there the registers hold a tile on its way, and
+// what a ring takes more is spilled (64 streams over 1500 keys: 65 us, 61 so).
+template <int NT> constexpr int kAheadSteps = NT > 1 ? 4 : 0;
 
 // S^T for a tile of 32 NT keys: s[n] += K q.
 template <typename T, int DP, int NT>
@@ -177,7 +178,7 @@ __device__ inline void add_scores(const unsigned char *lk, f32x16 (&s)[NT], cons
 #pragma unroll
     for (int e = 0; e < kSteps; ++e) {
         if (e + kAhead < kSteps) ring[(e + kAhead) % kRing] = piece(e + kAhead);
-        __builtin_amdgcn_sched_barrier(0);
+        if (kAhead) __builtin_amdgcn_sched_barrier(0);
         const u32x4 k = ring[e % kRing];
         if constexpr (S::kF32) {
 #pragma unroll
@@ -249,7 +250,7 @@ __device__ inline float add_values(const unsigned char *lv, f32x16 (&s)[NT], flo
         for (int e = 0; e < kSteps; ++e) {
             const int g = e / kD, d = e % kD;
             if (e + kAhead < kSteps) ring[(e + kAhead) % kRing] = values(e + kAhead);
-            __builtin_amdgcn_sched_barrier(0);
+            if (kAhead) __builtin_amdgcn_sched_barrier(0);
             w.o[d] = mma(T(), ring[e % kRing], p, w.o[d]);
             if (g + 1 < kGroups) {
 #pragma unroll
@@ -760,7 +761,9 @@ __device__ inline void keys_body(const args &a, const job &j, const place &at, u
 
 // The blocks of one job, or of two at once, evenly mixed: a prefix's products
 // and the streams' own keys, which wait for memory, share the compute units.
-template <typename T, int DP, int NT, int WAVES, bool DIRECT, bool ROWS_ONLY>
+// KINDS: the kinds of blocks that the launch has (1: many rows, 2: few); a kind
+// alone has its registers to itself.
+template <typename T, int DP, int NT, int WAVES, bool DIRECT, int KINDS>
 __global__ __launch_bounds__(256, sizeof(typename T::raw) * DP <= 256 ? 2 : 1) void attn_kernel(args a) {
     extern __shared__ __align__(16) unsigned char lds[];
     // Blocks are dealt to the eight dies in turn; each die gets a run of
@@ -771,13 +774,13 @@ __global__ __launch_bounds__(256, sizeof(typename T::raw) * DP <= 256 ? 2 : 1) v
     const int before = static_cast<int>(at * n0 / total), after = static_cast<int>((at + 1) * n0 / total);
     const job &j = after > before ? a.jobs[0] : a.jobs[1];
     const place p = place_of(a, j, after > before ? before : at - before);
-    if constexpr (WAVES > 0 && !ROWS_ONLY) {
-        if (!j.many) {
+    if constexpr ((KINDS & 2) != 0) {
+        if (KINDS == 2 || !j.many) {
             keys_body<T, DP, WAVES, DIRECT>(a, j, p, lds);
             return;
         }
     }
-    rows_body<T, DP, NT, DIRECT>(a, j, p, lds);
+    if constexpr ((KINDS & 1) != 0) rows_body<T, DP, NT, DIRECT>(a, j, p, lds);
 }
 
 template <typename T, int DP, int NT, int WAVES>
@@ -786,15 +789,19 @@ aq_status run(aq_ctx *ctx, const args &a) {
     static_assert(kKeys >= WAVES * 32 * DP * 4, "the waves' sums fit where the tiles were");
     uint32_t lds = 0;
     int64_t blocks = 0;
+    int kinds = 0;
     for (const job &j : a.jobs) {
         if (!j.blocks) continue;
+        kinds |= j.many ? 1 : 2;
         const uint32_t need = j.many ? kRows : kKeys;
         if (need > lds) lds = need;
         blocks += j.blocks;
     }
-    auto kernel = !a.direct ? attn_kernel<T, DP, NT, WAVES, false, false> : attn_kernel<T, DP, NT, WAVES, true, false>;
-    // Many rows alone have a kernel without the other kind of block, whose registers they do not need.
-    if (a.direct && a.jobs[0].many && !a.jobs[1].blocks) kernel = attn_kernel<T, DP, NT, WAVES, true, true>;
+    auto kernel = a.direct ? attn_kernel<T, DP, NT, WAVES, true, 1> : attn_kernel<T, DP, NT, WAVES, false, 1>;
+    if constexpr (WAVES > 0) {
+        if (kinds == 2) kernel = a.direct ? attn_kernel<T, DP, NT, WAVES, true, 2> : attn_kernel<T, DP, NT, WAVES, false, 2>;
+        if (kinds == 3) kernel = a.direct ? attn_kernel<T, DP, NT, WAVES, true, 3> : attn_kernel<T, DP, NT, WAVES, false, 3>;
+    }
     aq_status st = aq_launch_lds(ctx, reinterpret_cast<const void *>(kernel), lds, "attention");
     if (st != AQ_OK) return st;
     aq_launch_timed(ctx, true, kernel, dim3(static_cast<uint32_t>(blocks)), dim3(256), lds, a);
