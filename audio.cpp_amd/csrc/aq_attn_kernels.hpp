@@ -487,17 +487,20 @@ __device__ inline bool hide_odd(unsigned char *lv, int thread) {
     return odd;
 }
 
-// The values that hide_odd() took out of own keys first to end, to the rows
-// that see them.  A weight is above 0 and its product with such a value is
-// that value again, which no finite sum changes: it is added as it is.
+// The values that hide_odd() took out of own keys, to the rows that see them;
+// first and end count from the walk's start, in tiles of `tile` keys.  A weight
+// is above 0 and its product with such a value is that value again, which no
+// finite sum changes: it is added as it is.
 template <typename T, int DP>
-__device__ inline void add_odd(const args &a, const typename T::raw *v, int64_t v_row, int first, int end, row_state<T, DP> &w) {
+__device__ inline void add_odd(const args &a, const key_walk<T> &walk, int first, int end, int tile, row_state<T, DP> &w) {
+    first -= walk.prefix_tiles * tile;
+    end = min(end - walk.prefix_tiles * tile, walk.own);   // no key past those that a row sees is read
     const int half = (threadIdx.x & 63) >> 5;
 #pragma unroll 1
     for (int key = first; key < end; ++key) {
         int D = key < w.see ? a.D : 0;
         asm("" : "+v"(D));   // (compared anew for each key: 16 DP / 32 comparisons kept over the loop fill the scalar registers)
-        const typename T::raw *row = v + key * v_row;
+        const typename T::raw *row = walk.v + key * walk.v_row;
 #pragma unroll
         for (int d = 0; d < DP / 32; ++d) {
 #pragma unroll
@@ -615,18 +618,19 @@ __device__ inline int least_of(int see) {
     return see;
 }
 
-// Where a block stands in its job.  The key head is outermost, so that blocks
-// near each other share a prefix; the streams' order comes next.
+// Where a block stands in its job.  Row tiles are next to each other, since
+// they read the same keys; the key head is outermost, so that blocks near each
+// other share a prefix.
 struct place {
     int hk, b, tile, split;   // b: 0 for the prefix alone
 };
 
 __device__ inline place place_of(const args &a, const job &j, int at) {
     place p;
-    p.split = at % j.splits;
-    at /= j.splits;
     p.tile = at % j.tiles;
     at /= j.tiles;
+    p.split = at % j.splits;
+    at /= j.splits;
     const int streams = j.walk == kPrefix ? 1 : a.B;
     p.b = at % streams;
     p.hk = at / streams;
@@ -669,7 +673,7 @@ __device__ inline void rows_body(const args &a, const job &j, const place &at, u
         if (tile >= mixed) odd |= __syncthreads_or(hide_odd<T, DP, KT, 256>(now + kTile, threadIdx.x)) != 0;
         take_tile<T, DP, NT>(a, walk, tile, use, now, now + kTile, w);
     }
-    if (odd) add_odd(a, walk.v, walk.v_row, max(max(first, mixed) - walk.prefix_tiles, 0) * KT, (end - walk.prefix_tiles) * KT, w);
+    if (odd) add_odd(a, walk, max(first, mixed) * KT, end * KT, KT, w);
     w.l += __shfl_xor(w.l, 32);
     __syncthreads();   // no tile is read any more
     close_rows<T, DP, kTile, DIRECT>(a, j.part + at.split, w, lds + wave * kTile);
@@ -723,7 +727,7 @@ __device__ inline void keys_body(const args &a, const job &j, const place &at, u
     }
     if (odd)   // of this wave's tiles
         for (tile = first + wave; tile < end; tile += WAVES)
-            if (tile >= mixed) add_odd(a, walk.v, walk.v_row, (tile - walk.prefix_tiles) * KT, (tile - walk.prefix_tiles + 1) * KT, w);
+            if (tile >= mixed) add_odd(a, walk, tile * KT, (tile + 1) * KT, KT, w);
     w.l += __shfl_xor(w.l, 32);
     if (wave < WAVES && lane < 32) {
         ml[wave][0][lane] = w.m;
@@ -767,13 +771,19 @@ template <typename T, int DP, int NT, int WAVES, bool DIRECT, int KINDS>
 __global__ __launch_bounds__(256, sizeof(typename T::raw) * DP <= 256 ? 2 : 1) void attn_kernel(args a) {
     extern __shared__ __align__(16) unsigned char lds[];
     // Blocks are dealt to the eight dies in turn; each die gets a run of
-    // neighbours, which share keys, and so its cache serves them.
-    const int total = gridDim.x, die = blockIdx.x % 8;
-    const int at = die * (total / 8) + min(die, total % 8) + blockIdx.x / 8;
-    const int64_t n0 = a.jobs[0].blocks;
-    const int before = static_cast<int>(at * n0 / total), after = static_cast<int>((at + 1) * n0 / total);
-    const job &j = after > before ? a.jobs[0] : a.jobs[1];
-    const place p = place_of(a, j, after > before ? before : at - before);
+    // neighbours of either job, which share keys, and so its cache serves
+    // them.  Within a die the two jobs alternate while both last.
+    const int die = blockIdx.x % 8, n = blockIdx.x / 8;
+    const int n0 = a.jobs[0].blocks, n1 = a.jobs[1].blocks, more0 = n0 % 8, more1 = n1 % 8;
+    const int mine0 = n0 / 8 + (die < more0), mine1 = n1 / 8 + ((die + 8 - more0) % 8 < more1);
+    int from1 = 0;   // the second job's blocks of the dies before: its remainder goes to the dies that the first's left out
+    for (int d = 0; d < die; ++d) from1 += n1 / 8 + ((d + 8 - more0) % 8 < more1);
+    const int both = 2 * min(mine0, mine1);
+    const bool one = n < both ? n % 2 == 0 : mine0 > mine1;
+    const int nth = n < both ? n / 2 : n - both / 2;
+    const job &j = one ? a.jobs[0] : a.jobs[1];
+    const int at = one ? n0 / 8 * die + min(die, more0) + nth : from1 + nth;
+    const place p = place_of(a, j, at);
     if constexpr ((KINDS & 2) != 0) {
         if (KINDS == 2 || !j.many) {
             keys_body<T, DP, WAVES, DIRECT>(a, j, p, lds);

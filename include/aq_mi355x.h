@@ -612,7 +612,7 @@ typedef struct aq_heads {
  *            nearest inside
  *   mask     device, [B, S] bytes with row stride mask_ld (0: one for all
  *            streams), or NULL
- *   scale    above 0
+ *   scale    above 0, below 1e38
  * D from 1 to 256, S up to 2^30, B * T * heads up to 2^30, and fewer than 2^24
  * blocks of 32 rows of one stream and key head (128 from 33 rows on).  Scores, sums and
  * weights are fp32; with 16-bit types each p is rounded to the type before it
