@@ -181,7 +181,7 @@ aq_status checked(aq_ctx *ctx, const char *name, int type, int64_t B, int64_t T,
         return aq_fail(ctx, AQ_E_INVALID_ARG, "%s: type %d is not F32, F16 or BF16", name, type);
     if (!(scale > 0.0f) || !(scale < 1e38f))
         return aq_fail(ctx, AQ_E_INVALID_ARG, "%s: scale %g is not above 0 and below 1e38", name, static_cast<double>(scale));
-    if (B < 0 || T < 0 || keys < 0 || S < 0 || keys > kMost || S > kMost || heads < 1 || kv_heads < 1 || heads > kMost ||
+    if (B < 0 || T < 0 || keys < 0 || S < 0 || keys > kMost || S > kMost || keys + S > kMost || heads < 1 || kv_heads < 1 || heads > kMost ||
         heads % kv_heads != 0 || D < 1 || D > 256)
         return aq_fail(ctx, AQ_E_SHAPE, "%s: B=%lld T=%lld keys=%lld + %lld (up to 2^30) heads=%lld kv_heads=%lld D=%lld (1 to 256)",
                        name, (long long)B, (long long)T, (long long)keys, (long long)S, (long long)heads, (long long)kv_heads,
