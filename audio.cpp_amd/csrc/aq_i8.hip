@@ -443,8 +443,9 @@ void launch_quantize(aq_ctx *ctx, const void *x, int64_t x_ld, const args &a, i3
                         rows, x_ld, a.M, a.K, a.kblocks, to, scales);
 }
 
-// Rows of x at a time in operand order: 64 MB of them, but at least 64.
-constexpr int64_t kPackedBytes = int64_t{64} << 20;
+// Rows of x at a time in operand order: 64 MB of them, but at least 64, and no
+// more than a grid's second axis takes of 16.
+constexpr int64_t kPackedBytes = int64_t{64} << 20, kPackedRows = int64_t{1} << 19;
 
 void free_all(aq_i8 *w) {
     for (void *p : {static_cast<void *>(w->w), static_cast<void *>(w->scale), static_cast<void *>(w->bias)})
@@ -527,6 +528,7 @@ aq_status aq_i8_forward(aq_ctx *ctx, const aq_i8 *w, int x_type, const void *x, 
     if (x_type == AQ_T_I8 && (h == kSplit ? M <= 16 : pieces)) return launch_product<false>(ctx, a, h);
     int64_t rows = kPackedBytes / (int64_t{w->kblocks} * 64) / 64 * 64;
     if (rows < 64) rows = 64;
+    if (rows > kPackedRows) rows = kPackedRows;
     if (rows > (M + 15) / 16 * 16) rows = (M + 15) / 16 * 16;
     const size_t bytes = static_cast<size_t>(rows) * static_cast<size_t>(w->kblocks) * 64;
     uint8_t *packed = nullptr;
