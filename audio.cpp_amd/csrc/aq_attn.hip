@@ -36,20 +36,25 @@ __global__ __launch_bounds__(256) void attn_join_kernel(join_args a) {
     for (int d = 32; d; d >>= 1) m = fmaxf(m, __shfl_xor(m, d));
     const float from = m == -INFINITY ? 0.0f : m;
     float l = 0.0f, o[4] = {};
-#pragma unroll 4
-    for (int p = set; p < a.parts; p += kAt) {
+    const auto add = [&](int p, auto load) {
         const int64_t row = p * a.rows + r;
         const float by = __builtin_amdgcn_exp2f(a.ml[row * 2] - from);
         l = __fmaf_rn(a.ml[row * 2 + 1], by, l);
-        float v[4] = {};
-        const float *sums = a.sums + row * a.D + at;
-        if (at + 4 <= a.D) std::memcpy(v, sums, 16);
-        else
-#pragma unroll
-            for (int i = 0; i < 4; ++i)
-                if (at + i < a.D) v[i] = sums[i];
+        float v[4];
+        load(a.sums + row * a.D, v);
 #pragma unroll
         for (int i = 0; i < 4; ++i) o[i] = __fmaf_rn(v[i], by, o[i]);
+    };
+    if (a.D % 4 == 0) {   // one load each without a condition (lanes past the end repeat the last): several are on their way
+        const int from4 = min(at, a.D - 4);
+#pragma unroll 8
+        for (int p = set; p < a.parts; p += kAt) add(p, [&](const float *sums, float(&v)[4]) { std::memcpy(v, sums + from4, 16); });
+    } else {
+        for (int p = set; p < a.parts; p += kAt)
+            add(p, [&](const float *sums, float(&v)[4]) {
+#pragma unroll
+                for (int i = 0; i < 4; ++i) v[i] = sums[min(at + i, a.D - 1)];
+            });
     }
 #pragma unroll
     for (int d = LANES; d < 64; d <<= 1) {
@@ -57,7 +62,7 @@ __global__ __launch_bounds__(256) void attn_join_kernel(join_args a) {
 #pragma unroll
         for (int i = 0; i < 4; ++i) o[i] += __shfl_xor(o[i], d);
     }
-    if (set != 0) return;
+    if (set != 0 || at >= a.D) return;
     const float by = l == 0.0f ? 0.0f : 1.0f / l;
     typename T::raw *to = static_cast<typename T::raw *>(a.out) + b * a.batch + t * a.row + h * a.head + at;
     typename T::raw y[4];
