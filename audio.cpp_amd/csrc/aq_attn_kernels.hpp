@@ -22,6 +22,17 @@
 // the keys averages); an f16 p is 2^10 times the weight, so that small weights
 // are not lost below its range.  fp32 inputs keep fp32 products throughout.
 //
+// What bounds it.  Many rows: 860 to 990 TFLOP/s (8 x 4096 rows of 16 heads over
+// 1500 keys in 449 us, 16 x 512 rows over a prefix of 8192 in 572), where a
+// large product of the library's reaches 1110 to 1270 on the same card: the
+// matrix instructions 39 % of the clocks and the vector instructions (two thirds
+// of them for the exponentials) as much, two waves a SIMD (227 registers) that
+// cover each other's waits.  Few rows, the keys' way from memory: 64 streams over
+// 1500 keys, 266 MB, 55 us (4.8 TB/s).  Both at once, a token of 128 streams
+// over 16384 shared and up to 1024 own keys: 127 us, of which the own keys'
+// 368 MB take 75 and the prefix 49 alone; side by side they gain little, as the
+// prefix's four row tiles read it again past what the own keys leave of the caches.
+//
 // A key that a row does not see is never multiplied into it: its score is
 // -infinity whatever the product gave, keys that no row of the tile sees are
 // zeros in LDS, and where a causal tile that some rows see in part holds values
@@ -278,6 +289,10 @@ __device__ inline void add_tile(const unsigned char *lk, const unsigned char *lv
     const int half = (threadIdx.x & 63) >> 5;
     f32x16 s[NT];
     add_scores<T, DP, NT>(lk, s, w);
+    // Of a SIMD's two waves the one with exponentials and products to mix goes
+    // first, the one with products alone fills what is left (8 x 4096 rows over
+    // 1500 keys: 462 -> 449 us, 16 x 512 over 8192 + 512: 598 -> 573).
+    if (NT > 1) __builtin_amdgcn_s_setprio(1);
     if (!all) {
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
@@ -304,6 +319,7 @@ __device__ inline void add_tile(const unsigned char *lk, const unsigned char *lv
         for (int d = 0; d < DP / 32; ++d) w.o[d] *= keep;
     }
     w.l += add_values<T, DP, NT>(lv, s, c, (w.m == -INFINITY ? 0.0f : w.m) - kShift, w);
+    if (NT > 1) __builtin_amdgcn_s_setprio(0);
 }
 
 // The keys that a walk meets one after the other: the prefix's tiles, then the
