@@ -24,9 +24,9 @@
 //
 // What bounds it.  Many rows: 860 to 990 TFLOP/s (8 x 4096 rows of 16 heads over
 // 1500 keys in 449 us, 16 x 512 rows over a prefix of 8192 in 572), where a
-// large product of the library's reaches 1110 to 1270 on the same card: the
-// matrix instructions 39 % of the clocks and the vector instructions (two thirds
-// of them for the exponentials) as much, two waves a SIMD (227 registers) that
+// large product of the library's reaches 1110 to 1270: the matrix instructions
+// 45 % of the clocks and the vector instructions (two thirds of them for the
+// exponentials) 51 %, on two waves a SIMD (227 registers) that
 // cover each other's waits.  Few rows, the keys' way from memory: 64 streams over
 // 1500 keys, 266 MB, 55 us (4.8 TB/s).  Both at once, a token of 128 streams
 // over 16384 shared and up to 1024 own keys: 127 us, of which the own keys'
