@@ -88,14 +88,14 @@ constexpr int64_t kPartBytes = int64_t{256} << 20;
 
 int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
 
-// A job over `rows` rows (of each of `groups` groups) and `keys` keys: in how
-// many parts the keys are taken so that the card is full.
-aq_attn_impl::job job_of(const aq_ctx *ctx, int walk, int type, int D, int64_t groups, int64_t rows, int64_t keys, int64_t most_parts) {
+// A job over `rows` rows (of each of `groups` groups) and `keys` keys: the keys
+// are taken in so many parts that there are `want` blocks.
+aq_attn_impl::job job_of(int64_t want, int walk, int type, int D, int64_t groups, int64_t rows, int64_t keys, int64_t most_parts) {
     aq_attn_impl::job j{};
     j.walk = walk;
     j.many = rows > 32 || (type == AQ_T_F32 && D > 128);   // (such rows have the first kind of block only)
     j.tiles = static_cast<int>(ceil_div(rows, j.many ? 128 : 32));
-    const int64_t blocks = groups * j.tiles, want = 2 * ctx->num_cus;
+    const int64_t blocks = groups * j.tiles;
     // At least this many keys a part: fp32 products are slow enough for one
     // tile (5 x 23 rows over 701 + 211 keys: 25 us, 30 with 128 keys a part,
     // 61 with 512); 16-bit ones are not worth the joining.
@@ -115,13 +115,22 @@ aq_status attend(aq_ctx *ctx, int type, args a) {
     // not fill a tile of rows; then its own keys are a part of their own.
     const bool apart = a.P > 0 && a.B > 1 && per_stream < 64 && most_parts >= 2;
     int parts;
+    // A compute unit holds two blocks.  A prefix's jobs share it with the own
+    // keys', and each of its parts is written and joined: one block a unit, and
+    // three for four units where the own keys outnumber the prefix's.  In us,
+    // one token, 32/8 heads of 128, for 192, 256 and 512 blocks: 128 streams over
+    // 16384 + 1024 keys 124, 134, 129; over 4096 + 1024 94, 97, 105; over 65536 +
+    // 64 313, 256, 268; 32 streams over 16384 + 1024 51, 54, 65; over 16384 + 16
+    // 38, 37, 51.
+    const int64_t full = 2 * ctx->num_cus;
+    const int64_t beside = static_cast<int64_t>(a.B) * a.S >= a.P ? ctx->num_cus * 3 / 4 : ctx->num_cus;
     if (apart) {
-        a.jobs[0] = job_of(ctx, aq_attn_impl::kPrefix, type, a.D, a.Hkv, per_stream * a.B, a.P, most_parts / 2);
-        a.jobs[1] = job_of(ctx, aq_attn_impl::kOwn, type, a.D, heads, per_stream, a.S, most_parts / 2);
+        a.jobs[0] = job_of(beside, aq_attn_impl::kPrefix, type, a.D, a.Hkv, per_stream * a.B, a.P, most_parts / 2);
+        a.jobs[1] = job_of(full, aq_attn_impl::kOwn, type, a.D, heads, per_stream, a.S, most_parts / 2);
         a.jobs[1].part = a.jobs[0].splits;
         parts = a.jobs[0].splits + a.jobs[1].splits;
     } else {
-        a.jobs[0] = job_of(ctx, aq_attn_impl::kBoth, type, a.D, heads, per_stream, static_cast<int64_t>(a.P) + a.S, most_parts);
+        a.jobs[0] = job_of(full, aq_attn_impl::kBoth, type, a.D, heads, per_stream, static_cast<int64_t>(a.P) + a.S, most_parts);
         parts = a.jobs[0].splits;
     }
     if (int64_t{a.jobs[0].blocks} + a.jobs[1].blocks >= int64_t{1} << 24)

@@ -29,7 +29,7 @@
 // exponentials) 51 %, on two waves a SIMD (227 registers) that
 // cover each other's waits.  Few rows, the keys' way from memory: 64 streams over
 // 1500 keys, 266 MB, 55 us (4.8 TB/s).  Both at once, a token of 128 streams
-// over 16384 shared and up to 1024 own keys: 127 us, of which the own keys'
+// over 16384 shared and up to 1024 own keys: 122 us, of which the own keys'
 // 368 MB take 75 and the prefix 49 alone; side by side they gain little, as the
 // prefix's four row tiles read it again past what the own keys leave of the caches.
 //
@@ -419,8 +419,8 @@ struct stager {
 // The same through registers, for a tile that one wave has to itself: the next
 // tile's pieces are on their way in registers while one is used.  Such keys are
 // read once, so they are the first to leave the caches: a prefix stays there
-// (a token of 128 streams over 16384 + 1024 keys: 136 us with plain loads, 123
-// so; of 64 streams over 1500 keys, 60 and 55).
+// (a token of 128 streams over 16384 + 1024 keys: 137 us with plain loads, 130
+// so; of 64 streams over 1500 keys, 61 and 55).
 template <typename T, int DP, int KT, bool DIRECT>
 struct carrier {
     using S = shape<T, DP>;
