@@ -122,7 +122,13 @@ aq_status attend(aq_ctx *ctx, int type, args a) {
     // 16384 + 1024 keys 124, 134, 129; over 4096 + 1024 94, 97, 105; over 65536 +
     // 64 313, 256, 268; 32 streams over 16384 + 1024 51, 54, 65; over 16384 + 16
     // 38, 37, 51.
-    const int64_t full = 2 * ctx->num_cus;
+    // Other jobs: one block a unit too (in us, with 256 and 512 blocks: one row
+    // of 32/8 heads over 65536 keys 54, 58; 4 streams over 8192 31, 34; 16 rows of
+    // 2 streams over 8192 28, 31; fp32, of which a unit holds one block, 200 rows
+    // over 2000 54, 65), but two where so many 16-bit rows share each key that
+    // products bound it (512 rows of 8 heads over 16384: 59, 54).
+    const bool wide = per_stream > 256 && type != AQ_T_F32 && a.D <= 128;
+    const int64_t full = wide ? 2 * ctx->num_cus : ctx->num_cus;
     const int64_t beside = static_cast<int64_t>(a.B) * a.S >= a.P ? ctx->num_cus * 3 / 4 : ctx->num_cus;
     if (apart) {
         a.jobs[0] = job_of(beside, aq_attn_impl::kPrefix, type, a.D, a.Hkv, per_stream * a.B, a.P, most_parts / 2);
