@@ -17,8 +17,8 @@
 // lane (fp32).  A row's m, l and rescaling are plain registers; one exchange
 // per tile joins the two halves' maxima.
 //
-// Scores, m, l and o are fp32.  p is rounded to the 16-bit type of v (half a
-// step of 2^-9, 2^-12 for f16, with errors of either sign that the sum over
+// Scores, m, l and o are fp32.  p is rounded to the 16-bit type of v (by at most
+// 2^-8 of itself, 2^-11 for f16, with errors of either sign that the sum over
 // the keys averages); an f16 p is 2^10 times the weight, so that small weights
 // are not lost below its range.  fp32 inputs keep fp32 products throughout.
 //

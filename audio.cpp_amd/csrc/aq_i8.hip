@@ -8,7 +8,7 @@
 // has the same layout, by 16 rows of x.
 //
 // What bounds it.  Few rows of x, the weights' way from memory: 64 x 8192 x
-// 16384, 134 MB, 32 us (4.2 TB/s; 40 with bringing bf16 rows to 8 bits).  Many
+// 16384, 134 MB, 27 us (5.0 TB/s; 36 with bringing bf16 rows to 8 bits).  Many
 // rows, the matrix instructions: 16384 x 8192 x 8192 in 1.04 ms, 2.1 POP/s, as
 // fast as the library's product of whole numbers.  One row of 1024 x 1536: 3 us
 // in the kernel, latency of the loads, of the join and of the launch.
@@ -424,8 +424,14 @@ aq_status launch_product(aq_ctx *ctx, const args &a, how h) {
         return launch<false, 1, 1, 4>(ctx, a, 8);
     } else {
         if (a.M <= 16) return launch<true, 1, 1, 4>(ctx, a, 8);
-        if (a.M <= 32) return launch<true, 2, 2, 2>(ctx, a, 8);
-        return launch<true, 4, 4, 1>(ctx, a, 4);
+        // Four tiles by 64 rows read the weights once for them, where there are
+        // enough such blocks; in us, two tiles by 32 rows and these with eight and
+        // with four waves: 64 x 8192 x 16384, packing
+        // included, 47, 35, 40; 128 rows 83, 58, 47;
+        // 64 x 4096 x 4096 11.6, 12.3, 14.5; 64 x 8192 x 2048 11.5, 17, 22.
+        const int64_t blocks = int64_t{(a.tiles + 3) / 4} * ((a.M + 63) / 64);
+        if (a.M <= 32 || blocks < ctx->num_cus) return launch<true, 2, 2, 2>(ctx, a, 8);
+        return launch<true, 4, 4, 1>(ctx, a, a.M <= 64 ? 8 : 4);
     }
 }
 

@@ -652,7 +652,7 @@ typedef struct aq_heads {
  * blocks of 32 rows of one stream and key head (128 from 33 rows on).  Scores, sums and
  * weights are fp32; with 16-bit types each p is rounded to the type before it
  * meets v, an F32 call is fp32 throughout.  The order of a row's sum depends
- * on the sizes alone, not on timing.  Calls of few rows use the context's
+ * on the sizes and lengths alone, not on timing.  Calls of few rows use the context's
  * scratch. */
 aq_status aq_cross_attention(aq_ctx *ctx, int type, int64_t B, int64_t T, int64_t S, int64_t heads, int64_t kv_heads, int64_t D,
                              aq_heads q, aq_heads k, aq_heads v, const int32_t *q_len, const int32_t *kv_len,
