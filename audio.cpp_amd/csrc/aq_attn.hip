@@ -93,13 +93,16 @@ int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
 aq_attn_impl::job job_of(int64_t want, int walk, int type, int D, int64_t groups, int64_t rows, int64_t keys, int64_t most_parts) {
     aq_attn_impl::job j{};
     j.walk = walk;
-    j.many = rows > 32 || (type == AQ_T_F32 && D > 128);   // (such rows have the first kind of block only)
+    // fp32 products bound either kind of block, so what counts is how few rows
+    // the last tile wastes.  (Of more than 128 columns there is the first kind only.)
+    const bool f32 = type == AQ_T_F32;
+    j.many = rows > (f32 ? 96 : 32) || (f32 && D > 128);
     j.tiles = static_cast<int>(ceil_div(rows, j.many ? 128 : 32));
     const int64_t blocks = groups * j.tiles;
     // At least this many keys a part: fp32 products are slow enough for one
-    // tile (5 x 23 rows over 701 + 211 keys: 25 us, 30 with 128 keys a part,
-    // 61 with 512); 16-bit ones are not worth the joining.
-    const int64_t least = type == AQ_T_F32 ? 32 : 256;
+    // tile, or one of each wave's (3 x 111 rows over 333 keys: 19 us, 31 with 128
+    // keys a part, 60 with 512); 16-bit ones are not worth the joining.
+    const int64_t least = !f32 ? 256 : j.many ? 32 : 128;
     const int64_t most = std::min(most_parts, ceil_div(keys, least));
     j.splits = static_cast<int>(std::max<int64_t>(1, std::min(most, want / std::max<int64_t>(blocks, 1))));
     j.blocks = static_cast<int>(blocks * j.splits);
@@ -112,8 +115,11 @@ aq_status attend(aq_ctx *ctx, int type, args a) {
     a.rows = static_cast<int64_t>(a.B) * a.T * a.H;
     const int64_t part_bytes = a.rows * (a.D + 2) * 4, most_parts = std::max<int64_t>(kPartBytes / part_bytes, 1);
     // The streams' rows go over the prefix together where a stream alone would
-    // not fill a tile of rows; then its own keys are a part of their own.
-    const bool apart = a.P > 0 && a.B > 1 && per_stream < 64 && most_parts >= 2;
+    // not fill half a tile of rows; then its own keys are a part of their own.
+    // In us, alone and together: 16 streams over 8192 + 512 keys, bf16, 32 rows
+    // each 58, 53; 64 rows 101, 83; 80 rows 103, 115; 64 streams over 4096 + 600,
+    // 64 rows 104, 100; 80 rows 104, 117; fp32, 16 rows 112, 108; 32 rows 105, 197.
+    const bool apart = a.P > 0 && a.B > 1 && per_stream <= (type == AQ_T_F32 ? 16 : 64) && most_parts >= 2;
     int parts;
     // A compute unit holds two blocks.  A prefix's jobs share it with the own
     // keys', and each of its parts is written and joined: one block a unit, and

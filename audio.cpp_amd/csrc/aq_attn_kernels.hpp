@@ -698,7 +698,7 @@ __device__ inline void rows_body(const args &a, const job &j, const place &at, u
     close_rows<T, DP, kTile, DIRECT>(a, j.part + at.split, w, lds + wave * kTile);
 }
 
-// Few rows: 32 a block; each of its first WAVES waves takes every WAVES-th
+// Few rows (fp32: up to 96 of a stream): 32 a block; each of its first WAVES waves takes every WAVES-th
 // tile, with LDS of its own, and the waves' sums are joined in LDS, in the
 // waves' order.
 template <typename T, int DP, int WAVES, bool DIRECT>
