@@ -418,7 +418,8 @@ struct stager {
 
 // The same through registers, for a tile that one wave has to itself: the next
 // tile's pieces are on their way in registers while one is used.  Such keys are
-// read once, so they are the first to leave the caches: a prefix stays there
+// read once (in fp32 up to three times, by products far slower than memory), so
+// they are the first to leave the caches: a prefix stays there
 // (a token of 128 streams over 16384 + 1024 keys: 137 us with plain loads, 130
 // so; of 64 streams over 1500 keys, 61 and 55).
 template <typename T, int DP, int KT, bool DIRECT>
@@ -698,9 +699,9 @@ __device__ inline void rows_body(const args &a, const job &j, const place &at, u
     close_rows<T, DP, kTile, DIRECT>(a, j.part + at.split, w, lds + wave * kTile);
 }
 
-// Few rows (fp32: up to 96 of a stream): 32 a block; each of its first WAVES waves takes every WAVES-th
-// tile, with LDS of its own, and the waves' sums are joined in LDS, in the
-// waves' order.
+// Few rows (fp32: up to 96 of a stream): 32 a block; each of its first WAVES
+// waves takes every WAVES-th tile, with LDS of its own, and the waves' sums are
+// joined in LDS, in the waves' order.
 template <typename T, int DP, int WAVES, bool DIRECT>
 __device__ inline void keys_body(const args &a, const job &j, const place &at, unsigned char *lds) {
     using S = shape<T, DP>;

@@ -649,7 +649,7 @@ typedef struct aq_heads {
  *            streams), or NULL
  *   scale    above 0, below 1e38
  * D from 1 to 256, S up to 2^30, B * T * heads up to 2^30, and fewer than 2^24
- * blocks of 32 rows of one stream and key head (128 from 33 rows on).  Scores, sums and
+ * blocks of 32 rows of one stream and key head (128 from 97 rows on).  Scores, sums and
  * weights are fp32; with 16-bit types each p is rounded to the type before it
  * meets v, an F32 call is fp32 throughout.  The order of a row's sum depends
  * on the sizes and lengths alone, not on timing.  Calls of few rows use the context's
