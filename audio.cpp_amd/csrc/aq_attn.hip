@@ -300,7 +300,8 @@ aq_status aq_prefix_attention(aq_ctx *ctx, int type, int64_t B, int64_t T, int64
     a.G = a.H / a.Hkv;
     a.D = static_cast<int>(D);
     a.causal = 1;
-    a.direct = (S == 0 || (pieces(k, D, size) && pieces(v, D, size))) &&
+    // Rows of q and out go by whole pieces too, where there is no key at all as well.
+    a.direct = D * size % 16 == 0 && (S == 0 || (pieces(k, D, size) && pieces(v, D, size))) &&
                (P == 0 || (pieces(prefix_k, D, size) && pieces(prefix_v, D, size)));
     return attend(ctx, type, a);
 }

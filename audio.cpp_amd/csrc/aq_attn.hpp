@@ -33,7 +33,7 @@ struct args {
     float c;       // scale * log2(e)
     int B, T, S, P, H, Hkv, G, D;
     int causal;    // own keys up to the row's own
-    int direct;    // rows of keys and values start and end at 16 bytes
+    int direct;    // rows of keys and values start and end at 16 bytes, and any row is a whole number of such pieces
     job jobs[2];   // of the launch; the second may be empty
     // Parts that another launch joins (null: the launch writes `out`): sums
     // [part][row][D] and their references and weights [part][row][2], row =
