@@ -149,18 +149,24 @@ __global__ __launch_bounds__(ROWS * WAVES * 64) void i8_quantize_kernel(const ty
 
 // ---- the product ---------------------------------------------------------------
 
-// What the four columns from n on are scaled with; columns past the end repeat the last.
+// What the four columns from n on are scaled with; columns past the end repeat
+// the last.  wide: a sum (up to 2^31) times one of the scales may pass fp32's end.
 struct columns {
     float scale[4], bias[4];
+    bool wide;
 };
+
+constexpr float kWideScale = 0x1p96f;
 
 __device__ inline columns columns_of(const args &a, int n) {
     columns v;
+    v.wide = false;
 #pragma unroll
     for (int c = 0; c < 4; ++c) {
         const int at = min(n + c, a.N - 1);
         v.scale[c] = a.scale[at];
         v.bias[c] = a.bias ? a.bias[at] : 0.0f;
+        v.wide = v.wide || __builtin_fabsf(v.scale[c]) > kWideScale;
     }
     return v;
 }
@@ -171,9 +177,15 @@ __device__ inline void store4(const args &a, int m, int n, i32x4 sum, const colu
     const int most = min(4, a.N - n);
     float o[4];
 #pragma unroll
-    for (int c = 0; c < 4; ++c) {
-        o[c] = static_cast<float>(sum[c]) * v.scale[c] * xs;   // (the scales' product alone may be subnormal)
-        if (a.bias) o[c] += v.bias[c];
+    for (int c = 0; c < 4; ++c) o[c] = static_cast<float>(sum[c]) * v.scale[c] * xs;   // (the scales' product alone may be subnormal)
+    if (v.wide) {   // such a scale comes last: beyond fp32 before it is beyond after it
+#pragma unroll
+        for (int c = 0; c < 4; ++c)
+            if (__builtin_fabsf(v.scale[c]) > kWideScale) o[c] = static_cast<float>(sum[c]) * xs * v.scale[c];
+    }
+    if (a.bias) {
+#pragma unroll
+        for (int c = 0; c < 4; ++c) o[c] += v.bias[c];
     }
     const int64_t at = m * a.y_ld + n;
     if (a.y_type == AQ_T_F32) {

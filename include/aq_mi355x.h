@@ -615,6 +615,7 @@ aq_status aq_i8_upload(aq_ctx *ctx, int64_t out_features, int64_t in_features, c
  *   x_scale  device [M] for I8; NULL for the others
  *   y        device [M, out_features], row stride y_ld, y_type F32, F16 or BF16
  * The sums are exact; the conversion to fp32, the scaling and the bias round.
+ * A product within fp32's range has its value whichever of the scales is beyond 2^96.
  * A floating row of zeros has scale 0; one with a value that is not finite
  * gives a row of NaN.  A floating x, or one of more than 16 rows, is laid out
  * in the context's scratch first. */
