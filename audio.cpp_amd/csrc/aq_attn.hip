@@ -16,6 +16,7 @@ struct join_args {
     const int32_t *q_len;
     int64_t rows, batch, row, head;   // strides of out
     int T, H, D, parts;
+    float c;
 };
 
 // One wave a row: out = sum over parts of 2^(m_part - m) sums_part, over the
@@ -34,11 +35,10 @@ __global__ __launch_bounds__(256) void attn_join_kernel(join_args a) {
     for (int p = lane; p < a.parts; p += 64) m = fmaxf(m, a.ml[(p * a.rows + r) * 2]);
 #pragma unroll
     for (int d = 32; d; d >>= 1) m = fmaxf(m, __shfl_xor(m, d));
-    const float from = m == -INFINITY ? 0.0f : m;
     float l = 0.0f, o[4] = {};
     const auto add = [&](int p, auto load) {
         const int64_t row = p * a.rows + r;
-        const float by = __builtin_amdgcn_exp2f(a.ml[row * 2] - from);
+        const float by = aq_attn_impl::weight_of(a.ml[row * 2], m, a.c);
         l = __fmaf_rn(a.ml[row * 2 + 1], by, l);
         float v[4];
         load(a.sums + row * a.D, v);
@@ -159,7 +159,7 @@ aq_status attend(aq_ctx *ctx, int type, args a) {
                    : type == AQ_T_F16 ? aq_attn_impl::launch_f16(ctx, a)
                                       : aq_attn_impl::launch_bf16(ctx, a);
     if (st != AQ_OK || parts == 1) return st;
-    const join_args j{a.sums, a.ml, a.out, a.q_len, a.rows, a.so.batch, a.so.row, a.so.head, a.T, a.H, a.D, parts};
+    const join_args j{a.sums, a.ml, a.out, a.q_len, a.rows, a.so.batch, a.so.row, a.so.head, a.T, a.H, a.D, parts, a.c};
     if (type == AQ_T_F32) launch_join<aq_types::f32>(ctx, j);
     else if (type == AQ_T_F16) launch_join<aq_types::f16>(ctx, j);
     else launch_join<aq_types::bf16>(ctx, j);

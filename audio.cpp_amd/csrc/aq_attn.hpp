@@ -36,11 +36,23 @@ struct args {
     int direct;    // rows of keys and values start and end at 16 bytes, and any row is a whole number of such pieces
     job jobs[2];   // of the launch; the second may be empty
     // Parts that another launch joins (null: the launch writes `out`): sums
-    // [part][row][D] and their references and weights [part][row][2], row =
-    // (b T + t) H + h.
+    // [part][row][D] and their references (scores) and weights [part][row][2],
+    // row = (b T + t) H + h.
     float *sums, *ml;
     int64_t rows;   // B T H
 };
+
+// Whether a reference, given as the score that it is c times, is so large that
+// its rounding (by up to 2^-25 of it) is not small in an exponent.  Scores of
+// that size have been rounded by as much themselves.
+__device__ inline bool is_far(float score, float c) { return __builtin_fabsf(score * c) > 0x1p16f && score > -INFINITY; }
+
+// 2^(c (score - top)), what sums with one reference are multiplied by beside
+// those with a larger one; 0 for sums of nothing.
+__device__ inline float weight_of(float score, float top, float c) {
+    const float near = score * c - (top == -INFINITY ? 0.0f : top * c), far = (score - top) * c;
+    return __builtin_amdgcn_exp2f(is_far(top, c) ? far : near);
+}
 
 aq_status launch_f32(aq_ctx *ctx, const args &a);
 aq_status launch_f16(aq_ctx *ctx, const args &a);

@@ -7,6 +7,11 @@
 //   o = o 2^(m - m') + sum p v,  l = l 2^(m - m') + sum p,   out = o / l
 // with c = scale log2(e).  m' stays m while it would grow by no more than 5:
 // a p of up to 32 is as good as one of up to 1, and most tiles rescale nothing.
+// m is c times a score.  Its rounding shifts all exponents of a row alike, which
+// out does not see; where m is so large that the shift is not small beside 1
+// (or has no value in fp32), they are c (s - score) instead.  That path is one
+// branch of a tile (8 x 4096 rows over 1500 keys 449 -> 452 us, 16 x 512 over
+// 8192 + 512 569 -> 577).
 //
 // Both products have the keys' side as the first operand, so that every lane
 // works for one row: S^T = K Q^T has a row per column, the lane's own, with 16
@@ -89,6 +94,10 @@ __device__ inline uint32_t finite_bits(uint32_t v) {
     return ((v & kLow) == kLow ? 0u : v & 0xFFFFu) | ((v & kHigh) == kHigh ? 0u : v & 0xFFFF0000u);
 }
 
+// The lanes whose reference asks for the exponents of far ones: it is far, or
+// it is the first and may be -infinity by its product with c alone.
+__device__ inline uint64_t far_rows(float score, float c) { return __ballot(is_far(score, c) || (c > 1.0f && score == -INFINITY)); }
+
 // A piece of a row, elements at.. of D; zeros from D on, and where !use.
 template <typename T>
 __device__ inline u32x4 load_piece(const typename T::raw *row, int at, int D, bool use) {
@@ -117,9 +126,11 @@ struct row_state {
     u32x4 q[kQ];
     f32x16 o[DP / 32];
     float m, l;        // the row's; l holds the half's keys
+    float score;       // m = c score, rounded
     int b, t, h;       // the lane's row
     bool used;         // it exists
     int see;           // own keys that it sees
+    uint64_t far;      // far_rows() of the wave
 };
 
 template <typename T, int DP, bool DIRECT>
@@ -158,8 +169,9 @@ __device__ inline void open_rows(const args &a, int walk, int b0, int r, int hk,
     for (int d = 0; d < DP / 32; ++d)
 #pragma unroll
         for (int i = 0; i < 16; ++i) w.o[d][i] = 0.0f;
-    w.m = -INFINITY;
+    w.m = w.score = -INFINITY;
     w.l = 0.0f;
+    w.far = far_rows(w.score, a.c);
 }
 
 // Steps of a chain of products whose operands come from LDS: kAhead of them are
@@ -310,15 +322,28 @@ __device__ inline void add_tile(const unsigned char *lk, const unsigned char *lv
     // The sums' reference moves only when a row's maximum has outgrown it by
     // 2^kSlack: until then the weights are that much above 1 at most.
     // (Row by row: a row's result does not depend on its neighbours'.)
-    const bool grown = top * c > w.m + kSlack;
-    if (__ballot(grown) != 0) {
-        const float keep = grown ? __builtin_amdgcn_exp2f(w.m - top * c) : 1.0f;
+    bool grown = top * c > w.m + kSlack;
+    if ((__ballot(grown) | w.far) != 0) {
+        if (is_far(w.score, c) || w.score == -INFINITY) grown = (top - w.score) * c > kSlack;
+        const float keep = grown ? weight_of(w.score, top, c) : 1.0f;
+        w.score = grown ? top : w.score;
         w.m = grown ? top * c : w.m;
         w.l *= keep;
 #pragma unroll
         for (int d = 0; d < DP / 32; ++d) w.o[d] *= keep;
+        w.far = far_rows(w.score, c);
     }
-    w.l += add_values<T, DP, NT>(lv, s, c, (w.m == -INFINITY ? 0.0f : w.m) - kShift, w);
+    float from = (w.m == -INFINITY ? 0.0f : w.m) - kShift;
+    if (__builtin_expect(w.far != 0, 0)) {   // out of line; the exponents themselves, by distance where the row's reference is far
+        const bool far = is_far(w.score, c);
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) s[n][i] = far ? __fmaf_rn(s[n][i] - w.score, c, kShift) : __fmaf_rn(s[n][i], c, -from);
+        c = 1.0f;
+        from = 0.0f;
+    }
+    w.l += add_values<T, DP, NT>(lv, s, c, from, w);
     if (NT > 1) __builtin_amdgcn_s_setprio(0);
 }
 
@@ -599,7 +624,7 @@ __device__ inline void close_rows(const args &a, int part, row_state<T, DP> &w, 
     static_assert(32 * kCols * 4 <= BYTES, "the columns of a turn fit");
     const int lane = threadIdx.x & 63, half = lane >> 5, col = lane & 31;
     const int64_t start = row_start<T, DP>(a, part, w);
-    if (half == 0) put_ml(a, start, w.m, w.l);
+    if (half == 0) put_ml(a, start, w.score, w.l);
     const float by = share_of(a, w.l);
 #pragma unroll
     for (int turn = 0; turn < kTurns; ++turn) {
@@ -750,17 +775,16 @@ __device__ inline void keys_body(const args &a, const job &j, const place &at, u
             if (tile >= mixed) add_odd(a, walk, tile * KT, (tile + 1) * KT, KT, w);
     w.l += __shfl_xor(w.l, 32);
     if (wave < WAVES && lane < 32) {
-        ml[wave][0][lane] = w.m;
+        ml[wave][0][lane] = w.score;
         ml[wave][1][lane] = w.l;
     }
     __syncthreads();   // (the tiles are not used any more either)
     float m = -INFINITY, l = 0.0f;
 #pragma unroll
     for (int i = 0; i < WAVES; ++i) m = fmaxf(m, ml[i][0][lane & 31]);
-    const float from = m == -INFINITY ? 0.0f : m;
 #pragma unroll
-    for (int i = 0; i < WAVES; ++i) l = __fmaf_rn(ml[i][1][lane & 31], __builtin_amdgcn_exp2f(ml[i][0][lane & 31] - from), l);
-    const float keep = __builtin_amdgcn_exp2f(w.m - from);
+    for (int i = 0; i < WAVES; ++i) l = __fmaf_rn(ml[i][1][lane & 31], weight_of(ml[i][0][lane & 31], m, a.c), l);
+    const float keep = weight_of(w.score, m, a.c);
     f32x16 *const red = reinterpret_cast<f32x16 *>(lds);   // [WAVES][DP / 32][64]
     if (wave < WAVES) {
 #pragma unroll

@@ -33,3 +33,51 @@ def test_no_key_at_all(ctx, t, D, T):
         for b in range(B):
             want[b, :rows[b], :, :D] = 0
         assert torch.equal(around, want)
+
+
+FAR = {"f16": (4096.0, 2.0 ** 6), "bf16": (2.0 ** 24, 2.0 ** 18), "f32": (2.0 ** 24, 2.0 ** 8)}
+
+
+@pytest.mark.parametrize("t", TYPES)
+@pytest.mark.parametrize("sign", [1, -1])
+@pytest.mark.parametrize("scale", [2.0 ** -8, 1.0, 5.0, 1e37])
+@pytest.mark.parametrize("B,T,P,S,D", [(1, 1, 0, 300, 64), (3, 5, 300, 40, 64), (2, 70, 90, 130, 128), (1, 1, 3000, 20, 128),
+                                       (2, 140, 0, 300, 256)])
+def test_scores_far_from_zero(ctx, t, sign, scale, B, T, P, S, D):
+    """Scores of 2^30 (f16) and 2^54, exact in fp32, whose own rounding is far above what a weight may be off by: keys
+    that are alike share the weight, and one that stands out takes all of it; at a scale of 1e37 the scores' products
+    with it are beyond fp32."""
+    size, step = FAR[t]
+    H, Hkv, far = 4, 2, -1 if sign < 0 else 1
+    kw = dict(dtype=TYPES[t], device="cuda")
+    q = torch.full((B, T, H, D), size, **kw)
+    k, pk = torch.full((B, S, Hkv, D), sign * size, **kw), torch.full((P, Hkv, D), sign * size, **kw)
+    v, pv = torch.zeros((B, S, Hkv, D), **kw), torch.zeros((P, Hkv, D), **kw)
+    v[:], pv[:] = torch.arange(S, device="cuda").remainder(8)[:, None, None], torch.arange(P, device="cuda").remainder(8)[:, None, None]
+    u = {"f32": 0.0, "f16": 2.0 ** -11, "bf16": 2.0 ** -8}[t]
+    own = S - T   # keys that every row sees
+    out = torch.empty_like(q)
+
+    def check(alone):
+        """What each row gets: the mean over the keys that it sees, or the value of the one that stands out."""
+        aqmi.prefix_attention(ctx, q, pk, pv, k, v, out, scale=scale)
+        for i in sorted({0, T // 2, T - 1}):
+            seen = torch.cat((pv.double(), v[0, :own + i + 1].double()))[:, 0, 0]
+            want = (seen.mean() if alone is None else torch.tensor(float(alone))).item()
+            # each rounding of a weight and of the output, and S + P fp32 additions to either sum
+            assert bool(((out[:, i].double() - want).abs() <= want * (2 * u + (S + P) * 2.0 ** -22) + 1e-6).all()), i
+        if P == 0 and T == 1:   # the same keys without an order
+            crossed = torch.empty_like(q)
+            aqmi.cross_attention(ctx, q, k, v, crossed, scale=scale)
+            assert torch.equal(crossed, out)
+
+    check(None)
+    at = own // 3
+    k[:, at] = sign * size + step   # the largest of all scores, by 2^24 and more
+    v[:, at] = 5
+    check(5)
+    k[:, at] = sign * size
+    k[:, :own] = sign * size - step   # far below the others: rows that see those give these nothing
+    pk[:] = sign * size - step
+    v[:, own:] = 3
+    check(3)
