@@ -65,7 +65,8 @@ class CodeLayer:
         aqmi.add_rmsnorm(self.ctx, block, self.norm, 1e-6, residual=stream, sum=stream, q=self.q, scale=self.q_scale)
 
     def step(self, stream, block):
-        """One token of each stream; the block's output, not yet added to the stream."""
+        """One token of each stream (of TOKENS at most: `len` is on the device and not looked at here); the block's
+        output, not yet added to the stream."""
         self.normalised(stream, block)
         self.qkv.forward(self.q, self.heads.view(self.streams, -1), self.q_scale)
         at = self.len.long()
@@ -83,6 +84,8 @@ class CodeLayer:
 
 
 def main(streams: int = 4, steps: int = 8) -> None:
+    if steps > TOKENS:
+        raise ValueError(f"{steps} steps: a stream's caches hold {TOKENS} tokens")
     g = torch.Generator(device="cuda").manual_seed(0)
     ctx = aqmi.Context(0)
     layer, head = CodeLayer(ctx, streams), CodeStep(ctx, streams)
