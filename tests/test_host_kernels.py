@@ -1,4 +1,4 @@
-"""Which kernels attention takes, against a HIP runtime that runs none
+"""Which kernels a layer's operators take, against a HIP runtime that runs none
 (tests/cpp/host_kernels.cpp), so without a GPU."""
 
 import pathlib
@@ -9,7 +9,7 @@ import pytest
 BIN = pathlib.Path(__file__).resolve().parent / "cpp" / "host_kernels"
 
 
-def test_whole_pieces_only_where_rows_are_whole():
+def test_whole_pieces_only_where_rows_are_whole_and_the_kernels_that_the_tests_reach():
     if not BIN.exists():
         pytest.skip("tests/cpp/host_kernels not built (run __graft_entry__.build())")
     r = subprocess.run([str(BIN)], capture_output=True, text=True, timeout=60)
