@@ -27,16 +27,18 @@
 // the keys averages); an f16 p is 2^10 times the weight, so that small weights
 // are not lost below its range.  fp32 inputs keep fp32 products throughout.
 //
-// What bounds it.  Many rows: 860 to 990 TFLOP/s (8 x 4096 rows of 16 heads over
-// 1500 keys in 449 us, 16 x 512 rows over a prefix of 8192 in 572), where a
+// What bounds it.  Many rows: 870 to 980 TFLOP/s (8 x 4096 rows of 16 heads over
+// 1500 keys in 452 us, 16 x 512 rows over a prefix of 8192 in 577), where a
 // large product of the library's reaches 1110 to 1270: the matrix instructions
 // 45 % of the clocks and the vector instructions (two thirds of them for the
 // exponentials) 51 %, on two waves a SIMD (227 registers) that
 // cover each other's waits.  Few rows, the keys' way from memory: 64 streams over
 // 1500 keys, 266 MB, 55 us (4.8 TB/s).  Both at once, a token of 128 streams
-// over 16384 shared and up to 1024 own keys: 122 us, of which the own keys'
-// 368 MB take 75 and the prefix 49 alone; side by side they gain little, as the
-// prefix's four row tiles read it again past what the own keys leave of the caches.
+// over 16384 shared and up to 1024 own keys: 122 us with the joining, where the
+// own keys' 368 MB take 72 alone and the prefix 44, in a launch of its kind of
+// blocks.  Side by side they gain nothing, and not for want of caches: 451 MB
+// are fetched, as by both alone, and three of four reads of the prefix hit.  In
+// the launch for both kinds the prefix takes 69 beside own blocks without a key.
 //
 // A key that a row does not see is never multiplied into it: its score is
 // -infinity whatever the product gave, keys that no row of the tile sees are

@@ -8,9 +8,11 @@
 // has the same layout, by 16 rows of x.
 //
 // What bounds it.  Few rows of x, the weights' way from memory: 64 x 8192 x
-// 16384, 134 MB, 27 us (5.0 TB/s; 36 with bringing bf16 rows to 8 bits).  Many
+// 16384, 134 MB, 26 us (5.1 TB/s; 36 with bringing bf16 rows to 8 bits).  128
+// rows of that size take 44 us: W is read once for 64 of them.  Many
 // rows, the matrix instructions: 16384 x 8192 x 8192 in 1.04 ms, 2.1 POP/s, as
-// fast as the library's product of whole numbers.  One row of 1024 x 1536: 3 us
+// fast as the library's product of whole numbers (bf16 rows 1.17 ms: bringing
+// them to 8 bits reads them twice, at half the rate of a copy).  One row of 1024 x 1536: 3 us
 // in the kernel, latency of the loads, of the join and of the launch.
 //
 // The sums are whole numbers of 32 bits (in_features below 2^17, so that
@@ -416,10 +418,13 @@ enum how : int { kLarge, kMedium, kSplit };
 
 // A block of a size is taken where its tiles give three of four compute units
 // one, or where there are so few k-blocks that splitting them gains nothing.
-// In us, 8-bit x, large, medium, split:
-//   K = 4096, N = 4096:    M = 512: 54, 25, 21;    1024: 56, 27, 36;   4096: 75, 111, 120
-//   K = 8192, N = 16384:   M = 128: 97, 43, 38;     200: 97, 48, 67;   1024: 143, 200, 219
-//   K = 1024, N = 1536:    M = 128: 21, 9.9, 11.7; 4096: 25, 19, 28
+// In us, 8-bit x, large, medium, split, with weights that come from memory
+// (matrices in turn, more than the caches hold):
+//   K = 4096, N = 4096:    M = 512: 57, 27, 22;   1024: 56, 29, 36;   4096: 71, 98, 115
+//   K = 8192, N = 16384:   M = 128: 94, 56, 44;    200: 101, 51, 69;  1024: 132, 196, 228
+//   K = 1024, N = 1536:    M = 128: 21, 11, 9;    4096: 25, 18, 28
+// and with the same matrix again: 53, 24, 20; 54, 27, 33; 71, 89, 113; 93, 42,
+// 37; 94, 49, 64; 119, 172, 221; 20, 9.4, 9.5; 25, 19, 28.
 how how_of(const aq_ctx *ctx, const args &a) {
     const int64_t large = int64_t{(a.tiles + 15) / 16} * ((a.M + 255) / 256);
     const int64_t medium = int64_t{(a.tiles + 7) / 8} * ((a.M + 127) / 128);
@@ -438,9 +443,9 @@ aq_status launch_product(aq_ctx *ctx, const args &a, how h) {
         if (a.M <= 16) return launch<true, 1, 1, 4>(ctx, a, 8);
         // Four tiles by 64 rows read the weights once for them, where there are
         // enough such blocks; in us, two tiles by 32 rows and these with eight and
-        // with four waves: 64 x 8192 x 16384, packing
-        // included, 47, 35, 40; 128 rows 83, 58, 47;
-        // 64 x 4096 x 4096 11.6, 12.3, 14.5; 64 x 8192 x 2048 11.5, 17, 22.
+        // with four waves, packing included, weights from memory: 64 x 8192 x
+        // 16384 46, 34, 37; 128 rows 81, 56, 44; 64 x 4096 x 4096 10.5, 15, 18;
+        // 64 x 8192 x 2048 14, 23, 29.
         const int64_t blocks = int64_t{(a.tiles + 3) / 4} * ((a.M + 63) / 64);
         if (a.M <= 32 || blocks < ctx->num_cus) return launch<true, 2, 2, 2>(ctx, a, 8);
         return launch<true, 4, 4, 1>(ctx, a, a.M <= 64 ? 8 : 4);

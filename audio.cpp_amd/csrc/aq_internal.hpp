@@ -25,8 +25,9 @@ struct aq_ctx {
     // exact scan takes, 7: largest logits and candidates of sampled rows,
     // 8: rows of x in operand order, 9: an attention's parts).
     static constexpr int kScratchSlots = 10;
-    // Slots from here on (tens of MB, for an attention's parts up to 256, and
-    // more for rows of millions of columns) at least double when they grow, where the memory is there, and
+    // Slots from here on (tens of MB, up to 256 MiB for an attention's parts, and
+    // more for rows of millions of columns) at least double when they grow, where
+    // the memory is there (so a buffer may be nearly twice what calls asked), and
     // leave the buffers that they outgrow allocated until the context ends: a
     // captured graph of a call goes on using its own.
     static constexpr int kFirstKept = 7;

@@ -616,7 +616,8 @@ aq_status aq_i8_upload(aq_ctx *ctx, int64_t out_features, int64_t in_features, c
  *   y        device [M, out_features], row stride y_ld, y_type F32, F16 or BF16
  * The sums are exact; the conversion to fp32, the scaling and the bias round.
  * A product within fp32's range has its value whichever of the scales is beyond 2^96.
- * A floating row of zeros has scale 0; one with a value that is not finite
+ * A floating row of zeros has scale 0 (and a scale below 2^-126 keeps fewer
+ * bits); one with a value that is not finite
  * gives a row of NaN.  A floating x, or one of more than 16 rows, is laid out
  * in the context's scratch first. */
 aq_status aq_i8_forward(aq_ctx *ctx, const aq_i8 *w, int x_type, const void *x, int64_t x_ld, const float *x_scale,
@@ -636,7 +637,10 @@ typedef struct aq_heads {
  *   out[b, t, h] = sum_j p[j] v[b, j, g] / sum_j p[j],  p[j] = exp(scale * q[b, t, h] . k[b, j, g]),
  * over the keys j < kv_len[b] with mask[b, j] != 0, where g = h / (heads /
  * kv_heads).  What lies in keys that are left out does not matter, NaN
- * included.  A row without a key (or whose scores are all -infinity) is 0.
+ * included.  A row without a key (or whose scores are all -infinity) is 0.  An
+ * infinite value makes its column of a row that sees it infinite (or NaN, where
+ * its weight vanishes), a NaN makes it NaN; a score of +infinity or NaN makes
+ * the whole row NaN.
  *   type     F32, F16 or BF16: q, k, v and out
  *   q, out   device, [B, T, heads, D]; rows of out must not overlap.  out may
  *            be q with the same strides, and else none of the inputs.
@@ -650,11 +654,14 @@ typedef struct aq_heads {
  *            streams), or NULL
  *   scale    above 0, below 1e38
  * D from 1 to 256, S up to 2^30, B * T * heads up to 2^30, and fewer than 2^24
- * blocks of 32 rows of one stream and key head (128 from 97 rows on).  Scores, sums and
+ * blocks: a stream's rows of one key head go by 32, or by 128 where they are
+ * more than 32 (F32: more than 96, and always where D > 128).  Scores, sums and
  * weights are fp32; with 16-bit types each p is rounded to the type before it
- * meets v, an F32 call is fp32 throughout.  The order of a row's sum depends
- * on the sizes and lengths alone, not on timing.  Calls of few rows use the context's
- * scratch. */
+ * meets v, an F32 call is fp32 throughout.  The sums are formed before they are
+ * divided, of weights up to 32: F32 and BF16 values above 1e37 over their
+ * number of keys may take them beyond fp32.  The order of a row's sum depends
+ * on the sizes and lengths alone, not on timing.  Calls of few rows use the
+ * context's scratch. */
 aq_status aq_cross_attention(aq_ctx *ctx, int type, int64_t B, int64_t T, int64_t S, int64_t heads, int64_t kv_heads, int64_t D,
                              aq_heads q, aq_heads k, aq_heads v, const int32_t *q_len, const int32_t *kv_len,
                              const uint8_t *mask, int64_t mask_ld, float scale, aq_heads out);
@@ -662,7 +669,8 @@ aq_status aq_cross_attention(aq_ctx *ctx, int type, int64_t B, int64_t T, int64_
 /* Causal attention of B streams that share a prefix of P keys (the same
  * formula): row t of stream b, with n = q_len[b] rows and m = kv_len[b] own
  * keys, sees all of the prefix and its own keys j <= m - n + t; the last n own
- * keys are the rows' own.  The prefix is read for all streams together.
+ * keys are the rows' own.  Streams of up to 64 rows of a key head (F32: 16) go
+ * over the prefix together; longer ones read it each.
  *   prefix_k, prefix_v  device, [P, kv_heads, D] (batch_ld is not looked at)
  *   k, v                device, [B, S, kv_heads, D]: the streams' own keys, of
  *                       which kv_len[b] are in use (NULL: S)
