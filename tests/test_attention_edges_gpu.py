@@ -81,3 +81,38 @@ def test_scores_far_from_zero(ctx, t, sign, scale, B, T, P, S, D):
     pk[:] = sign * size - step
     v[:, own:] = 3
     check(3)
+
+
+def test_two_contexts_at_once():
+    """Calls of two contexts on two streams, side by side on the device, each with parts in its own scratch."""
+    g = torch.Generator().manual_seed(9)
+    made = lambda *s: torch.randn(s, generator=g).bfloat16().cuda()
+    work, streams = [], [torch.cuda.Stream() for _ in range(2)]
+    for B, P, S in ((40, 3000, 300), (3, 9000, 500)):
+        q, k, v, pk, pv = made(B, 1, 8, 128), made(B, S, 2, 128), made(B, S, 2, 128), made(P, 2, 128), made(P, 2, 128)
+        alone = torch.empty_like(q)
+        context = aqmi.Context(0)
+        aqmi.prefix_attention(context, q, pk, pv, k, v, alone)
+        work.append((context, (q, pk, pv, k, v), alone, [torch.empty_like(q) for _ in range(20)]))
+    torch.cuda.synchronize()
+    for i in range(20):
+        for stream, (context, inputs, _, outs) in zip(streams, work):
+            with torch.cuda.stream(stream):
+                aqmi.prefix_attention(context, *inputs, outs[i])
+    torch.cuda.synchronize()
+    for _, _, alone, outs in work:
+        assert all(torch.equal(out, alone) for out in outs)
+
+
+@pytest.mark.parametrize("t", TYPES)
+@pytest.mark.parametrize("T", [1, 40, 150])
+def test_subnormal_values(ctx, t, T):
+    """The mean of equal values is that value: the weights' rounding is less than half a step of a 16-bit type's subnormal
+    values; in f32 each of 300 products with a weight rounds to a multiple of 2^-149."""
+    g = torch.Generator().manual_seed(T)
+    for value in {"f16": (2.0 ** -24, 2.0 ** -15), "bf16": (2.0 ** -133, 2.0 ** -127), "f32": (2.0 ** -130, 2.0 ** -127)}[t]:
+        q, k = (torch.randn((2, n, 2, 64), generator=g).to(TYPES[t]).cuda() for n in (T, 300))
+        v, out = torch.full_like(k, value), torch.empty_like(q)
+        aqmi.cross_attention(ctx, q, k, v, out)
+        allowed = 300 * 2.0 ** -149 if t == "f32" else 0.0
+        assert bool(((out.double() - value).abs() <= allowed).all())

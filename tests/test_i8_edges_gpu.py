@@ -65,3 +65,37 @@ def test_small_rows_with_large_weights(ctx, M):
     assert np.abs(np.abs(xd * 127 / most - np.floor(xd * 127 / most)) - 0.5).min() > 1e-9
     ref = (q @ codes.astype(np.float64).T) * (most / 127) * scale.astype(np.float64)
     near(y, ref, ref)
+
+
+@pytest.mark.parametrize("t", ["i8", "bf16"])
+@pytest.mark.parametrize("M", [16, 40, 140])
+def test_rows_farther_apart_than_32_bits(ctx, t, M):
+    """The last rows of x and of y start past 2^32 bytes and 2^32 elements; the results are those of rows next to each other."""
+    step, K, N = -(-(1 << 32) // (M - 1) // 16) * 16 + 16, 208, 270
+    r = np.random.default_rng(M)
+    lin = aqmi.I8Linear(ctx, r.integers(-128, 128, (N, K), dtype=np.int8), np.full(N, 1e-3, np.float32))
+    g = torch.Generator().manual_seed(M)
+    x, s = torch.randint(-128, 128, (M, K), generator=g, dtype=torch.int8).cuda(), torch.rand(M, generator=g).cuda()
+    if t != "i8":
+        x, s = x.bfloat16(), None
+    near_y = torch.empty((M, N), dtype=torch.bfloat16, device="cuda")
+    lin.forward(x, near_y, s)
+    far_x = torch.empty(M * step, dtype=x.dtype, device="cuda").view(M, step)[:, :K]
+    far_x.copy_(x)
+    far_y = torch.empty(M * step, dtype=torch.bfloat16, device="cuda").view(M, step)[:, :N]
+    lin.forward(far_x, far_y, s)
+    assert torch.equal(far_y, near_y)
+
+
+def test_results_past_32_bits(ctx):
+    """600000 rows of 4096 columns: 2.4 G results, of large blocks."""
+    M, K, N = 600000, 64, 4096
+    r = np.random.default_rng(1)
+    lin = aqmi.I8Linear(ctx, r.integers(-128, 128, (N, K), dtype=np.int8), np.full(N, 1e-3, np.float32))
+    x = torch.randint(-128, 128, (1000, K), generator=torch.Generator().manual_seed(1), dtype=torch.int8).cuda().repeat(M // 1000, 1)
+    s = torch.full((M,), 0.5, device="cuda")
+    y = torch.empty((M, N), dtype=torch.bfloat16, device="cuda")
+    lin.forward(x, y, s)
+    want = torch.empty((1000, N), dtype=torch.bfloat16, device="cuda")
+    lin.forward(x[:1000], want, s[:1000])
+    assert bool((y.view(-1, 1000, N) == want).all())
